@@ -111,6 +111,9 @@ _SIGNATURES = {
                            c_float, c_int, c_float, c_float, c_float, P, c_longlong, P, P],
     "esp_attn_decode_diff": [P, P, P, P, P, P, P, P, P, P, P, c_int, c_int, c_int, c_int, c_int, c_int, c_int, c_int, c_int,
                              c_int, c_int, c_float, c_int, c_float, c_float, c_float, c_float, P, c_longlong, P, P],
+    "esp_kv8_append": [P, P, P, P, P, P, c_int, c_int, P, P, P, P, P, c_int, c_int, c_int, c_int, c_int, c_int, c_int, P, P],
+    "esp_attn_decode_kv8": [P, P, P, P, P, P, P, P, P, P, P, P, c_int, c_int, c_int, c_int, c_int, c_int, c_int, c_int, c_int, P, P],
+    "esp_attn_run_kv8": [P, P, P, P, P, P, P, P, P, P, c_int, c_int, c_int, c_int, c_int, c_int, c_int, P, P],
 }
 
 _bound: dict = {}
@@ -1521,3 +1524,145 @@ def pair_rope_unitnorm_kvwrite(qkv, bias, inv_freq, rot, eps, unit_norm, v_share
         _ptr(k_cache, q_out.dtype, "k_cache"), _ptr(v_cache, q_out.dtype, "v_cache"), _is_bf16(q_out),
         _ptr(block_table, torch.int32), block_table.shape[1], k_cache.shape[0], page, qkv.shape[0], nh, nkv, hd, vd,
         1 if write_kv else 0, _ptr(status, torch.int32), _stream()), "pair_rope_unitnorm_kvwrite")
+
+
+# ---------------------------------------------------------------- the 8-bit key/value cache
+# A row (the key or the value of one position and one key/value head) is kept as hd e4m3 numbers times a power of two 2^e,
+# e the smallest whole number from -100 on with max |x| <= 448 * 2^e.  Pools: codes float8_e4m3fn [pages, nkv, 64, hd] of
+# keys and of values, exponents uint8 [pages, nkv, 2, 64] (e + 127; of keys, then of values), so that a row is
+# codes.float() * 2.0 ** (exponent - 127).  A row with a NaN, an infinity or a magnitude above 448 * 2^100 is kept as the
+# exponent 255: what attends to it is NaN.
+KV8_PAGE = 64
+_E4M3 = torch.float8_e4m3fn
+
+
+def kv8_fits(hd: int, page: int = KV8_PAGE) -> bool:
+    """Head and page sizes that the 8-bit cache's kernels take."""
+    return hd % 8 == 0 and 0 < hd <= 256 and page == KV8_PAGE
+
+
+@functools.lru_cache(maxsize=64)
+def _sm_count(device: int) -> int:
+    return torch.cuda.get_device_properties(device).multi_processor_count
+
+
+def _kv8_check(what, q, k, v, exps, block_table, page, nh, nkv, hd, vectors):
+    """What the three entry points refuse alike; ``vectors``: (name, tensor or None, least length)."""
+    if nh <= 0 or nkv <= 0 or nh % nkv or nh > 65535:
+        raise Backend(f"{what}: {nh} query heads do not divide among {nkv} key/value heads")
+    if not kv8_fits(hd, page):
+        raise Backend(f"{what}: heads of {hd} channels in pages of {page}; they are multiples of 8 up to 256 in pages of {KV8_PAGE}")
+    if q.dim() < 2 or q.numel() != q.shape[0] * nh * hd:
+        raise Backend(f"{what}: queries of shape {tuple(q.shape)} are not rows of {nh} heads of {hd}")
+    if k is not None:
+        if k.dim() != 4 or tuple(k.shape[1:]) != (nkv, page, hd) or v.shape != k.shape:
+            raise Backend(f"{what}: pools of shape {tuple(k.shape)} and {tuple(v.shape)} are not [pages, {nkv}, {page}, {hd}]")
+        if tuple(exps.shape) != (k.shape[0], nkv, 2, page):
+            raise Backend(f"{what}: exponents of shape {tuple(exps.shape)} are not [pages, {nkv}, 2, {page}]")
+        if block_table.dim() != 2:
+            raise Backend(f"{what}: the page table has {block_table.dim()} dimensions, not [sequences, pages]")
+    for name, t, least in vectors:
+        if t is not None and t.numel() < least:
+            raise Backend(f"{what}: {name} has {t.numel()} elements, {least} are needed")
+    for name, t, step in (("queries", q, 16), ("keys", k, 16), ("values", v, 16), ("exponents", exps, 4)):
+        if t is not None and t.data_ptr() % step:
+            raise Backend(f"{what}: the {name} do not start on a multiple of {step} bytes")
+    if not q.is_cuda:
+        raise Backend(f"{what}: queries must live on the GPU; this library has no CPU path")
+    _stream()
+    if q.get_device() != torch.cuda.current_device() or q.get_device() != _device_index:
+        raise Backend(f"{what}: the queries live on {q.device}, kernels are launched on cuda:{_device_index}")
+
+
+def kv8_rope_append(qkv, bias, tok_seq, tok_pos, cos, sin, rot, q_out, k, v, exps, block_table, page, nh, nkv, hd, write_kv, status):
+    """Adds the bias, rotates queries and keys over their first ``rot`` channels (split-half, 32-bit, tables
+    [positions, rot / 2]; ``rot`` 0: no rotation) and stores keys and values as rows of the 8-bit cache, each rounded once.
+    qkv float32 [N, (nh + 2 nkv) hd]; q_out bfloat16 [N, nh * hd].  ``write_kv`` false: queries alone, the pools may be None.
+    A row whose position has no page is left out and the status says so.  Two tokens of a call must not share a position."""
+    n = qkv.shape[0]
+    if qkv.dim() != 2 or qkv.shape[1] != (nh + 2 * nkv) * hd:
+        raise Backend("kv8_rope_append: qkv width disagrees with the head counts")
+    if rot < 0 or rot > hd or rot % 2:
+        raise Backend(f"kv8_rope_append: {rot} rotated channels of heads of {hd}")
+    if write_kv and k is None:
+        raise Backend("kv8_rope_append: no pools to write keys and values to")
+    if q_out.shape[0] != n:
+        raise Backend(f"kv8_rope_append: {q_out.shape[0]} rows for the queries of {n} tokens")
+    if rot and (cos is None or sin is None or cos.shape != sin.shape or cos.dim() != 2 or cos.shape[1] != rot // 2):
+        raise Backend(f"kv8_rope_append: cosines and sines are not [positions, {rot // 2}]")
+    if n == 0:
+        return
+    _kv8_check("kv8_rope_append", q_out, k if write_kv else None, v, exps, block_table, page, nh, nkv, hd,
+               (("the bias", bias, qkv.shape[1]), ("tok_seq", tok_seq, n), ("tok_pos", tok_pos, n)))
+    _check(_fn("kv8", "esp_kv8_append")(
+        _ptr(qkv, torch.float32, "qkv"), _ptr(bias, torch.float32, "bias"), _ptr(tok_seq, torch.int32, "tok_seq"),
+        _ptr(tok_pos, torch.int32, "tok_pos"), _ptr(cos, torch.float32, "cos") if rot else None, _ptr(sin, torch.float32, "sin") if rot else None,
+        rot, cos.shape[0] if rot else 0, _ptr(q_out, torch.bfloat16, "q_out"), _ptr(k, _E4M3, "keys") if write_kv else None,
+        _ptr(v, _E4M3, "values") if write_kv else None, _ptr(exps, torch.uint8, "exponents") if write_kv else None,
+        _ptr(block_table, torch.int32, "page table") if write_kv else None, block_table.shape[1] if write_kv else 0,
+        k.shape[0] if write_kv else 0, n, nh, nkv, hd, 1 if write_kv else 0, _ptr(status, torch.int32, "status"), _stream()),
+        "kv8_rope_append")
+
+
+@functools.lru_cache(maxsize=4096)
+def attn_decode_kv8_split(n_rows: int, kv_blocks: int, positions: int, sm_count: int = 148) -> int:
+    """Key positions a block of ``attn_decode_kv8``, whole pages of 64, the same for every row of the step."""
+    pages, room = max(1, (positions + 63) // 64), 2 * sm_count
+    pairs = max(1, n_rows * kv_blocks)
+    parts = max(1, min(pages // 4, room // pairs))
+    return 64 * ((pages + parts - 1) // parts)
+
+
+def attn_decode_kv8(q, k, v, exps, out, ws, tok_seq, tok_pos, block_table, page, nh, nkv, hd, window, status, seq_past=None):
+    """Attention of one token row per sequence (or of any rows, each on its own) over the 8-bit cache, split over the keys:
+    scores over sqrt(hd), keys max(0, pos - window + 1) .. pos (``window`` None or 0: all).  q and out bfloat16 [N, nh * hd];
+    query head i reads key/value head i // (nh / nkv).  ``ws``: the ``Workspace`` that holds the scratch; calls that may
+    overlap on the device (other streams, captured graphs replayed beside each other) need one each.  ``seq_past``
+    (int32 per sequence of the step: positions that were cached before the step's copies to the device): blocks whose
+    keys are all older load them without waiting for the kernel before this one."""
+    n = q.shape[0]
+    if out.numel() != q.numel():
+        raise Backend(f"attn_decode_kv8: {tuple(out.shape)} for the results of queries {tuple(q.shape)}")
+    if window is not None and window < 0:
+        raise Backend(f"attn_decode_kv8: a window of {window} positions")
+    if n == 0:
+        return
+    _kv8_check("attn_decode_kv8", q, k, v, exps, block_table, page, nh, nkv, hd,
+               (("tok_seq", tok_seq, n), ("tok_pos", tok_pos, n), ("seq_past", seq_past, block_table.shape[0])))
+    positions = block_table.shape[1] * page
+    group = nh // nkv
+    split = attn_decode_kv8_split(n, nkv * ((group + 15) // 16), min(positions, window + page) if window else positions, _sm_count(_device_index))
+    n_splits = max(1, (positions + split - 1) // split)
+    part_o = part_ml = counters = None
+    if n_splits > 1:
+        part_o = ws.get("attn_kv8_part_o", (n, nh, n_splits, hd), torch.float32)
+        part_ml = ws.get("attn_kv8_part_ml", (n, nh, n_splits, 2), torch.float32)
+        counters = ws.get("attn_kv8_counters", (n * nh,), torch.int32, zeroed=True)
+    _check(_fn("kv8", "esp_attn_decode_kv8")(
+        _ptr(q, torch.bfloat16, "q"), _ptr(k, _E4M3, "keys"), _ptr(v, _E4M3, "values"), _ptr(exps, torch.uint8, "exponents"),
+        _ptr(out, torch.bfloat16, "out"), _ptr(part_o), _ptr(part_ml), _ptr(counters), _ptr(tok_seq, torch.int32, "tok_seq"),
+        _ptr(tok_pos, torch.int32, "tok_pos"), _ptr(seq_past, torch.int32, "seq_past"), _ptr(block_table, torch.int32, "page table"),
+        block_table.shape[1], k.shape[0], n, nh, nkv, hd, int(window or 0), split, n_splits, _ptr(status, torch.int32, "status"), _stream()),
+        "attn_decode_kv8")
+
+
+def attn_prefill_kv8(q, k, v, exps, out, tile_seq, tile_first, seq_start, seq_past, block_table, page, nh, nkv, hd, window, status):
+    """Causal attention of runs of new tokens, packed back to back, over the 8-bit cache that holds their own keys already:
+    the step's rows seq_start[i] .. seq_start[i + 1] are sequence i's, behind seq_past[i] cached positions.  ``tile_seq`` and
+    ``tile_first``: the tiles of ATTN_TC05_TILE_ROWS new tokens (sequence, index of the tile's first token among the
+    sequence's new ones), best with those first that see the most keys.  The rest as for ``attn_decode_kv8``."""
+    if out.numel() != q.numel():
+        raise Backend(f"attn_prefill_kv8: {tuple(out.shape)} for the results of queries {tuple(q.shape)}")
+    if window is not None and window < 0:
+        raise Backend(f"attn_prefill_kv8: a window of {window} positions")
+    if q.shape[0] == 0 or tile_seq.numel() == 0:
+        return
+    _kv8_check("attn_prefill_kv8", q, k, v, exps, block_table, page, nh, nkv, hd,
+               (("tile_first", tile_first, tile_seq.numel()), ("seq_past", seq_past, block_table.shape[0]),
+                ("seq_start", seq_start, block_table.shape[0] + 1)))
+    _check(_fn("kv8", "esp_attn_run_kv8")(
+        _ptr(q, torch.bfloat16, "q"), _ptr(k, _E4M3, "keys"), _ptr(v, _E4M3, "values"), _ptr(exps, torch.uint8, "exponents"),
+        _ptr(out, torch.bfloat16, "out"), _ptr(tile_seq, torch.int32, "tile_seq"), _ptr(tile_first, torch.int32, "tile_first"),
+        _ptr(seq_start, torch.int32, "seq_start"), _ptr(seq_past, torch.int32, "seq_past"), _ptr(block_table, torch.int32, "page table"),
+        block_table.shape[1], k.shape[0], tile_seq.numel(), nh, nkv, hd, int(window or 0), _ptr(status, torch.int32, "status"), _stream()),
+        "attn_prefill_kv8")

@@ -159,7 +159,8 @@ class Workspace:
         self.frozen = False
         self.generation = 0          # bumped whenever a buffer moves; captured graphs check it
 
-    def get(self, name: str, shape: tuple, dtype) -> torch.Tensor:
+    def get(self, name: str, shape: tuple, dtype, zeroed: bool = False) -> torch.Tensor:
+        """``zeroed``: a new buffer holds zeros (counters that every kernel leaves at zero)."""
         seen = self._views.get((name, dtype, shape))
         if seen is not None:
             return seen
@@ -171,7 +172,7 @@ class Workspace:
         if buf is None or buf.numel() < count:
             if self.frozen:
                 raise Backend(f"workspace buffer {name} would have to grow while a captured graph holds it")
-            buf = torch.empty(max(count, 1), dtype=dtype, device=self.device)
+            buf = (torch.zeros if zeroed else torch.empty)(max(count, 1), dtype=dtype, device=self.device)
             self._bufs[key] = buf
             self.generation += 1
             self._views = {k: v for k, v in self._views.items() if (k[0], k[1]) != key}    # views of the old buffer

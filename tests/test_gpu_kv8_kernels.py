@@ -1,0 +1,513 @@
+"""The 8-bit cache's kernels against their definition in 64 bits (plain_kv8)."""
+import math
+
+import pytest
+import torch
+
+import plain_kv8 as plain
+from esp_b200.csrc import ops
+from esp_b200.parts.base import Workspace
+
+pytestmark = pytest.mark.gpu
+PAGE, BAD_INDEX = 64, 8
+E4M3 = torch.float8_e4m3fn
+
+
+def gen(seed):
+    return torch.Generator(device="cuda").manual_seed(seed)
+
+
+def pools(pages, nkv, hd, seed=None):
+    """Codes of keys and values and exponents; with a seed rows of ordinary size, else bytes that no kernel may use (NaN)."""
+    if seed is None:
+        k, v = (torch.full((pages, nkv, PAGE, hd), 0x7F, dtype=torch.uint8, device="cuda").view(E4M3) for _ in range(2))
+        return k, v, torch.full((pages, nkv, 2, PAGE), 255, dtype=torch.uint8, device="cuda")
+    g = gen(seed)
+    out, exps = [], torch.empty((pages, nkv, 2, PAGE), dtype=torch.uint8, device="cuda")
+    for which in range(2):
+        x = torch.randn((pages, nkv, PAGE, hd), generator=g, device="cuda") * torch.exp(torch.randn((pages, nkv, PAGE, 1), generator=g, device="cuda"))
+        if which == 0:
+            x[..., 3 % hd] *= 8
+        codes, e = plain.quantize(x.double())
+        out.append(codes.float().to(E4M3))
+        exps[:, :, which] = (e + 127).to(torch.uint8)
+    return out[0], out[1], exps
+
+
+def tables(lengths, seed, spare=3):
+    """Pages of the sequences in no order, -1 behind each sequence's last: (table, number of pages)."""
+    need = [(n + PAGE - 1) // PAGE for n in lengths]
+    total = sum(need) + spare
+    order = torch.randperm(total, generator=torch.Generator().manual_seed(seed)).to(torch.int32)
+    t, at = torch.full((len(lengths), max(need) + 1), -1, dtype=torch.int32), 0
+    for i, n in enumerate(need):
+        t[i, :n] = order[at:at + n]
+        at += n
+    return t.cuda(), total
+
+
+def ints(v):
+    return torch.tensor(v, dtype=torch.int32, device="cuda")
+
+
+def status():
+    return torch.zeros(1, dtype=torch.int32, device="cuda")
+
+
+def sequence_rows(pool, exps, which, pages, length):
+    """float64 [nkv, length, hd] of a sequence's rows."""
+    x = plain.stored(pool[pages], exps[pages, :, which])
+    return x.transpose(0, 1).flatten(1, 2)[:, :length]
+
+
+# ------------------------------------------------------------------------------------------------------- append
+APPEND = [
+    # nh, nkv, hd, rot, news, pasts, bias
+    (16, 16, 128, 128, [1], [0], True),
+    (16, 16, 128, 128, [1], [63], False),
+    (4, 2, 16, 16, [1, 1, 1], [5, 64, 127], True),
+    (5, 5, 24, 24, [3, 70], [62, 1], True),
+    (7, 1, 80, 40, [130], [17], False),
+    (6, 3, 96, 0, [9, 1], [120, 0], True),
+    (28, 4, 128, 128, [1] * 67, list(range(40, 107)), True),
+    (4, 4, 64, 64, [200, 1, 66], [0, 300, 62], False),
+    (2, 1, 192, 192, [65], [10], True),
+    (8, 8, 256, 256, [33, 40], [50, 0], True),
+    (3, 3, 256, 128, [5], [59], False),
+    (1, 1, 8, 4, [2], [0], False),
+]
+
+
+@pytest.mark.parametrize("nh,nkv,hd,rot,news,pasts,with_bias", APPEND)
+def test_append(nh, nkv, hd, rot, news, pasts, with_bias):
+    n, width = sum(news), (nh + 2 * nkv) * hd
+    g = gen(n + hd)
+    table, total = tables([a + b for a, b in zip(news, pasts)], 7)
+    k, v, exps = pools(total, nkv, hd, seed=n)
+    before = [t.clone() for t in (k.view(torch.uint8), v.view(torch.uint8), exps)]
+    qkv = torch.randn((n, width), generator=g, device="cuda") * torch.exp(2 * torch.randn((n, 1), generator=g, device="cuda"))
+    bias = torch.randn(width, generator=g, device="cuda") if with_bias else None
+    most = max(a + b for a, b in zip(news, pasts))
+    angle = torch.arange(most, device="cuda")[:, None] * 1e4 ** (-torch.arange(rot // 2, device="cuda") / max(1, rot // 2))
+    cos, sin = angle.cos().contiguous(), angle.sin().contiguous()
+    seq = ints([i for i, t in enumerate(news) for _ in range(t)])
+    pos = ints([p + j for p, t in zip(pasts, news) for j in range(t)])
+    q, st = torch.empty((n, nh * hd), dtype=torch.bfloat16, device="cuda"), status()
+    ops.kv8_rope_append(qkv, bias, seq, pos, cos, sin, rot, q, k, v, exps, table, PAGE, nh, nkv, hd, True, st)
+    assert st.item() == 0
+    x = (qkv.double() + (bias.double() if with_bias else 0)).view(n, nh + 2 * nkv, hd)
+    turned, big = x.clone(), x.abs()
+    if rot:
+        c, s = cos.double()[pos.long()], sin.double()[pos.long()]
+        turned[:, :nh + nkv] = plain.rotate(x[:, :nh + nkv], c, s, rot)
+        h = rot // 2
+        both = big[:, :nh + nkv, :h] + big[:, :nh + nkv, h:rot]
+        big[:, :nh + nkv, :rot] = torch.cat((both, both), -1)
+    # 32-bit: the bias's sum, two products and their sum are each off by at most half a step, 2^-24 of the operands' size
+    err = 4 * 2.0 ** -24 * (big + (bias.double().abs().max() if with_bias else 0))
+    got = q.double().view(n, nh, hd)
+    assert torch.all((got - turned[:, :nh]).abs() <= 2.0 ** -8 * turned[:, :nh].abs() + 2 * err[:, :nh])
+    page, place = table[seq.long(), (pos // PAGE).long()].long(), (pos % PAGE).long()
+    for pool, which, lo in ((k, 0, nh), (v, 1, nh + nkv)):
+        want, e64 = turned[:, lo:lo + nkv], plain.row_exponent(turned[:, lo:lo + nkv].abs().amax(-1))
+        e = exps[page, :, which, place].double() - 127
+        slack = err[:, lo:lo + nkv].amax(-1)
+        top = want.abs().amax(-1)
+        # the exponent of the definition, or the one of a maximum that rounding may have moved over a border
+        assert torch.all((e == plain.row_exponent(top + slack)) | (e == plain.row_exponent((top - slack).clamp_min(0))))
+        assert (e == e64).double().mean() > 0.99
+        rows = plain.stored(pool[page, :, place], exps[page, :, which, place])
+        # half a step of e4m3: 2^-4 of the number, or half of 2^(e - 9) below the normal range
+        half_step = torch.maximum(2.0 ** -4 * want.abs(), torch.exp2(e - 10)[..., None])
+        assert torch.all((rows - want).abs() <= half_step + 2 * err[:, lo:lo + nkv])
+        if not rot and not with_bias or (which == 1 and not with_bias):
+            codes, _ = plain.quantize(want)
+            assert torch.equal(pool[page, :, place].double(), codes)
+    # nothing else has changed
+    touched = torch.zeros((total, PAGE), dtype=torch.bool, device="cuda")
+    touched[page, place] = True
+    for t, old in zip((k.view(torch.uint8), v.view(torch.uint8)), before):
+        assert torch.equal(t.transpose(1, 2)[~touched], old.transpose(1, 2)[~touched])
+    assert torch.equal(exps.permute(0, 3, 1, 2)[~touched], before[2].permute(0, 3, 1, 2)[~touched])
+
+
+@pytest.mark.parametrize("hd,rot", [(128, 128), (128, 0), (80, 40), (256, 256), (64, 0)])
+def test_append_of_rows_at_the_borders(hd, rot):
+    """Maxima at and beside 448 * 2^e, ties, subnormal codes, zeros, the smallest and largest exponents, rows that are no numbers.
+    Position 0: the rotation is by an angle of zero, so numbers arrive as they are."""
+    rows = []
+    for e in (-100, -37, 0, 5, 100):
+        s = 2.0 ** e
+        rows += [[448 * s], [448 * (1 + 2.0 ** -23) * s, 1.0 * s], [-448 * s, 2.0 ** -9 * s, 2.0 ** -10 * s, 3 * 2.0 ** -10 * s, -5 * 2.0 ** -10 * s],
+                 [240 * s, 17 * s, 17.5 * s, 18 * s, 19 * s, 1.0625 * s, 1.1875 * s], [448.1 * s, -0.0]]
+    rows += [[0.0], [1e-45], [-1e-38, 3e-39], [2.0 ** -101 * 448], [math.inf], [1.0, -math.inf], [math.nan, 3.0], [3e38], [-0.0]]
+    n = len(rows)
+    x = torch.zeros((n, 3, hd), device="cuda")
+    for i, r in enumerate(rows):
+        x[i, 1, :len(r)] = torch.tensor(r)
+        x[i, 2, hd - len(r):] = torch.tensor(r)
+        if rot and not all(map(math.isfinite, r)):         # infinity times the sine 0 is not a number either way
+            x[i, 1] = 0
+    k, v, exps = pools(n, 1, hd)
+    cos, sin = torch.ones((1, rot // 2), device="cuda"), torch.zeros((1, rot // 2), device="cuda")
+    q = torch.empty((n, hd), dtype=torch.bfloat16, device="cuda")
+    table, st = torch.arange(n, dtype=torch.int32, device="cuda")[:, None].contiguous(), status()
+    ops.kv8_rope_append(x.view(n, -1), None, torch.arange(n, dtype=torch.int32, device="cuda"), ints([0] * n), cos, sin, rot, q, k, v, exps,
+                        table, PAGE, 1, 1, hd, True, st)
+    assert st.item() == 0
+    for pool, which in ((k, 0), (v, 1)):
+        codes, e = plain.quantize(x[:, 1 + which].double())
+        byte = torch.where(torch.isnan(e), 255.0, e + 127)
+        assert torch.equal(exps[:, 0, which, 0].double(), byte)
+        assert torch.equal(pool[:, 0, 0].double(), codes)
+
+
+def test_append_of_queries_alone_and_bad_places():
+    nh, nkv, hd = 4, 2, 64
+    qkv = torch.randn((5, (nh + 2 * nkv) * hd), generator=gen(1), device="cuda")
+    cos, sin = torch.ones((200, 32), device="cuda"), torch.zeros((200, 32), device="cuda")
+    k, v, exps = pools(3, nkv, hd)
+    q, st = torch.zeros((5, nh * hd), dtype=torch.bfloat16, device="cuda"), status()
+    seq, pos = ints([0, 0, 1, 1, 1]), ints([0, 1, 64, 65, 3])
+    ops.kv8_rope_append(qkv, None, seq, pos, cos, sin, hd, q, None, None, None, None, PAGE, nh, nkv, hd, False, st)
+    assert st.item() == 0
+    assert torch.equal(q, qkv[:, :nh * hd].to(torch.bfloat16))
+    # page 7 and page -1 are not there, position 200 has no angle, position 130 no entry of the table, -1 is no position
+    table = ints([[2, 0], [7, -1]])
+    for where in ([3, 0, 2, 2, 2], [3, 70, 0, 100, 2]):
+        st.zero_()
+        for t in (k.view(torch.uint8), v.view(torch.uint8), exps):
+            t.fill_(255)
+        ops.kv8_rope_append(qkv, None, ints([0, 0, 1, 1, 0]), ints([where[0], 64, where[2], 70, [200, 130][where[1] != 0]]), cos, sin, hd, q, k, v, exps,
+                            table, PAGE, nh, nkv, hd, True, st)
+        assert st.item() == BAD_INDEX
+        written = (exps[:, 0, 0] != 255).nonzero().tolist()
+        assert written == sorted([[2, 3], [0, 0]])
+    ops.kv8_rope_append(qkv[:1], None, ints([0]), ints([-1]), cos, sin, hd, q[:1], k, v, exps, table, PAGE, nh, nkv, hd, True, st)
+    assert st.item() == BAD_INDEX
+
+
+# ------------------------------------------------------------------------------------------------------- attention
+def check_rows(got, want, spread, q, k, hd, weight_step):
+    """|got - want| <= half a step of bfloat16 of the result, plus what rounding the weights (half a step of their type) and the
+    errors of the scores (twice: numerator and sum) and of exp2 (2^-21) may move it."""
+    nan = torch.isnan(want)
+    assert torch.equal(nan, torch.isnan(got))
+    slack = weight_step + 2 * plain.score_error(q, k, hd) + 2.0 ** -20
+    bound = 2.0 ** -8 * want.abs() + (1 + 2.0 ** -8) * slack * spread + 1e-38
+    off = (got - want).abs() - bound
+    assert torch.all(off[~nan] <= 0), f"off by {float((got - want)[~nan].abs().max())}, {float(off[~nan].max())} over the bound"
+
+
+DECODE = [
+    # nh, nkv, hd, lengths (the new token among them), window
+    (1, 1, 128, [1], 0),
+    (16, 16, 128, [1, 2, 31, 32, 33, 63, 64, 65], 0),
+    (16, 16, 128, [777], 0),
+    (28, 4, 128, [1000, 129, 4097], 0),
+    (12, 1, 128, [300, 5], 0),
+    (16, 1, 64, [513], 0),
+    (34, 2, 64, [129, 640], 0),
+    (40, 2, 128, [200], 0),
+    (4, 2, 16, [70, 3], 0),
+    (5, 5, 24, [150], 70),
+    (7, 7, 80, [99, 260], 0),
+    (6, 2, 104, [130], 64),
+    (8, 2, 192, [385, 64], 0),
+    (3, 3, 256, [200, 1], 0),
+    (20, 2, 256, [333], 100),
+    (4, 4, 64, [1, 5, 64, 65, 700, 1400], 1),
+    (4, 4, 64, [1, 5, 64, 65, 700, 1400], 64),
+    (8, 4, 128, [2000, 40], 333),
+    (2, 1, 128, [20000], 0),
+    (2, 1, 128, [20000, 300], 5000),
+    (16, 16, 128, [130] * 40, 0),
+]
+
+
+def decode_inputs(nh, nkv, hd, lengths, seed):
+    table, total = tables(lengths, seed)
+    k, v, exps = pools(total, nkv, hd, seed)
+    n = len(lengths)
+    q = (torch.randn((n, nh * hd), generator=gen(seed + 1), device="cuda") * 2).to(torch.bfloat16)
+    return table, k, v, exps, q, torch.arange(n, dtype=torch.int32, device="cuda"), ints([length - 1 for length in lengths])
+
+
+def check_decode(out, q, k, v, exps, table, lengths, nh, hd, window):
+    for i, length in enumerate(lengths):
+        pages = table[i, :(length + PAGE - 1) // PAGE].long()
+        kk, vv = (sequence_rows(p, exps, w, pages, length) for p, w in ((k, 0), (v, 1)))
+        qq = q[i].double().view(1, nh, hd)
+        want, spread = plain.attend(qq, kk, vv, torch.tensor([length - 1], device="cuda"), window)
+        check_rows(out[i].double().view(1, nh, hd), want, spread, qq, kk, hd, 2.0 ** -11)
+
+
+@pytest.mark.parametrize("nh,nkv,hd,lengths,window", DECODE)
+def test_decode(nh, nkv, hd, lengths, window):
+    table, k, v, exps, q, seq, pos = decode_inputs(nh, nkv, hd, lengths, 11)
+    out, st, ws = torch.full_like(q, math.nan), status(), Workspace(q.device)
+    for _ in range(2):                              # the second call finds the counters as the first one left them
+        out.fill_(math.nan)
+        ops.attn_decode_kv8(q, k, v, exps, out, ws, seq, pos, table, PAGE, nh, nkv, hd, window, st)
+        assert st.item() == 0
+        check_decode(out, q, k, v, exps, table, lengths, nh, hd, window)
+    # keys that were cached long before: the same bits
+    again = torch.empty_like(out)
+    ops.attn_decode_kv8(q, k, v, exps, again, ws, seq, pos, table, PAGE, nh, nkv, hd, window, st, seq_past=ints([length - 1 for length in lengths]))
+    assert torch.equal(out, again)
+
+
+@pytest.mark.parametrize("nh,nkv,hd", [(4, 4, 128), (12, 1, 64)])
+def test_decode_with_rows_that_are_no_numbers(nh, nkv, hd):
+    """NaN where the mask hides it (behind the row, ahead of its window) changes nothing; where it is seen the row is NaN."""
+    lengths, window = [300, 300, 300, 300], 100
+    table, k, v, exps, q, seq, pos = decode_inputs(nh, nkv, hd, lengths, 3)
+    out, st, ws = torch.empty_like(q), status(), Workspace(q.device)
+    ops.attn_decode_kv8(q, k, v, exps, out, ws, seq, pos, table, PAGE, nh, nkv, hd, window, st)
+    for i, (at, which) in enumerate([(199, 0), (200, 0), (200, 1), (199, 1)]):
+        exps[table[i, at // PAGE].long(), :, which, at % PAGE] = 255
+    last = table[:, 299 // PAGE].long()               # behind the last position: bytes that are no rows
+    exps[last, :, :, 300 % PAGE:] = 255
+    k.view(torch.uint8)[last, :, 300 % PAGE:] = 0x7F
+    v.view(torch.uint8)[last, :, 300 % PAGE:] = 0xFF
+    got = torch.empty_like(q)
+    ops.attn_decode_kv8(q, k, v, exps, got, ws, seq, pos, table, PAGE, nh, nkv, hd, window, st)
+    assert torch.equal(got[0], out[0]) and torch.equal(got[3], out[3])
+    assert torch.isnan(got[1]).all() and torch.isnan(got[2]).all()
+    assert st.item() == 0
+
+
+@pytest.mark.parametrize("group", [1, 12])
+@pytest.mark.parametrize("key_scale,value_scale", [(2.0 ** 90, 1.0), (2.0 ** -95, 1.0), (1.0, 2.0 ** 92), (1.0, 2.0 ** -92)])
+def test_decode_with_exponents_far_apart(group, key_scale, value_scale):
+    """Rows whose exponents differ by far more than a half's range; queries scaled against the keys."""
+    hd, length = 64, 500
+    g = gen(5)
+    x = torch.randn((2, length, hd), generator=g, device="cuda", dtype=torch.float64)
+    far = torch.arange(length, device="cuda") % 3 == 1
+    x[0] *= key_scale
+    x[1] *= torch.where(far, value_scale, 1.0)[:, None]
+    q = (torch.randn((1, group, hd), generator=g, device="cuda").double() * 3 / key_scale).to(torch.bfloat16)
+    table, total = tables([length], 2)
+    k, v, exps = pools(total, 1, hd, 1)
+    for which, pool in ((0, k), (1, v)):
+        codes, e = plain.quantize(x[which])
+        page, place = table[0, torch.arange(length, device="cuda") // PAGE].long(), torch.arange(length, device="cuda") % PAGE
+        pool.view(torch.uint8)[page, 0, place] = codes.float().to(E4M3).view(torch.uint8)
+        exps[page, 0, which, place] = (e + 127).to(torch.uint8)
+    out, st = torch.empty_like(q), status()
+    ops.attn_decode_kv8(q, k, v, exps, out, Workspace(q.device), ints([0]), ints([length - 1]), table, PAGE, group, 1, hd, 0, st)
+    assert st.item() == 0
+    check_decode(out, q, k, v, exps, table, [length], group, hd, 0)
+
+
+def test_decode_weights_of_few_strong_and_many_weak_keys():
+    """One key takes nearly all of the softmax's mass, thousands share the rest and all point the same way."""
+    hd, length = 64, 9000
+    table, total = tables([length], 2)
+    k, v, exps = pools(total, 1, hd, 1)
+    k.view(torch.uint8).zero_()
+    v.view(torch.uint8).fill_(0x38)                   # 1.0
+    exps.fill_(127)
+    first = table[0, 0].long()
+    k.view(torch.uint8)[first, 0, 0] = 0x38
+    v.view(torch.uint8)[first, 0, 0] = 0
+    for score in (8.0, 13.0):                         # weights of the others e^-8, e^-13 of the strong one's
+        q = torch.full((1, hd), score / math.sqrt(hd), device="cuda").to(torch.bfloat16)
+        out, st = torch.empty_like(q), status()
+        ops.attn_decode_kv8(q, k, v, exps, out, Workspace(q.device), ints([0]), ints([length - 1]), table, PAGE, 1, 1, hd, 0, st)
+        check_decode(out, q, k, v, exps, table, [length], 1, hd, 0)
+
+
+def test_decode_with_pages_that_are_none():
+    nh, nkv, hd, lengths = 4, 2, 128, [300, 200, 64, 100]
+    table, k, v, exps, q, seq, pos = decode_inputs(nh, nkv, hd, lengths, 9)
+    out, st, ws = torch.empty_like(q), status(), Workspace(q.device)
+    ops.attn_decode_kv8(q, k, v, exps, out, ws, seq, pos, table, PAGE, nh, nkv, hd, 0, st)
+    bad = table.clone()
+    bad[1, 1], bad[2, 0], bad[3, 1] = k.shape[0], -1, -2147483648
+    got = torch.empty_like(out)
+    ops.attn_decode_kv8(q, k, v, exps, got, ws, seq, pos, bad, PAGE, nh, nkv, hd, 0, st)
+    assert st.item() == BAD_INDEX
+    assert torch.equal(got[0], out[0]) and torch.isfinite(got).all()
+    assert (got[2] == 0).all()                        # not one page: no keys
+    st.zero_()
+    got.fill_(7)
+    ops.attn_decode_kv8(q, k, v, exps, got, ws, ints([0, 1, -1, 3]), ints([299, -1, 63, 99 + 64 * table.shape[1]]), table, PAGE, nh, nkv, hd, 0, st)
+    assert st.item() == BAD_INDEX and torch.equal(got[0], out[0]) and (got[1:] == 7).all()
+
+
+def test_decode_rows_do_not_depend_on_their_neighbours():
+    nh, nkv, hd, lengths = 8, 2, 128, [70, 700, 333]
+    table, k, v, exps, q, seq, pos = decode_inputs(nh, nkv, hd, lengths, 4)
+    ws, st, out = Workspace(q.device), status(), torch.empty_like(q)
+    ops.attn_decode_kv8(q, k, v, exps, out, ws, seq, pos, table, PAGE, nh, nkv, hd, 0, st)
+    order = [2, 0, 1, 2]
+    rows, got = torch.tensor(order, device="cuda"), torch.empty((4, nh * hd), dtype=torch.bfloat16, device="cuda")
+    # the same sequence twice in a call; rows in another order
+    ops.attn_decode_kv8(q[rows], k, v, exps, got, ws, ints(order), pos[rows], table, PAGE, nh, nkv, hd, 0, st)
+    if ops.attn_decode_kv8_split(3, nkv, 64 * table.shape[1]) == ops.attn_decode_kv8_split(4, nkv, 64 * table.shape[1]):
+        assert torch.equal(got, out[rows])
+    check_decode(got[:3], q[rows[:3]], k, v, exps, table[rows[:3]], [lengths[i] for i in order[:3]], nh, hd, 0)
+
+
+PREFILL = [
+    # nh, nkv, hd, news, pasts, window
+    (1, 1, 128, [1], [0], 0),
+    (2, 2, 128, [2], [0], 0),
+    (4, 4, 128, [200], [0], 0),
+    (4, 2, 128, [128, 127, 129], [0, 64, 63], 0),
+    (7, 1, 128, [300, 5, 1, 64], [1000, 0, 257, 128], 0),
+    (4, 2, 64, [257], [130], 0),
+    (2, 2, 64, [400], [100], 77),
+    (3, 3, 128, [300, 33], [500, 10], 129),
+    (2, 1, 128, [300], [0], 1),
+    (4, 2, 16, [150], [3], 0),
+    (5, 5, 24, [140, 2], [0, 70], 70),
+    (2, 1, 80, [130], [65], 0),
+    (3, 1, 104, [260], [0], 0),
+    (2, 2, 192, [140], [30], 0),
+    (2, 1, 256, [129, 20], [0, 200], 50),
+    (1, 1, 128, [1500], [700], 0),
+]
+
+
+def prefill_inputs(nh, nkv, hd, news, pasts, seed):
+    table, total = tables([a + b for a, b in zip(news, pasts)], seed)
+    k, v, exps = pools(total, nkv, hd, seed)
+    starts = [0]
+    for t in news:
+        starts.append(starts[-1] + t)
+    q = (torch.randn((starts[-1], nh * hd), generator=gen(seed + 1), device="cuda") * 2).to(torch.bfloat16)
+    tiles = sorted(((i, f) for i, t in enumerate(news) for f in range(0, t, 128)), key=lambda x: -(pasts[x[0]] + min(x[1] + 128, news[x[0]])))
+    return table, k, v, exps, q, starts, ints([t[0] for t in tiles]), ints([t[1] for t in tiles])
+
+
+def check_prefill(out, q, k, v, exps, table, starts, pasts, nh, hd, window):
+    for i, past in enumerate(pasts):
+        a, b = starts[i], starts[i + 1]
+        length = past + b - a
+        pages = table[i, :(length + PAGE - 1) // PAGE].long()
+        kk, vv = (sequence_rows(p, exps, w, pages, length) for p, w in ((k, 0), (v, 1)))
+        qq = q[a:b].double().view(b - a, nh, hd)
+        want, spread = plain.attend(qq, kk, vv, torch.arange(past, length, device="cuda"), window)
+        check_rows(out[a:b].double().view(b - a, nh, hd), want, spread, qq, kk, hd, 2.0 ** -8)
+
+
+@pytest.mark.parametrize("nh,nkv,hd,news,pasts,window", PREFILL)
+def test_prefill(nh, nkv, hd, news, pasts, window):
+    table, k, v, exps, q, starts, tile_seq, tile_first = prefill_inputs(nh, nkv, hd, news, pasts, 21)
+    out, st = torch.full_like(q, math.nan), status()
+    for _ in range(2):
+        out.fill_(math.nan)
+        ops.attn_prefill_kv8(q, k, v, exps, out, tile_seq, tile_first, ints(starts), ints(pasts), table, PAGE, nh, nkv, hd, window, st)
+        assert st.item() == 0
+        check_prefill(out, q, k, v, exps, table, starts, pasts, nh, hd, window)
+
+
+@pytest.mark.parametrize("hd", [64, 128, 256])
+def test_prefill_with_rows_that_are_no_numbers(hd):
+    """A position that is no number makes the rows that see it NaN, and leaves the others' bits alone: those before it, and those
+    whose window has passed it."""
+    nh, nkv, news, pasts, window = 4, 2, [400], [50], 150
+    table, k, v, exps, q, starts, tile_seq, tile_first = prefill_inputs(nh, nkv, hd, news, pasts, 5)
+    out, got, st = torch.empty_like(q), torch.empty_like(q), status()
+    args = (tile_seq, tile_first, ints(starts), ints(pasts), table, PAGE, nh, nkv, hd, window, st)
+    ops.attn_prefill_kv8(q, k, v, exps, out, *args)
+    for which, at in ((0, 211), (1, 230)):
+        kept = exps.clone()
+        exps[table[0, at // PAGE].long(), 0, which, at % PAGE] = 255
+        ops.attn_prefill_kv8(q, k, v, exps, got, *args)
+        assert st.item() == 0
+        pos = torch.arange(50, 450, device="cuda")
+        sees = (pos >= at) & (pos - at < window)
+        a, b = got.view(400, nh, hd), out.view(400, nh, hd)
+        assert torch.isnan(a[sees][:, :2]).all()
+        assert torch.equal(a[~sees], b[~sees]) and torch.equal(a[:, 2:], b[:, 2:])
+        exps.copy_(kept)
+    # what lies behind the last position is not looked at
+    last = table[0, 449 // PAGE].long()
+    exps[last, :, :, 450 % PAGE:] = 255
+    k.view(torch.uint8)[last, :, 450 % PAGE:] = 0x7F
+    v.view(torch.uint8)[last, :, 450 % PAGE:] = 0xFF
+    ops.attn_prefill_kv8(q, k, v, exps, got, *args)
+    assert torch.equal(got, out)
+
+
+@pytest.mark.parametrize("hd", [128, 192])
+@pytest.mark.parametrize("value_scale", [2.0 ** 92, 2.0 ** -92])
+def test_prefill_with_exponents_far_apart(hd, value_scale):
+    nh, nkv, news, pasts = 2, 1, [200], [100]
+    table, k, v, exps, q, starts, tile_seq, tile_first = prefill_inputs(nh, nkv, hd, news, pasts, 6)
+    shift = round(math.log2(value_scale))
+    e = exps[:, :, 1, ::3].int() + shift
+    exps[:, :, 1, ::3] = e.clamp(27, 227).to(torch.uint8)
+    exps[:, :, 0] = (exps[:, :, 0].int() + 60).to(torch.uint8)
+    q = (q.float() * 2.0 ** -60).to(torch.bfloat16)
+    out, st = torch.empty_like(q), status()
+    ops.attn_prefill_kv8(q, k, v, exps, out, tile_seq, tile_first, ints(starts), ints(pasts), table, PAGE, nh, nkv, hd, 0, st)
+    check_prefill(out, q, k, v, exps, table, starts, pasts, nh, hd, 0)
+
+
+@pytest.mark.parametrize("hd", [128, 192])
+def test_prefill_with_pages_that_are_none(hd):
+    nh, nkv, news, pasts = 2, 1, [150, 150], [100, 30]
+    table, k, v, exps, q, starts, tile_seq, tile_first = prefill_inputs(nh, nkv, hd, news, pasts, 8)
+    out, got, st = torch.empty_like(q), torch.empty_like(q), status()
+    ops.attn_prefill_kv8(q, k, v, exps, out, tile_seq, tile_first, ints(starts), ints(pasts), table, PAGE, nh, nkv, hd, 0, st)
+    assert st.item() == 0
+    bad = table.clone()
+    bad[1, 1] = k.shape[0] + 5
+    ops.attn_prefill_kv8(q, k, v, exps, got, tile_seq, tile_first, ints(starts), ints(pasts), bad, PAGE, nh, nkv, hd, 0, st)
+    assert st.item() == BAD_INDEX
+    assert torch.equal(got[:150], out[:150]) and torch.isfinite(got).all()
+
+
+# ------------------------------------------------------------------------------------------------------- together
+def test_append_then_attend_is_a_captured_step():
+    """A step as it is used, append then decode, on a stream of its own and replayed from a graph over changing inputs."""
+    nh, nkv, hd, lengths = 8, 2, 128, [130, 700]
+    n, width = 2, (nh + 2 * nkv) * hd
+    table, total = tables([length + 8 for length in lengths], 3)
+    k, v, exps = pools(total, nkv, hd, 2)
+    angle = torch.arange(800, device="cuda")[:, None] * 1e4 ** (-torch.arange(64, device="cuda") / 64)
+    cos, sin = angle.cos().contiguous(), angle.sin().contiguous()
+    qkv, q = torch.empty((n, width), device="cuda"), torch.empty((n, nh * hd), dtype=torch.bfloat16, device="cuda")
+    out, st, ws, seq, pos = torch.empty_like(q), status(), Workspace(q.device), ints([0, 1]), ints([0, 0])
+
+    def step():
+        ops.kv8_rope_append(qkv, None, seq, pos, cos, sin, hd, q, k, v, exps, table, PAGE, nh, nkv, hd, True, st)
+        ops.attn_decode_kv8(q, k, v, exps, out, ws, seq, pos, table, PAGE, nh, nkv, hd, 0, st)
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        pos.copy_(ints([length - 1 for length in lengths]))
+        qkv.normal_()
+        step()
+        graph = torch.cuda.CUDAGraph()
+        side.synchronize()
+        with torch.cuda.graph(graph, stream=side):
+            step()
+        for t in range(4):
+            now = [length + t for length in lengths]
+            pos.copy_(ints([length - 1 for length in now]))
+            qkv.normal_()
+            graph.replay()
+            side.synchronize()
+            assert st.item() == 0
+            check_decode(out, q, k, v, exps, table, now, nh, hd, 0)
+
+
+def test_prefill_and_decode_agree():
+    """The last row of a run sees what a decode step at its place sees."""
+    for hd, weight in ((128, 2.0 ** -8), (192, 2.0 ** -11)):
+        nh, nkv, news, pasts = 6, 2, [200, 129], [0, 300]
+        table, k, v, exps, q, starts, tile_seq, tile_first = prefill_inputs(nh, nkv, hd, news, pasts, 2)
+        out, st = torch.empty_like(q), status()
+        ops.attn_prefill_kv8(q, k, v, exps, out, tile_seq, tile_first, ints(starts), ints(pasts), table, PAGE, nh, nkv, hd, 0, st)
+        rows = torch.tensor([starts[1] - 1, starts[2] - 1], device="cuda")
+        one = torch.empty((2, nh * hd), dtype=torch.bfloat16, device="cuda")
+        ops.attn_decode_kv8(q[rows], k, v, exps, one, Workspace(q.device), ints([0, 1]), ints([199, 428]), table, PAGE, nh, nkv, hd, 0, st)
+        spread = torch.nan_to_num(plain.stored(v, exps[:, :, 1])).abs().max()
+        assert (one.double() - out[rows].double()).abs().max() <= (2 * 2.0 ** -8 + weight + 2.0 ** -11 + 1e-3) * spread
