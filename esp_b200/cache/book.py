@@ -81,6 +81,11 @@ class KvLayout:
         per_head = self.head_dim + ((self.value_dim or self.head_dim) if self.values else 0)
         return self.num_kv_heads * per_head
 
+    def row_bytes(self, element_bytes: int) -> int:
+        """Bytes that one position of one layer holds; elements of one byte (the 8-bit cache) carry an exponent a row."""
+        rows = self.num_kv_heads * (2 if self.values else 1)
+        return self.row_elements * element_bytes + (rows if element_bytes == 1 else 0)
+
 
 class GroupBook:
     """Pages of one layer group.  ``tables[slot][i]`` is the page that holds

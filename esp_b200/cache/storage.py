@@ -31,6 +31,7 @@ class LayerCache:
     writes: bool                       # False: it reads another call's keys and values
     state: Optional[torch.Tensor]      # [max_slots, *StateSpec.shape]
     page: int = PAGE
+    exps: Optional[torch.Tensor] = None    # the 8-bit cache: [pages, nkv, 2, PAGE] exponents of the keys' and values' rows
 
 
 class Cache:
@@ -39,10 +40,13 @@ class Cache:
 
     def __init__(self, requests: list, max_tokens: int, max_slots: int, max_positions: int, dtype, device,
                  model_states: Optional[dict] = None):
-        """``model_states``: name -> StateSpec of per-sequence state that belongs to no layer (what the model's
+        """``dtype``: of keys and values; float8_e4m3fn is the 8-bit cache, whose layers hold an exponent a row besides.
+
+        ``model_states``: name -> StateSpec of per-sequence state that belongs to no layer (what the model's
         embedding keeps, for instance); found again as ``self.named_state[name]``, zeroed when a slot is opened."""
         self.device = device
         self.dtype = dtype
+        self.eight_bit = dtype == torch.float8_e4m3fn
         layouts, members = [], []
         owner_group = {}
         for idx, (layout, _state, cache_of) in enumerate(requests):
@@ -63,12 +67,13 @@ class Cache:
         self.layouts = layouts
         self.members = members
         n_pages = self.book.n_pages
-        self.k_pools, self.v_pools = [], []
+        self.k_pools, self.v_pools, self.exp_pools = [], [], []
         for layout, m in zip(layouts, members):
             shape = (len(m), n_pages, layout.num_kv_heads, PAGE, layout.head_dim)
             self.k_pools.append(torch.zeros(shape, dtype=dtype, device=device))
             v_shape = (*shape[:-1], layout.value_dim or layout.head_dim)
             self.v_pools.append(torch.zeros(v_shape, dtype=dtype, device=device) if layout.values else None)
+            self.exp_pools.append(torch.zeros((*shape[:3], 2, PAGE), dtype=torch.uint8, device=device) if self.eight_bit else None)
         self.engine_state = torch.zeros((max_slots, STATE_WORDS), dtype=torch.int64, device=device)
         self.named_state = {name: torch.zeros((max_slots, *spec.shape), dtype=spec.dtype, device=device)
                             for name, spec in (model_states or {}).items()}
@@ -81,7 +86,8 @@ class Cache:
             if src in owner_group:
                 g, j = owner_group[src]
                 v_pool = self.v_pools[g][j] if self.v_pools[g] is not None else None
-                self.layers.append(LayerCache(self.k_pools[g][j], v_pool, g, cache_of is None, st))
+                exps = self.exp_pools[g][j] if self.eight_bit else None
+                self.layers.append(LayerCache(self.k_pools[g][j], v_pool, g, cache_of is None, st, exps=exps))
             else:
                 self.layers.append(LayerCache(None, None, None, False, st))
 
@@ -106,7 +112,7 @@ class Cache:
 
     def bytes_per_token(self) -> int:
         el = torch.empty((), dtype=self.dtype).element_size()
-        return sum(len(m) * l.row_elements * el for l, m in zip(self.layouts, self.members))
+        return sum(len(m) * l.row_bytes(el) for l, m in zip(self.layouts, self.members))
 
     def state_bytes(self) -> int:
         """Bytes of the mixers' per-sequence states over all slots."""

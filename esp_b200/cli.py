@@ -49,14 +49,15 @@ def cmd_generate(a) -> int:
     cache_tokens = a.cache_tokens or cache_tokens_for([len(r.prompt_ids) for r in reqs], a.max_tokens, window, a.max_batch)
     if a.model is not None:
         prov = DecoderProvider.load(a.model, dtype=a.dtype, device=a.device, max_batch=a.max_batch,
-                                    max_context=a.max_context, max_tokens=cache_tokens)
+                                    max_context=a.max_context, max_tokens=cache_tokens, cache_dtype=a.cache_dtype)
     else:
         # weights made on the device from the configuration and the seed: the same values that
         # ``random-model`` with this seed writes into a folder
         from .weights import InitSpec
         prov = DecoderProvider.from_random(config, a.weights_seed, init=InitSpec(a.weight_std, a.bias_std, a.norm_std),
                                            dtype=a.dtype, device=a.device, max_batch=a.max_batch,
-                                           max_context=a.max_context, max_tokens=cache_tokens, stored_dtype=a.store_dtype)
+                                           max_context=a.max_context, max_tokens=cache_tokens, stored_dtype=a.store_dtype,
+                                           cache_dtype=a.cache_dtype)
     if a.profile:
         # one eager prefill of the first request and one eager decode step of it, timed kernel by kernel
         from .engine import StepEntry
@@ -107,6 +108,8 @@ def main(argv=None) -> int:
     g.add_argument("--bias-std", type=float, default=0.0)
     g.add_argument("--norm-std", type=float, default=0.0)
     g.add_argument("--dtype", default="bfloat16", choices=["bfloat16", "float32"])
+    g.add_argument("--cache-dtype", default=None, choices=["float8_e4m3"],
+                   help="keep keys and values in 8 bits (default: in the activations' dtype)")
     g.add_argument("--device", default="cuda:0")
     g.add_argument("--prompt-ids", action="append", help="token ids, comma or space separated; repeat for a batch")
     g.add_argument("--prompt", action="append", help="text prompt (needs tokenizer.json); repeat for a batch")

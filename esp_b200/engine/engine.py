@@ -21,7 +21,7 @@ from ..cache.storage import STATE_RNG, STATE_WORDS
 from ..csrc import ops
 from ..sampling import as_signed64
 from ..config import config_from_json
-from ..errors import Backend, InvalidRequest, NonFiniteScores
+from ..errors import Backend, InvalidRequest, NonFiniteScores, Unsupported
 from ..parts import Runtime, StepContext
 from ..parts.base import SideStream, StepHost
 from ..weights import FolderSource, InitSpec, RandomSource, load_into
@@ -37,6 +37,28 @@ def parse_dtype(name) -> torch.dtype:
     if name not in DTYPES:
         raise InvalidRequest(f"dtype must be one of {sorted(DTYPES)}, got {name!r}")
     return DTYPES[name]
+
+
+def parse_cache_dtype(name, dtype: torch.dtype) -> torch.dtype:
+    """The dtype of cached keys and values: None is the engine's own; "float8_e4m3" the 8-bit cache of a bfloat16 engine."""
+    if name is None:
+        return dtype
+    if name in ("float8_e4m3", torch.float8_e4m3fn):
+        if dtype != torch.bfloat16:
+            raise InvalidRequest(f"the 8-bit cache belongs to a bfloat16 engine, this one runs in {dtype}")
+        return torch.float8_e4m3fn
+    if (DTYPES.get(name) if isinstance(name, str) else name) != dtype:
+        raise InvalidRequest(f"cache dtype must be the engine's own ({dtype}) or 'float8_e4m3', got {name!r}")
+    return dtype
+
+
+def check_kv8(model) -> None:
+    """Every layer with keys and values has to be able to keep them in 8 bits."""
+    for i, e in enumerate(model.plan.schedule):
+        mixer = model.blocks[e.layer].mixer
+        if getattr(mixer, "kv_layout", None) is not None and mixer.kv_layout() is not None and not getattr(mixer, "takes_kv8", False):
+            raise Unsupported("cache_dtype", f"float8_e4m3: layer {e.layer} (schedule entry {i}, {type(mixer).__name__}) keeps keys and values "
+                                             f"that the 8-bit cache does not take")
 
 
 class PendingTokens:
@@ -63,21 +85,26 @@ class StepEntry:
 
 class Engine:
     def __init__(self, config, source_factory, dtype="bfloat16", device="cuda:0", max_tokens: int = 8192,
-                 max_slots: Optional[int] = None, shrink_to_fit: bool = False):
+                 max_slots: Optional[int] = None, shrink_to_fit: bool = False, cache_dtype=None):
         """``source_factory(specs) -> source``: gives the loader its tensors.
         ``max_tokens`` sizes the cache; it is refused if weights and cache do not
         fit the device's free memory, or, with ``shrink_to_fit``, made as small
-        as fits (``self.max_tokens`` tells what it became)."""
+        as fits (``self.max_tokens`` tells what it became).  ``cache_dtype``
+        "float8_e4m3" keeps keys and values in 8 bits, with a power of two
+        per row (half the memory and the traffic of a bfloat16 cache)."""
         self.config = config
         self.plan = config.plan()
         self.dtype = parse_dtype(dtype)
+        self.cache_dtype = parse_cache_dtype(cache_dtype, self.dtype)
         if not torch.cuda.is_available():
             raise Backend("no CUDA device is visible; esp_b200 has no CPU path")
         torch.backends.cuda.matmul.allow_tf32 = False
         torch.backends.cudnn.allow_tf32 = False
-        self.rt = Runtime(device, self.dtype)
+        self.rt = Runtime(device, self.dtype, kv8=self.cache_dtype == torch.float8_e4m3fn)
         with torch.cuda.device(self.rt.device):
             self.model = DecoderModel(self.plan, self.rt)
+            if self.rt.kv8:
+                check_kv8(self.model)
             specs = [s for part in self.model.all_parts() for s in part.param_specs()]
             source = source_factory(specs)
             self.memory_plan = self._check_memory(specs, source, max_tokens, shrink_to_fit, max_slots)
@@ -89,7 +116,7 @@ class Engine:
                 max_slots = max(1, min(n_pages, 4096))
             self.max_slots = max_slots
             self.cache = Cache(self.model.cache_requests(), max_tokens, max_slots, self.plan.max_positions,
-                               self.dtype, self.rt.device, model_states=self.model.model_states())
+                               self.cache_dtype, self.rt.device, model_states=self.model.model_states())
         parts = self.model.all_parts()
         # a decode step is replayed from a captured graph only if every part says that it may be
         self._parts_graph_safe = all(getattr(p, "graph_safe", False) for p in parts)
@@ -126,7 +153,7 @@ class Engine:
         the device's free memory; refuses with the numbers instead of dying inside
         an allocation.  ``ESP_B200_MEMORY_HEADROOM`` (bytes, default 2 GiB) is kept
         for scratch buffers and the CUDA context."""
-        el = {torch.float32: 4, torch.bfloat16: 2, torch.float16: 2}
+        el = {torch.float32: 4, torch.bfloat16: 2, torch.float16: 2, torch.float8_e4m3fn: 1}
         have = set(source.names())
         weights = 0
         for sp in specs:
@@ -139,7 +166,7 @@ class Engine:
         per_token, per_slot = 0, 0
         for layout, state, cache_of in self.model.cache_requests():
             if layout is not None and cache_of is None:
-                per_token += layout.row_elements * el[self.dtype]
+                per_token += layout.row_bytes(el[self.cache_dtype])
             if state is not None:
                 per_slot += int(np.prod(state.shape)) * el.get(state.dtype, 4)
         # the mixers' states of fixed size: one row per slot
@@ -358,9 +385,9 @@ class Engine:
         c = self._host_counters
         c["steps"] += 1
         c["tokens"] += sum(news)
-        el = torch.empty((), dtype=self.dtype).element_size()
+        el = self.cache_dtype.itemsize
         for layout, members in zip(self.cache.layouts, self.cache.members):
-            per_key = len(members) * layout.row_elements * el
+            per_key = len(members) * layout.row_bytes(el)
             seen = 0
             for p, t in zip(pasts, news):
                 # the keys the sequence's last new token sees: every kernel streams a sequence's visible keys once

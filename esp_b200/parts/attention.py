@@ -156,9 +156,15 @@ class Attention(Part):
             views[self._name("o", True)] = self.b_o
         return views
 
+    @property
+    def takes_kv8(self) -> bool:
+        return getattr(self.position, "takes_kv8", False) and ops.kv8_fits(self.spec.head_dim)
+
     # -- which kernel a step of n token rows gets, and the index lists it needs ----------
     def kernel_for(self, n: int, page: int = PAGE) -> str:
         s, rt = self.spec, self.rt
+        if rt.kv8:
+            return "kv8_rows" if n <= DECODE_ROWS else "kv8_tiles"
         if rt.dtype == torch.bfloat16:
             if s.head_dim in (64, 128, 192, 256) and n <= DECODE_ROWS and page == PAGE:
                 return "split"         # few rows: split the keys over blocks so that the cache streams at full width
@@ -169,13 +175,13 @@ class Attention(Part):
         return "plain"
 
     def step_arrays_key(self):
-        return ("attention", self.rt.dtype, self.spec.head_dim)
+        return ("attention", self.rt.dtype, self.rt.kv8, self.spec.head_dim)
 
     def step_arrays(self, step):
         """Tiles of new tokens for the two prefill kernels: (sequence, first new token) per tile; for the
         tensor-memory kernel the tiles that see the most keys come first (its blocks take them in order)."""
         kind = self.kernel_for(step.n_tokens)
-        if kind == "tc05":
+        if kind in ("tc05", "kv8_tiles"):
             rows = ops.ATTN_TC05_TILE_ROWS
             tiles = sorted(((i, f) for i, t in enumerate(step.news) for f in range(0, t, rows)),
                            key=lambda sf: -(step.pasts[sf[0]] + min(sf[1] + rows, step.news[sf[0]])))
@@ -219,6 +225,9 @@ class Attention(Part):
         table = ctx.block_tables[layer.group]
         n = q.shape[0]
         kind = self.kernel_for(n, layer.page)
+        if rt.kv8:
+            self._attend_kv8(kind, q, o, ctx, layer, table)
+            return
         if kind in ("tc05", "flash"):
             rows = ops.ATTN_TC05_TILE_ROWS if kind == "tc05" else 64
             tile_seq, tile_first = ctx.arrays.get(f"attention.tiles{rows}.seq"), ctx.arrays.get(f"attention.tiles{rows}.first")
@@ -248,6 +257,16 @@ class Attention(Part):
         else:
             ops.attn_simt(q, layer.k, layer.v, o, ctx.tok_seq, ctx.tok_pos, table, layer.page, s.num_heads,
                           s.num_kv_heads, s.head_dim, s.window, rt.status)
+
+    def _attend_kv8(self, kind, q, o, ctx, layer, table):
+        s, rt = self.spec, self.rt
+        tile_seq, tile_first = (ctx.arrays.get(f"attention.tiles{ops.ATTN_TC05_TILE_ROWS}.{w}") for w in ("seq", "first"))
+        if kind == "kv8_tiles" and tile_seq is not None:
+            ops.attn_prefill_kv8(q, layer.k, layer.v, layer.exps, o, tile_seq, tile_first, ctx.seq_start, ctx.seq_past, table, layer.page,
+                                 s.num_heads, s.num_kv_heads, s.head_dim, s.window, rt.status)
+        else:                          # few rows, or a step made without this part's lists
+            ops.attn_decode_kv8(q, layer.k, layer.v, layer.exps, o, rt.ws, ctx.tok_seq, ctx.tok_pos, table, layer.page, s.num_heads,
+                                s.num_kv_heads, s.head_dim, s.window, rt.status, seq_past=ctx.seq_past if layer.writes else None)
 
 
 class NormedAttention(Part):

@@ -79,6 +79,8 @@ class Part:
     # True: the part may run inside a captured step (see the module's text); parts from outside the
     # library are taken to be unsafe until they say otherwise
     graph_safe = False
+    # mixers and position encodings: True: the part writes and reads the 8-bit cache (a layer's ``exps``) as well
+    takes_kv8 = False
 
     def param_specs(self) -> list:
         return []
@@ -232,12 +234,13 @@ class SideStream:
 class Runtime:
     """Device, activation dtype, scratch and the device status word."""
 
-    def __init__(self, device, dtype: torch.dtype, ffn_chunk_tokens: int = 16384):
+    def __init__(self, device, dtype: torch.dtype, ffn_chunk_tokens: int = 16384, kv8: bool = False):
         """``device`` None gives a runtime that can only enumerate parts and
         their parameters (used to write model folders without a GPU)."""
         if dtype not in (torch.float32, torch.bfloat16):
             raise InvalidConfig(f"dtype must be float32 or bfloat16, got {dtype}")
         self.dtype = dtype
+        self.kv8 = kv8                    # keys and values are cached in 8 bits
         self.shared_parts: dict = {}
         self.device = None
         self.side_stream = None

@@ -16,6 +16,7 @@ class RopeSplitHalf(Part):
     and kept as cos/sin tables [max_positions, rotary_dim/2]."""
 
     graph_safe = True
+    takes_kv8 = True
 
     def __init__(self, spec, rt):
         self.spec = spec
@@ -35,6 +36,10 @@ class RopeSplitHalf(Part):
 
     def rotate_and_store(self, qkv, bias, ctx, q_out, layer, nh, nkv, hd, status):
         table = ctx.block_tables[layer.group] if layer.group is not None else None
+        if layer.exps is not None:
+            ops.kv8_rope_append(qkv, bias, ctx.tok_seq, ctx.tok_pos, self.cos, self.sin, self.spec.rotary_dim, q_out, layer.k,
+                                layer.v, layer.exps, table, layer.page, nh, nkv, hd, layer.writes, status)
+            return
         ops.rope_kvwrite(qkv, bias, ctx.tok_seq, ctx.tok_pos, self.cos, self.sin, self.spec.rotary_dim, q_out,
                          layer.k, layer.v, table, layer.page, nh, nkv, hd, layer.writes, status)
 
@@ -42,7 +47,7 @@ class RopeSplitHalf(Part):
         """Optional short cut of a position part: the packed projection, this encoding and the cache write
         in one kernel.  False: not for these sizes; the caller projects and calls ``rotate_and_store``."""
         if (h.dtype != torch.bfloat16 or w_qkv.dtype != torch.bfloat16 or self.spec.rotary_dim != hd
-                or layer.group is None or not ops.qkv_rope_skinny_fits(h.shape[0], h.shape[1], hd)):
+                or layer.group is None or layer.exps is not None or not ops.qkv_rope_skinny_fits(h.shape[0], h.shape[1], hd)):
             return False
         ops.qkv_rope_skinny(h, w_qkv, bias, ctx.tok_seq, ctx.tok_pos, self.cos, self.sin, q_out, layer.k, layer.v,
                             ctx.block_tables[layer.group], layer.page, nh, nkv, hd, layer.writes, status)
@@ -53,12 +58,17 @@ class NoPosition(Part):
     """No encoding: queries and keys are stored as projected."""
 
     graph_safe = True
+    takes_kv8 = True
 
     def __init__(self, spec, rt):
         self.spec = spec
 
     def rotate_and_store(self, qkv, bias, ctx, q_out, layer, nh, nkv, hd, status):
         table = ctx.block_tables[layer.group] if layer.group is not None else None
+        if layer.exps is not None:
+            ops.kv8_rope_append(qkv, bias, ctx.tok_seq, ctx.tok_pos, None, None, 0, q_out, layer.k, layer.v, layer.exps, table,
+                                layer.page, nh, nkv, hd, layer.writes, status)
+            return
         ops.rope_kvwrite(qkv, bias, ctx.tok_seq, ctx.tok_pos, None, None, 0, q_out, layer.k, layer.v, table,
                          layer.page, nh, nkv, hd, layer.writes, status)
 

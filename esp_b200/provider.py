@@ -127,24 +127,26 @@ class DecoderProvider:
     # -- construction -----------------------------------------------------------
     @classmethod
     def load(cls, model_dir, dtype="bfloat16", device="cuda:0", max_batch: int = 64, max_context: Optional[int] = None,
-             max_tokens: Optional[int] = None) -> "DecoderProvider":
+             max_tokens: Optional[int] = None, cache_dtype=None) -> "DecoderProvider":
         """``max_context``: longest sequence to make room for (default: the
         model's).  ``max_tokens``: cache size in tokens; refused if it does not
         fit the device.  Default: room for max_batch sequences of max_context,
         at most 1M tokens and at most what the device's free memory holds
-        beside the weights."""
+        beside the weights.  ``cache_dtype`` "float8_e4m3": keys and values in
+        8 bits (see ``Engine``)."""
         model_dir = Path(model_dir)
         from .config import config_from_json
         config = config_from_json(model_dir)
         fit = max_tokens is None
         max_tokens = cls._cache_tokens(config, max_batch, max_context, max_tokens)
-        engine = Engine.from_folder(model_dir, dtype=dtype, device=device, max_tokens=max_tokens, shrink_to_fit=fit)
+        engine = Engine.from_folder(model_dir, dtype=dtype, device=device, max_tokens=max_tokens, shrink_to_fit=fit,
+                                    cache_dtype=cache_dtype)
         return cls(engine, load_tokenizer(model_dir), max_batch)
 
     @classmethod
     def from_random(cls, config, seed: int = 0, init=None, dtype="bfloat16", device="cuda:0", max_batch: int = 64,
                     max_context: Optional[int] = None, max_tokens: Optional[int] = None,
-                    stored_dtype=None) -> "DecoderProvider":
+                    stored_dtype=None, cache_dtype=None) -> "DecoderProvider":
         """Random weights made on the device.  ``stored_dtype``: the dtype a model
         folder of these weights would store them in (default: ``dtype``); with the
         same configuration, seed, ``init`` and stored dtype the values are those
@@ -153,7 +155,7 @@ class DecoderProvider:
         fit = max_tokens is None
         max_tokens = cls._cache_tokens(config, max_batch, max_context, max_tokens)
         engine = Engine.from_random(config, seed, init or InitSpec(), stored_dtype=stored_dtype, dtype=dtype, device=device,
-                                    max_tokens=max_tokens, shrink_to_fit=fit)
+                                    max_tokens=max_tokens, shrink_to_fit=fit, cache_dtype=cache_dtype)
         return cls(engine, None, max_batch)
 
     @staticmethod
