@@ -36,7 +36,7 @@ LIBRARIES = {
     # bfloat16 only: loaded when a model runs in bfloat16
     "bf16": ["gemm_skinny.cu", "attn_decode.cu", "attn_prefill.cu", "attn_latent_mma.cu", "linear_attn.cu"],
     # the 8-bit key/value cache (bfloat16 engines that ask for it): append, attention of few and of many new tokens
-    "kv8": ["kv8_append.cu", "attn_kv8.cu"],
+    "kv8": ["kv8_append.cu", "attn_kv8.cu", "attn_prefill_kv8.cu"],
     # tcgen05/TMEM products: bfloat16 with many rows (prefill), 32-bit with any number of rows
     "tc05": ["gemm_tc05.cu", "gemm_split.cu", "attn_prefill_tc05.cu", "attn_diff_tc05.cu"],
 }

@@ -113,6 +113,7 @@ _SIGNATURES = {
                              c_int, c_int, c_float, c_int, c_float, c_float, c_float, c_float, P, c_longlong, P, P],
     "esp_kv8_append": [P, P, P, P, P, P, c_int, c_int, P, P, P, P, P, c_int, c_int, c_int, c_int, c_int, c_int, c_int, P, P],
     "esp_attn_decode_kv8": [P, P, P, P, P, P, P, P, P, P, P, P, c_int, c_int, c_int, c_int, c_int, c_int, c_int, c_int, c_int, P, P],
+    "esp_attn_prefill_kv8": [P, c_longlong, P, P, P, P, P, P, P, P, P, c_int, c_int, c_int, c_int, c_int, c_int, c_int, P, P],
     "esp_attn_run_kv8": [P, P, P, P, P, P, P, P, P, P, c_int, c_int, c_int, c_int, c_int, c_int, c_int, P, P],
 }
 
@@ -1564,7 +1565,7 @@ def _kv8_check(what, q, k, v, exps, block_table, page, nh, nkv, hd, vectors):
     for name, t, least in vectors:
         if t is not None and t.numel() < least:
             raise Backend(f"{what}: {name} has {t.numel()} elements, {least} are needed")
-    for name, t, step in (("queries", q, 16), ("keys", k, 16), ("values", v, 16), ("exponents", exps, 4)):
+    for name, t, step in (("queries", q, 16), ("keys", k, 16), ("values", v, 16), ("exponents", exps, 16)):
         if t is not None and t.data_ptr() % step:
             raise Backend(f"{what}: the {name} do not start on a multiple of {step} bytes")
     if not q.is_cuda:
@@ -1660,9 +1661,11 @@ def attn_prefill_kv8(q, k, v, exps, out, tile_seq, tile_first, seq_start, seq_pa
     _kv8_check("attn_prefill_kv8", q, k, v, exps, block_table, page, nh, nkv, hd,
                (("tile_first", tile_first, tile_seq.numel()), ("seq_past", seq_past, block_table.shape[0]),
                 ("seq_start", seq_start, block_table.shape[0] + 1)))
-    _check(_fn("kv8", "esp_attn_run_kv8")(
-        _ptr(q, torch.bfloat16, "q"), _ptr(k, _E4M3, "keys"), _ptr(v, _E4M3, "values"), _ptr(exps, torch.uint8, "exponents"),
-        _ptr(out, torch.bfloat16, "out"), _ptr(tile_seq, torch.int32, "tile_seq"), _ptr(tile_first, torch.int32, "tile_first"),
-        _ptr(seq_start, torch.int32, "seq_start"), _ptr(seq_past, torch.int32, "seq_past"), _ptr(block_table, torch.int32, "page table"),
-        block_table.shape[1], k.shape[0], tile_seq.numel(), nh, nkv, hd, int(window or 0), _ptr(status, torch.int32, "status"), _stream()),
-        "attn_prefill_kv8")
+    pools = (_ptr(k, _E4M3, "keys"), _ptr(v, _E4M3, "values"), _ptr(exps, torch.uint8, "exponents"), _ptr(out, torch.bfloat16, "out"),
+             _ptr(tile_seq, torch.int32, "tile_seq"), _ptr(tile_first, torch.int32, "tile_first"), _ptr(seq_start, torch.int32, "seq_start"),
+             _ptr(seq_past, torch.int32, "seq_past"), _ptr(block_table, torch.int32, "page table"), block_table.shape[1], k.shape[0],
+             tile_seq.numel(), nh, nkv, hd, int(window or 0), _ptr(status, torch.int32, "status"), _stream())
+    if hd <= 128:                      # scores and weighted values in tensor memory
+        _check(_fn("kv8", "esp_attn_prefill_kv8")(_ptr(q, torch.bfloat16, "q"), q.shape[0], *pools), "attn_prefill_kv8")
+    else:                              # the streaming kernel, sixteen rows a block
+        _check(_fn("kv8", "esp_attn_run_kv8")(_ptr(q, torch.bfloat16, "q"), *pools), "attn_prefill_kv8")

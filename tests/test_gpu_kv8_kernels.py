@@ -369,6 +369,12 @@ PREFILL = [
     (2, 2, 192, [140], [30], 0),
     (2, 1, 256, [129, 20], [0, 200], 50),
     (1, 1, 128, [1500], [700], 0),
+    # enough (tile, head) items that two tiles of a sequence go together
+    (32, 4, 64, [1300, 700, 129, 64], [0, 333, 5, 1000], 0),
+    (48, 16, 128, [1030, 400], [70, 0], 0),
+    (40, 8, 128, [1700, 130, 1, 300], [200, 1000, 64, 0], 260),
+    (60, 60, 104, [1281], [0], 1),
+    (48, 3, 24, [900, 900], [3, 60], 1000),
 ]
 
 
