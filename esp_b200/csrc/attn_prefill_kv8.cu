@@ -2,7 +2,7 @@
 // windowed, grouped query heads, runs of unequal length packed back to back.  Heads of up to 128 channels.
 //
 //   S = Q K^T      tcgen05.mma, 128 queries by 128 keys, accumulated in 32-bit in tensor memory
-//   P = 2^(S log2(e) / sqrt(hd) - m)   in 32-bit, by the thread that owns the row; rounded to bfloat16 and written over S, where the next
+//   P = 2^(S log2(e) / sqrt(hd) - m)   in 32-bit, by two threads a row; rounded to bfloat16 and written over S, where the next
 //                  product reads it as its A operand
 //   O += P V       tcgen05.mma, accumulated in tensor memory
 //
@@ -25,9 +25,11 @@ namespace {
 using namespace tc05;
 constexpr int BM = 128, BN = 128, ATOM = 128 * 128;     // ATOM: bytes of a 64-channel slice of 128 rows
 constexpr int STAGES = 2;                               // blocks of keys (and of values) in shared memory as bfloat16
-// warps: 0-3 and 4-7 the groups of row threads, 8-11 codes to bfloat16, 12 MMA, 13 queries, 14 and 15 none.  Registers are moved
-// between them (whole groups of four warps): 256 * 176 + 128 * 96 + 128 * 64 = 65,536, the launch's 512 * 128.
-constexpr int ROW_WARPS = 8, CONV_WARPS = 4, MMA_WARP = 12, Q_WARP = 13, THREADS = 512;
+// warps: 0-7 and 8-15 the groups of row threads (two threads a row), 16-23 codes to bfloat16, 24 MMA, 25 queries, 26 pages and
+// exponents, 27 none.  Registers are moved between them (whole groups of four warps): 512 * 80 + 256 * 64 + 128 * 56 = 64,512,
+// the launch's 896 * 72.
+constexpr int ROW_WARPS = 16, CONV_WARPS = 8, MMA_WARP = 24, Q_WARP = 25, PAGE_WARP = 26, THREADS = 896;
+constexpr int AHEAD = 4;                                // blocks of keys whose pages and exponents are known ahead
 constexpr int LIST = 4096;                              // tiles of a launch
 constexpr float LAZY = 8.f;
 
@@ -40,19 +42,29 @@ struct Params {
     int* status;
 };
 
-__device__ __forceinline__ unsigned idesc_attn(int n, bool b_mn_major) {
+__host__ __device__ constexpr unsigned idesc_attn(int n, bool b_mn_major) {
     return (1u << 4) | (1u << 7) | (1u << 10) | (b_mn_major ? (1u << 16) : 0u) | ((unsigned)(n >> 3) << 17) | ((unsigned)(128 >> 4) << 24);
 }
-// an MN-major operand: rows are consecutive keys, 128 bytes of channels each; the next 64 channels lie ``lbo`` bytes further
-__device__ __forceinline__ unsigned long long smem_desc_mn(const void* p, unsigned lbo) {
-    unsigned long long d = 0;
-    d |= (unsigned long long)((smem_u32(p) & 0x3FFFFu) >> 4);
-    d |= (unsigned long long)((lbo >> 4) & 0x3FFFu) << 16;
-    d |= (unsigned long long)(1024 >> 4) << 32;
-    d |= (unsigned long long)1 << 46;
-    d |= (unsigned long long)2 << 61;
-    return d;
+// Operand descriptors (128-byte swizzle, groups of 8 rows 1,024 bytes apart): the high word is the same for all, the low word
+// holds the address and, for an MN-major operand (rows are keys, 128 bytes of channels each), how far the next 64
+// channels lie.
+constexpr unsigned DESC_HIGH = (1024u >> 4) | (1u << 14) | (2u << 29);
+__device__ __forceinline__ unsigned desc_low(unsigned addr, unsigned next) { return ((addr & 0x3FFFFu) >> 4) | (next >> 4) << 16; }
+// D += A B with A in tensor memory
+__device__ __forceinline__ void tc_mma_ta_lo(unsigned tmem_d, unsigned tmem_a, unsigned b_lo, unsigned idesc, unsigned accumulate) {
+    asm volatile(
+        "{\n.reg .pred p;\n.reg .b64 db;\n"
+        "setp.ne.b32 p, %5, 0;\n"
+        "mov.b64 db, {%2, %3};\n"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], db, %4, p;\n}\n"
+        ::"r"(tmem_d), "r"(tmem_a), "r"(b_lo), "r"(DESC_HIGH), "r"(idesc), "r"(accumulate) : "memory");
 }
+__device__ __forceinline__ bool elect_one() {
+    unsigned r;
+    asm volatile("{\n.reg .pred p;\nelect.sync _|p, 0xffffffff;\nselp.u32 %0, 1, 0, p;\n}\n" : "=r"(r));
+    return r != 0;
+}
+__device__ __forceinline__ int uniform(int x) { return __shfl_sync(0xffffffffu, x, 0); }
 __device__ __forceinline__ float fast_exp2(float x) {
     float y;
     asm("ex2.approx.ftz.f32 %0, %1;\n" : "=f"(y) : "f"(x));
@@ -81,6 +93,15 @@ __device__ __forceinline__ void tc_ask32(unsigned taddr, unsigned (&r)[32]) {
           "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
         : "r"(taddr));
 }
+__device__ __forceinline__ void tc_ld8(unsigned taddr, unsigned (&r)[8]) {
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];\n"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]) : "r"(taddr));
+    asm volatile("tcgen05.wait::ld.sync.aligned;\n" : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7])::"memory");
+}
+__device__ __forceinline__ void tc_st8(unsigned taddr, const unsigned (&r)[8]) {
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};\n"
+                 ::"r"(taddr), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]) : "memory");
+}
 // the loads have arrived: their registers pass through here, so that no use is moved ahead of the wait
 __device__ __forceinline__ void tc_wait_ld(unsigned (&r)[32]) {
     asm volatile("tcgen05.wait::ld.sync.aligned;\n"
@@ -102,6 +123,15 @@ __device__ __forceinline__ unsigned mul_bf16x2(unsigned a, unsigned b) {
     return r;
 }
 
+// What the converting warps are told of a block of keys: its two pages' places in the pools ((page * nkv + head), -1: none), the
+// rows that exist for the item, and the exponents of the pages' keys and values.
+template <int R> struct Word;
+template <> struct Word<4> { typedef unsigned type; };
+template <> struct Word<2> { typedef unsigned short type; };
+struct Entry {
+    int block[2], lo, hi;                               // hi -1: no more work
+    unsigned char exps[2][2][KV8_PAGE];
+};
 // What a block works on: one or two tiles of 128 query rows of a head.
 struct Item {
     int seq, h, kvh, row0, first, news, past, blk0, nb, key_lo, key_hi;
@@ -140,14 +170,17 @@ __global__ void __launch_bounds__(THREADS, 1) attn_prefill_kv8_kernel(const __gr
     unsigned char* v_s = k_s + STAGES * TILE;            // [STAGES]
     unsigned long long* bars = reinterpret_cast<unsigned long long*>(v_s + STAGES * TILE);
     unsigned long long *q_full = bars, *q_empty = bars + 1, *drained = bars + 2, *s_full = bars + 4, *p_ready = bars + 6, *o_full = bars + 8,
-                       *o_free = bars + 10, *k_full = bars + 12, *k_empty = k_full + STAGES, *v_full = k_empty + STAGES, *v_empty = v_full + STAGES;
-    constexpr int N_BARS = 12 + 4 * STAGES;
+                       *o_free = bars + 10, *k_full = bars + 12, *k_empty = k_full + STAGES, *v_full = k_empty + STAGES, *v_empty = v_full + STAGES,
+                       *e_full = v_empty + STAGES, *e_empty = e_full + AHEAD;
+    constexpr int N_BARS = 12 + 4 * STAGES + 2 * AHEAD;
     unsigned* tmem_slot = reinterpret_cast<unsigned*>(bars + N_BARS);
     volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
     int* n_active = reinterpret_cast<int*>(tmem_slot + 2);
-    float* xsum = reinterpret_cast<float*>(bars + 32);   // [group][row]: the groups' sums where they share a tile
-    float* xref = xsum + 2 * 128;                        // [group][row]: the maxima that they go with
-    unsigned short* list = reinterpret_cast<unsigned short*>(xref + 2 * 128);
+    float* xmax = reinterpret_cast<float*>(bars + 32);   // [group][parity][side][row]: maxima of a block
+    float* xsum = xmax + 2 * 2 * 2 * 128;                // [group][side][row]: sums at the item's end
+    float* xref = xsum + 2 * 2 * 128;                    // [group][row]: the maxima that they go with
+    Entry* entries = reinterpret_cast<Entry*>(xref + 2 * 128);           // [AHEAD]
+    unsigned short* list = reinterpret_cast<unsigned short*>(entries + AHEAD);
     static_assert(N_BARS <= 30, "the barriers and three words take 256 bytes");
     if (reinterpret_cast<unsigned char*>(list + LIST) > smem_raw + p.smem_bytes) {
         if (threadIdx.x == 0) atomicOr(p.status, ESP_STATUS_SMEM_LAYOUT);
@@ -157,13 +190,14 @@ __global__ void __launch_bounds__(THREADS, 1) attn_prefill_kv8_kernel(const __gr
     if (threadIdx.x == 0) {
         for (int i = 0; i < N_BARS; i++) mbar_init(&bars[i], 1);
         for (int g = 0; g < 2; g++) {
-            mbar_init(&p_ready[g], 4);                   // a warp of the group's rows each
-            mbar_init(&o_free[g], 4);
+            mbar_init(&p_ready[g], 8);                   // a warp of the group's rows each
+            mbar_init(&o_free[g], 8);
         }
         for (int s = 0; s < STAGES; s++) {
             mbar_init(&k_full[s], CONV_WARPS);
             mbar_init(&v_full[s], CONV_WARPS);
         }
+        for (int s = 0; s < AHEAD; s++) mbar_init(&e_empty[s], CONV_WARPS);
         *abort_flag = 0;
         asm volatile("fence.mbarrier_init.release.cluster;\n" ::: "memory");
     }
@@ -188,12 +222,12 @@ __global__ void __launch_bounds__(THREADS, 1) attn_prefill_kv8_kernel(const __gr
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
-    const unsigned tmem = *tmem_slot, tm_s = tmem, tm_o = tmem + 256;    // S of the groups at columns 0 and 128, O at 256 and 384
+    const unsigned tmem = (unsigned)uniform((int)*tmem_slot), tm_s = tmem, tm_o = tmem + 256;    // S of the groups at columns 0 and 128, O at 256 and 384
     const int n_items = *n_active * p.nh, G = gridDim.x;
     // block b takes the items b, 2G-1-b, 2G+b, ...: a long one is followed by a short one
     auto item_of = [&](int round) { return round * G + ((round & 1) ? G - 1 - (int)blockIdx.x : (int)blockIdx.x); };
 
-    if (warp >= MMA_WARP) asm volatile("setmaxnreg.dec.sync.aligned.u32 64;\n");
+    if (warp >= MMA_WARP) asm volatile("setmaxnreg.dec.sync.aligned.u32 56;\n");
     if (warp == Q_WARP) {
         bool ok = true;
         int issued = 0;
@@ -218,232 +252,260 @@ __global__ void __launch_bounds__(THREADS, 1) attn_prefill_kv8_kernel(const __gr
             if (issued > 0) mbar_wait(q_full, (issued - 1) & 1);         // its copies land before the block ends
         }
     } else if (warp == MMA_WARP) {
-        if (lane == 0) {
-            const unsigned idesc_s = idesc_attn(BN, false), idesc_pv = idesc_attn(HD, true);
-            const unsigned long long dq = smem_desc(q_s), dk = smem_desc(k_s), dv = smem_desc_mn(v_s, ATOM);
-            bool ok = true;
-            int b0 = 0;                                                   // key blocks before this item
-            unsigned ph_p = 0, ph_o = 0;                                  // a bit a group: the phase of its P, of its O
-            for (int round = 0; ok && !*abort_flag; round++) {
-                const int item = item_of(round);
-                if (item >= n_items) break;
-                const Item t = load_item(p, list, item);
-                ok = mbar_wait(q_full, round & 1);
+        // The whole warp walks the blocks, so that what the MMAs are given is known to be the same for all lanes; one of them
+        // issues.  S of a block overwrites the P before it, so its group's P V comes first: the tensor core runs one
+        // thread's products in the order in which they were issued.
+        const bool leader = elect_one();
+        constexpr unsigned idesc_s = idesc_attn(BN, false), idesc_pv = idesc_attn(HD, true);
+        const unsigned dq = desc_low(smem_u32(q_s), 16), dk = desc_low(smem_u32(k_s), 16), dv = desc_low(smem_u32(v_s), ATOM);
+        bool ok = true;
+        int b0 = 0;                                                       // key blocks before this item
+        unsigned ph_p = 0, ph_o = 0;                                      // a bit a group: the phase of its P, of its O
+        for (int round = 0; ok; round++) {
+            const int item = item_of(round);
+            if (item >= n_items) break;
+            const Item t = load_item(p, list, item);
+            const int pair = uniform(t.pair), nb = uniform(t.nb), lo0 = uniform(t.lo(0, p.window)), hi0 = uniform(t.hi(0)),
+                      lo1 = uniform(t.lo(1, p.window)), hi1 = uniform(t.hi(1));
+            ok = __all_sync(0xffffffffu, mbar_wait(q_full, round & 1));
+            unsigned begun = 0;                                           // a bit a group: its O holds something of this item
+            auto issue_s = [&](const int g, int j, bool last_use, bool last) {
+                const int st = (b0 + j) % STAGES;
+                if (!__all_sync(0xffffffffu, !*abort_flag && mbar_wait(&k_full[st], ((b0 + j) / STAGES) & 1))) return false;
                 tc_fence_after();
-                unsigned begun = 0;                                       // a bit a group: its O holds something of this item
-                auto issue_s = [&](int g, int j, bool last_use, bool last) {
-                    const int st = (b0 + j) % STAGES;
-                    if (!mbar_wait(&k_full[st], ((b0 + j) / STAGES) & 1)) return false;
-                    tc_fence_after();
-                    const unsigned long long a = dq + (t.pair ? (unsigned)(g * TILE) >> 4 : 0u), b = dk + ((st * TILE) >> 4);
+                const unsigned qa = dq + (pair ? (unsigned)(g * TILE) >> 4 : 0u), kb = dk + ((unsigned)(st * TILE) >> 4);
+                if (leader) {
 #pragma unroll
                     for (int kk = 0; kk < HD / 16; kk++) {
                         const unsigned off = ((kk >> 2) * ATOM + (kk & 3) * 32) >> 4;
-                        tc_mma(tm_s + g * BN, a + off, b + off, idesc_s, kk > 0 ? 1u : 0u);
+                        tc_mma_lo(tm_s + g * BN, qa + off, kb + off, DESC_HIGH, idesc_s, kk > 0 ? 1u : 0u);
                     }
                     tc_commit(&s_full[g]);
                     if (last_use) tc_commit(&k_empty[st]);
                     if (last) tc_commit(q_empty);
-                    return true;
-                };
-                auto issue_pv = [&](int g, int j, bool last_use, bool last) {
-                    const int st = (b0 + j) % STAGES;
-                    // the row threads have read the O of the item before
-                    if (!(begun >> g & 1) && !mbar_wait(&o_free[g], (ph_o >> g & 1) ^ 1)) return false;
-                    if (!mbar_wait(&p_ready[g], ph_p >> g & 1) || !mbar_wait(&v_full[st], ((b0 + j) / STAGES) & 1)) return false;
-                    tc_fence_after();
-                    ph_p ^= 1u << g;
+                }
+                __syncwarp();
+                return true;
+            };
+            auto issue_pv = [&](const int g, int j, bool last_use, bool last) {
+                const int st = (b0 + j) % STAGES;
+                // the first P V of an item: the row threads have read the O of the item before
+                bool fine = !*abort_flag && ((begun >> g & 1) || mbar_wait(&o_free[g], (ph_o >> g & 1) ^ 1));
+                fine = fine && mbar_wait(&v_full[st], ((b0 + j) / STAGES) & 1) && mbar_wait(&p_ready[g], ph_p >> g & 1);
+                if (!__all_sync(0xffffffffu, fine)) return false;
+                tc_fence_after();
+                const unsigned vb = dv + ((unsigned)(st * TILE) >> 4), first = begun >> g & 1;
+                if (leader) {
 #pragma unroll
                     for (int kk = 0; kk < BN / 16; kk++)
-                        tc_mma_ta(tm_o + g * BN, tm_s + g * BN + kk * 8, dv + ((st * TILE + kk * 16 * 128) >> 4), idesc_pv, kk > 0 ? 1u : begun >> g & 1);
-                    if (!(begun >> g & 1)) ph_o ^= 1u << g;
-                    begun |= 1u << g;
+                        tc_mma_ta_lo(tm_o + g * BN, tm_s + g * BN + (kk >> 2) * 64 + (kk & 3) * 8, vb + ((kk * 16 * 128) >> 4), idesc_pv, kk > 0 ? 1u : first);
                     if (last_use) tc_commit(&v_empty[st]);
                     if (last) tc_commit(&o_full[g]);
-                    return true;
-                };
-                // S of a block overwrites the P before it, so its group's P V comes first: the tensor core runs one
-                // thread's products in the order in which they were issued
-                if (t.pair) {
-                    const int lo0 = t.lo(0, p.window), hi0 = t.hi(0), lo1 = t.lo(1, p.window), hi1 = t.hi(1);
-                    for (int j = 0; j <= t.nb && ok && !*abort_flag; j++) {
-                        if (ok && j - 1 >= lo0 && j - 1 <= hi0) ok = issue_pv(0, j - 1, j - 1 < lo1, j - 1 == hi0);
-                        if (ok && j >= lo0 && j <= hi0) ok = issue_s(0, j, j < lo1, false);
-                        if (ok && j - 1 >= lo1 && j - 1 <= hi1) ok = issue_pv(1, j - 1, true, j - 1 == hi1);
-                        if (ok && j >= lo1 && j <= hi1) ok = issue_s(1, j, true, j == hi1);
-                    }
-                } else {
-                    for (int j = 0; j < t.nb + 2 && ok && !*abort_flag; j++) {
-                        if (j >= 2) ok = issue_pv(j & 1, j - 2, true, j >= t.nb);
-                        if (ok && j < t.nb) ok = issue_s(j & 1, j, true, j + 1 == t.nb);
-                    }
                 }
-                b0 += t.nb;
+                __syncwarp();
+                ph_p ^= 1u << g;
+                if (!first) ph_o ^= 1u << g;
+                begun |= 1u << g;
+                return true;
+            };
+            if (pair) {
+                for (int j = 0; j <= nb && ok; j++) {
+                    if (ok && j - 1 >= lo0 && j - 1 <= hi0) ok = issue_pv(0, j - 1, j - 1 < lo1, j - 1 == hi0);
+                    if (ok && j >= lo0 && j <= hi0) ok = issue_s(0, j, j < lo1, false);
+                    if (ok && j - 1 >= lo1 && j - 1 <= hi1) ok = issue_pv(1, j - 1, true, j - 1 == hi1);
+                    if (ok && j >= lo1 && j <= hi1) ok = issue_s(1, j, true, j == hi1);
+                }
+            } else {
+                for (int j = 0; j < nb + 2 && ok; j++) {
+                    if (j >= 2) ok = j & 1 ? issue_pv(1, j - 2, true, j >= nb) : issue_pv(0, j - 2, true, j >= nb);
+                    if (ok && j < nb) ok = j & 1 ? issue_s(1, j, true, j + 1 == nb) : issue_s(0, j, true, j + 1 == nb);
+                }
             }
-            if (!ok) {
+            b0 += nb;
+        }
+        if (!ok || *abort_flag) {
+            if (leader) {
                 atomicOr(p.status, ESP_STATUS_WAIT_EXPIRED);
                 *abort_flag = 1;
-            }
-            if (!ok || *abort_flag) {                                    // its products end before tensor memory is given back
-                tc_commit(drained);
+                tc_commit(drained);                                       // its products end before tensor memory is given back
                 mbar_wait(drained, 0);
             }
+            __syncwarp();
+        }
+    } else if (warp == PAGE_WARP) {
+        // ---- the blocks' pages and exponents, ahead of the warps that convert them
+        bool ok = true;
+        int n = 0;                                                        // entries so far
+        for (int round = 0; ok; round++) {
+            const int item = item_of(round);
+            const bool end = item >= n_items;
+            Item t{};
+            if (!end) t = load_item(p, list, item);
+            int place = -1;                                               // this lane's page of 16 blocks, as its place in the pools
+            for (int j = 0; j < (end ? 1 : t.nb) && ok; j++, n++) {
+                if ((j & 15) == 0 && !end) {
+                    const int page_idx = (t.blk0 + j) * 2 + lane;
+                    place = -1;
+                    if (page_idx <= t.key_hi / KV8_PAGE && page_idx >= t.key_lo / KV8_PAGE) {
+                        const int page = p.block_table[(size_t)t.seq * p.table_stride + page_idx];
+                        if (page >= 0 && page < p.n_pages) place = page * p.nkv + t.kvh;
+                        else atomicOr(p.status, ESP_STATUS_BAD_INDEX);
+                    }
+                }
+                const int mine = __shfl_sync(0xffffffffu, place, ((j & 15) * 2 + (lane >> 4)) & 31), s = n % AHEAD;
+                uint2 e = make_uint2(0u, 0u);                             // 16 lanes a page, 8 exponents each
+                if (!end && mine >= 0) e = *reinterpret_cast<const uint2*>(p.exps + (size_t)mine * 2 * KV8_PAGE + (lane & 15) * 8);
+                ok = __all_sync(0xffffffffu, !*abort_flag && mbar_wait(&e_empty[s], ((n / AHEAD) & 1) ^ 1));
+                if (!ok) break;
+                Entry& x = entries[s];
+                *reinterpret_cast<uint2*>(&x.exps[lane >> 4][0][0] + (lane & 15) * 8) = e;
+                if ((lane & 15) == 0) x.block[lane >> 4] = mine;
+                if (lane == 0) {
+                    const int key0 = (t.blk0 + j) * BN;
+                    x.lo = max(0, t.key_lo - key0);
+                    x.hi = end ? -1 : min(BN, t.key_hi + 1 - key0);
+                }
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&e_full[s]);
+            }
+            if (end) break;
+        }
+        if (!ok && lane == 0) {
+            atomicOr(p.status, ESP_STATUS_WAIT_EXPIRED);
+            *abort_flag = 1;
         }
     } else if (warp >= MMA_WARP) {
-        // no work: two of the four warps whose registers went to the others
+        // no work: its registers went to the others
     } else if (warp >= ROW_WARPS) {
-        asm volatile("setmaxnreg.dec.sync.aligned.u32 96;\n");
         // ---- codes to bfloat16.  A thread has a 16-channel piece c of R rows that follow one another (their exponents are one
         // load), and takes them in an order in which eight lanes' stores fall into different banks: half of the lanes
-        // are at an odd row while the others are at an even one.  Units of work, one behind the other: the keys of
-        // block 0, then keys of block i and values of block i - 1 in turn.  A piece's registers get the next unit's codes as
-        // soon as they have been converted.
+        // are at an odd row while the others are at an even one.  Keys and values of the blocks in turn; the codes of the next are
+        // asked for when one has been converted, all together: a load asked for between two pieces would be waited for with
+        // the next piece's, as a warp can tell only a few loads apart (418 cycles a piece).
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 64;\n");
         const int t = threadIdx.x - ROW_WARPS * 32;
-        constexpr int R = HD == 128 ? 8 : 4;
+        constexpr int R = HD == 128 ? 4 : 2;
         const int odd = (t >> 2) & 1, c = HD == 128 ? (t & 3) | ((t >> 1) & 4) : t & 3, row_lo = R * (HD == 128 ? (t >> 4) * 2 + odd : t >> 2);
         const bool whole_pieces = p.hd % 16 == 0;
-        const int live_lo = c * 16 < p.hd, live_hi = c * 16 + 8 < p.hd;   // the piece's halves that the heads have
-        struct Cursor {
-            int round, u, seq, kvh, blk0, nb, key_lo, key_hi;
-            bool done;
-            __device__ __forceinline__ bool is_v() const { return u == 2 * nb - 1 || (u > 0 && (u & 1) == 0); }
-            __device__ __forceinline__ int block() const { return u == 0 ? 0 : u == 2 * nb - 1 ? nb - 1 : (u & 1) ? (u + 1) / 2 : u / 2 - 1; }
-        };
-        auto open = [&](Cursor& cu, int round) {
-            const int item = item_of(round);
-            cu.done = item >= n_items;
-            cu.round = round;
-            cu.u = 0;
-            if (cu.done) return;
-            const Item it = load_item(p, list, item);
-            cu.seq = it.seq, cu.kvh = it.kvh, cu.blk0 = it.blk0, cu.nb = it.nb, cu.key_lo = it.key_lo, cu.key_hi = it.key_hi;
-        };
-        auto next = [&](Cursor& cu) {
-            if (!cu.done && ++cu.u == 2 * cu.nb) open(cu, cu.round + 1);
-        };
-        // this thread's page of a unit; -1: no rows of it are to be read
-        auto page_of = [&](const Cursor& cu) {
-            if (cu.done) return -1;
-            const int key = (cu.blk0 + cu.block()) * BN + row_lo;
-            if (key > cu.key_hi || key + R <= cu.key_lo) return -1;
-            const int page = p.block_table[(size_t)cu.seq * p.table_stride + key / KV8_PAGE];
-            if (page >= 0 && page < p.n_pages) return page;
-            atomicOr(p.status, ESP_STATUS_BAD_INDEX);
-            return -1;
-        };
-        struct Unit {                                                    // where a unit's rows are, and their exponents
-            const unsigned char* src;
-            unsigned rows;                                               // a bit for every row that is to be read
-            unsigned long long ke, ve;
-        };
-        auto unit_of = [&](const Cursor& cu, int page) {
-            Unit x{nullptr, 0u, 0ull, 0ull};
-            if (page < 0) return x;
-            const int key = (cu.blk0 + cu.block()) * BN + row_lo;
-            const int a = max(0, cu.key_lo - key), b = min(R, cu.key_hi + 1 - key);
-            x.rows = ((1u << b) - 1u) & ~((1u << a) - 1u);
-            const size_t block = (size_t)page * p.nkv + cu.kvh;
-            x.src = (cu.is_v() ? p.v : p.k) + (block * KV8_PAGE + key % KV8_PAGE) * p.hd + c * 16;
-            const unsigned char* e = p.exps + block * 2 * KV8_PAGE + key % KV8_PAGE;
-            if constexpr (R == 8) {
-                x.ke = *reinterpret_cast<const unsigned long long*>(e);
-                x.ve = *reinterpret_cast<const unsigned long long*>(e + KV8_PAGE);
+        const bool live_lo = c * 16 < p.hd, live_hi = c * 16 + 8 < p.hd;  // the piece's halves that the heads have
+        // row r of the piece goes to at ^ (r * 144) and its second half to that ^ 16: row r lies 128 r bytes further, its
+        // 16-byte pieces swapped by r
+        const unsigned to = (HD == 128 ? (c >> 2) * ATOM : 0) + row_lo * 128 + (((c & 3) * 2) << 4 ^ (row_lo & 7) << 4);
+        const int half = row_lo / KV8_PAGE, in_page = row_lo % KV8_PAGE;
+        // asks for a block's keys or values
+        auto ask = [&](uint4 (&w)[R], const Entry& x, const unsigned char* pool) {
+            const int block = x.block[half], a = x.lo - row_lo, b = x.hi - row_lo;
+            const unsigned char* from = pool + ((size_t)max(block, 0) * KV8_PAGE + in_page) * p.hd + c * 16;
+            if (block >= 0 && a <= 0 && b >= R && p.hd == HD) {
+#pragma unroll
+                for (int i = 0; i < R; i++) w[i] = *reinterpret_cast<const uint4*>(from + (i ^ odd) * HD);
             } else {
-                x.ke = *reinterpret_cast<const unsigned*>(e);
-                x.ve = *reinterpret_cast<const unsigned*>(e + KV8_PAGE);
-            }
-            return x;
-        };
-        auto read = [&](const Unit& x, int i) {
-            uint4 w = make_uint4(0u, 0u, 0u, 0u);
-            const int r = i ^ odd;
-            if (x.rows >> r & 1) {
-                const unsigned char* from = x.src + (size_t)r * p.hd;
-                if (whole_pieces) {
-                    if (live_lo) w = *reinterpret_cast<const uint4*>(from);
-                } else {
-                    if (live_lo) {
-                        const uint2 y = *reinterpret_cast<const uint2*>(from);
-                        w.x = y.x, w.y = y.y;
-                    }
-                    if (live_hi) {
-                        const uint2 y = *reinterpret_cast<const uint2*>(from + 8);
-                        w.z = y.x, w.w = y.y;
+#pragma unroll
+                for (int i = 0; i < R; i++) {
+                    const int r = i ^ odd;
+                    const bool there = block >= 0 && r >= a && r < b;
+                    w[i] = make_uint4(0u, 0u, 0u, 0u);
+                    if (whole_pieces) {
+                        if (there && live_lo) w[i] = *reinterpret_cast<const uint4*>(from + r * p.hd);
+                    } else {
+                        uint2 y = make_uint2(0u, 0u), z = y;
+                        if (there && live_lo) y = *reinterpret_cast<const uint2*>(from + r * p.hd);
+                        if (there && live_hi) z = *reinterpret_cast<const uint2*>(from + r * p.hd + 8);
+                        w[i] = make_uint4(y.x, y.y, z.x, z.y);
                     }
                 }
             }
-            return w;
         };
-        Cursor cur, nxt;
-        open(cur, 0);
-        nxt = cur;
-        next(nxt);
-        Unit now = unit_of(cur, page_of(cur)), then;
-        int page_then = page_of(nxt);
-        uint4 buf[R];
+        // the codes times their powers of two, to the stage at ``at``
+        auto convert = [&](const uint4 (&codes)[R], const Entry& x, const bool is_v, unsigned at) {
+            typedef typename Word<R>::type Exps;                          // a byte for each of the thread's rows
+            const unsigned ke = *reinterpret_cast<const Exps*>(&x.exps[half][0][in_page]), ve = *reinterpret_cast<const Exps*>(&x.exps[half][1][in_page]);
+            // else: a position that is no number, or 2^(120 + e) beyond a bfloat16
+            const bool plain = !__vcmpgtu4(ke, 0x86868686u) && !__vcmpgtu4(ve, 0x86868686u);
+            if (__all_sync(0xffffffffu, plain)) {
 #pragma unroll
-        for (int i = 0; i < R; i++) buf[i] = read(now, i);
-        int n_k = 0, n_v = 0;
-        bool ok = true;
-        while (!cur.done) {
-            const bool is_v = cur.is_v();
-            int& n = is_v ? n_v : n_k;
-            const int st = n % STAGES;
-            then = unit_of(nxt, page_then);
-            ok = !*abort_flag && mbar_wait(is_v ? &v_empty[st] : &k_empty[st], ((n / STAGES) & 1) ^ 1);
-            if (!__all_sync(0xffffffffu, ok)) {
-                ok = false;
-                break;
-            }
-            unsigned char* dst = (is_v ? v_s : k_s) + st * TILE + (HD == 128 ? (c >> 2) * ATOM : 0);
-            const int piece = (c & 3) * 2;
+                for (int i = 0; i < R; i++) {
+                    const unsigned word = is_v ? ve : ke;
+                    // the byte of row i ^ odd, and 2^(120 + e) twice
+                    const unsigned f = ((odd ? word >> (8 * (i ^ 1)) : word >> (8 * i)) & 255u) * 0x00800080u + 0x3c003c00u;
+                    const unsigned w[4] = {codes[i].x, codes[i].y, codes[i].z, codes[i].w};
+                    unsigned o[8];
 #pragma unroll
-            for (int i = 0; i < R; i++) {
-                const int r = i ^ odd, row = row_lo + r;
-                const int ke = (int)(now.ke >> (8 * r)) & 255, ve = (int)(now.ve >> (8 * r)) & 255;
-                const bool bad = (ke == KV8_NAN || ve == KV8_NAN) && (now.rows >> r & 1);
-                const int byte = is_v ? ve : ke, up = byte + 120, more = max(up - 254, 0);
-                // 2^(120 + e), in two factors where one bfloat16 does not hold it; a position that is no number: NaN, 0
-                unsigned f = (unsigned)(up - more) << 7;
-                f = bad ? (is_v ? 0u : 0x7fffu) : f;
-                f |= f << 16;
-                unsigned o[8];
-                const unsigned w[4] = {buf[i].x, buf[i].y, buf[i].z, buf[i].w};
-#pragma unroll
-                for (int u = 0; u < 4; u++) {
-                    o[2 * u] = mul_bf16x2(spread_codes<0x9180>(w[u]), f);
-                    o[2 * u + 1] = mul_bf16x2(spread_codes<0xB3A2>(w[u]), f);
+                    for (int u = 0; u < 4; u++) {
+                        o[2 * u] = mul_bf16x2(spread_codes<0x9180>(w[u]), f);
+                        o[2 * u + 1] = mul_bf16x2(spread_codes<0xB3A2>(w[u]), f);
+                    }
+                    const unsigned dst = at ^ (unsigned)((i ^ odd) * 144);
+                    asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};\n" ::"r"(dst), "r"(o[0]), "r"(o[1]), "r"(o[2]), "r"(o[3]) : "memory");
+                    asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};\n" ::"r"(dst ^ 16u), "r"(o[4]), "r"(o[5]), "r"(o[6]), "r"(o[7]) : "memory");
                 }
-                if (more > 0 && !bad) {
-                    const unsigned f2 = (unsigned)(127 + more) << 7, ff = f2 | f2 << 16;
+            } else {
 #pragma unroll
-                    for (int u = 0; u < 8; u++) o[u] = mul_bf16x2(o[u], ff);
+                for (int i = 0; i < R; i++) {
+                    const int r = i ^ odd;
+                    const unsigned k8 = ke >> (8 * r) & 255u, v8 = ve >> (8 * r) & 255u;
+                    const bool bad = (k8 == KV8_NAN || v8 == KV8_NAN) && r >= x.lo - row_lo && r < x.hi - row_lo;
+                    const int up = (int)(is_v ? v8 : k8) + 120, more = max(up - 254, 0);   // two factors
+                    unsigned f = (unsigned)(up - more) << 7, f2 = (unsigned)(127 + more) << 7;
+                    f = bad ? (is_v ? 0u : 0x7fffu) : f;                  // a key of NaN with a value of zeros
+                    f2 = bad ? 0x3f80u : f2;
+                    f |= f << 16;
+                    f2 |= f2 << 16;
+                    const unsigned w[4] = {codes[i].x, codes[i].y, codes[i].z, codes[i].w};
+                    unsigned o[8];
+#pragma unroll
+                    for (int u = 0; u < 4; u++) {
+                        o[2 * u] = mul_bf16x2(mul_bf16x2(spread_codes<0x9180>(w[u]), f), f2);
+                        o[2 * u + 1] = mul_bf16x2(mul_bf16x2(spread_codes<0xB3A2>(w[u]), f), f2);
+                    }
+                    const unsigned dst = at ^ (unsigned)(r * 144);
+                    asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};\n" ::"r"(dst), "r"(o[0]), "r"(o[1]), "r"(o[2]), "r"(o[3]) : "memory");
+                    asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};\n" ::"r"(dst ^ 16u), "r"(o[4]), "r"(o[5]), "r"(o[6]), "r"(o[7]) : "memory");
                 }
-                unsigned char* at = dst + row * 128;
-                *reinterpret_cast<uint4*>(at + ((piece ^ (row & 7)) << 4)) = make_uint4(o[0], o[1], o[2], o[3]);
-                *reinterpret_cast<uint4*>(at + (((piece + 1) ^ (row & 7)) << 4)) = make_uint4(o[4], o[5], o[6], o[7]);
-                buf[i] = read(then, i);
             }
-            n++;
+        };
+        auto wait_all = [&](unsigned long long* bar, int parity) { return (bool)__all_sync(0xffffffffu, !*abort_flag && mbar_wait(bar, parity)); };
+        uint4 codes[R];
+        bool ok = wait_all(&e_full[0], 0);
+        if (ok && entries[0].hi >= 0) ask(codes, entries[0], p.k);
+        for (int n = 0; ok; n++) {
+            const Entry& x = entries[n % AHEAD];
+            if (x.hi < 0) break;
+            const int st = n % STAGES, free_parity = ((n / STAGES) & 1) ^ 1;
+            ok = wait_all(&k_empty[st], free_parity);
+            if (!ok) break;
+            convert(codes, x, false, smem_u32(k_s) + st * TILE + to);
+            ask(codes, x, p.v);
             fence_async_smem();
             __syncwarp();
-            if (lane == 0) mbar_arrive(is_v ? &v_full[st] : &k_full[st]);
-            cur = nxt;
-            now = then;
-            next(nxt);
-            page_then = page_of(nxt);
+            if (lane == 0) mbar_arrive(&k_full[st]);
+            ok = wait_all(&v_empty[st], free_parity);
+            if (!ok) break;
+            convert(codes, x, true, smem_u32(v_s) + st * TILE + to);
+            const Entry& y = entries[(n + 1) % AHEAD];
+            ok = wait_all(&e_full[(n + 1) % AHEAD], ((n + 1) / AHEAD) & 1);
+            if (!ok) break;
+            if (y.hi >= 0) ask(codes, y, p.k);
+            fence_async_smem();
+            __syncwarp();
+            if (lane == 0) {
+                mbar_arrive(&v_full[st]);
+                mbar_arrive(&e_empty[n % AHEAD]);
+            }
         }
         if (!ok && lane == 0) {
             atomicOr(p.status, ESP_STATUS_WAIT_EXPIRED);
             *abort_flag = 1;
         }
     } else {
-        // ---- row threads: TMEM lane = query row
-        asm volatile("setmaxnreg.inc.sync.aligned.u32 176;\n");
-        const int quad = warp & 3, grp = warp >> 2, r = quad * 32 + lane;
+        // ---- row threads: TMEM lane = query row; two threads a row, each with 64 keys of a block
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 80;\n");
+        const int quad = warp & 3, side = (warp >> 2) & 1, grp = warp >> 3, r = quad * 32 + lane;
         const unsigned lane_sel = (unsigned)(quad * 32) << 16;
+        const int bar_grp = 1 + grp * 4 + quad, bar_row = 9 + quad;
         const float sc = p.scale_log2;
-        const unsigned s_addr = tm_s + grp * BN + lane_sel, o_addr = tm_o + grp * BN + lane_sel;
+        const unsigned s_addr = tm_s + grp * BN + lane_sel + side * 64;
+        const unsigned o_addr = tm_o + grp * BN + lane_sel;
         bool ok = true;
         unsigned n_b = 0, ph_o = 0;                                       // blocks so far; a bit a group: the phase of its O
         for (int round = 0; ok; round++) {
@@ -459,30 +521,43 @@ __global__ void __launch_bounds__(THREADS, 1) attn_prefill_kv8_kernel(const __gr
                 const int key0 = (t.blk0 + j) * BN;
                 ok = !*abort_flag && mbar_wait(&s_full[grp], n_b & 1);
                 ok = __all_sync(0xffffffffu, ok);
-                if (!ok) break;
                 tc_fence_after();
-                unsigned s[4][32];
-#pragma unroll
-                for (int c = 0; c < 4; c++) tc_ask32(s_addr + c * 32, s[c]);
-#pragma unroll
-                for (int c = 0; c < 4; c++) tc_wait_ld(s[c]);
-                if (key0 + BN - 1 > first_pos || key0 < key_first_last) {
-                    // live columns: c_lo .. c_lo + c_span, one unsigned comparison each
-                    const int c_lo = key_first - key0;
-                    const unsigned c_span = (unsigned)(pos - key_first);
-#pragma unroll
-                    for (int c = 0; c < 4; c++)
+                // live columns of an edge block: c_lo .. c_lo + c_span, one unsigned comparison each
+                const bool edge = key0 + BN - 1 > first_pos || key0 < key_first_last;
+                const int c_lo = key_first - key0 - side * 64;
+                const unsigned c_span = (unsigned)(pos - key_first);
+                // 32 scores at a time: the second half for its maximum, then the first, which stays; the second is read again when its
+                // weights are made.  (All 64 in registers would spill, and what shared memory leaves of L1 does not hold spills.)
+                unsigned s[32];
+                auto scores = [&](int at) {
+                    tc_ask32(s_addr + at, s);
+                    tc_wait_ld(s);
+                    if (edge) {
 #pragma unroll
                         for (int i = 0; i < 32; i++)
-                            if ((unsigned)(c * 32 + i - c_lo) > c_span) s[c][i] = 0xff800000u;
+                            if ((unsigned)(at + i - c_lo) > c_span) s[i] = 0xff800000u;
+                    }
+                };
+                float mx = -INFINITY;
+                if (ok) {
+                    float m4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+                    for (int half = 1; half >= 0; half--) {
+                        scores(half * 32);
+#pragma unroll
+                        for (int i = 0; i < 32; i += 8)
+#pragma unroll
+                            for (int u = 0; u < 4; u++) m4[u] = fmaxf(fmaxf(m4[u], __uint_as_float(s[i + u])), __uint_as_float(s[i + u + 4]));
+                    }
+                    mx = fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3]));
                 }
-                float m4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-#pragma unroll
-                for (int i = 0; i < 32; i += 2)
-#pragma unroll
-                    for (int c = 0; c < 4; c++) m4[c] = fmaxf(fmaxf(m4[c], __uint_as_float(s[c][i])), __uint_as_float(s[c][i + 1]));
-                const float m_new = fmaxf(m_ref, fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3])) * sc);
-                const bool grew = m_new > m_ref + LAZY;
+                float* xp = xmax + (grp * 2 + (n_b & 1)) * 256;                      // by turns: one meeting a block is enough
+                xp[side * 128 + r] = mx;
+                ok = all_agree(ok, bar_grp, 64);                                     // the row's two threads go on or leave together
+                if (!ok) break;
+                mx = fmaxf(mx, xp[(side ^ 1) * 128 + r]);
+                const float m_new = fmaxf(m_ref, mx * sc);
+                const bool grew = m_new > m_ref + LAZY;                              // the same for both threads of the row
                 if (j == j0) {
                     m_ref = m_new;
                 } else if (__any_sync(0xffffffffu, grew)) {
@@ -490,30 +565,33 @@ __global__ void __launch_bounds__(THREADS, 1) attn_prefill_kv8_kernel(const __gr
                     if (grew) m_ref = m_new;
                     l_run *= alpha;
 #pragma unroll 1
-                    for (int u = 0; u < HD; u += 16) {
-                        float x[16];
-                        unsigned y[16];
-                        tc_ld16(o_addr + u, x);
+                    for (int u = side * (HD / 2); u < (side + 1) * (HD / 2); u += 8) {
+                        unsigned x[8];
+                        tc_ld8(o_addr + u, x);
 #pragma unroll
-                        for (int i = 0; i < 16; i++) y[i] = __float_as_uint(x[i] * alpha);
-                        tc_st16(o_addr + u, y);
+                        for (int i = 0; i < 8; i++) x[i] = __float_as_uint(__uint_as_float(x[i]) * alpha);
+                        tc_st8(o_addr + u, x);
                     }
                 }
                 const float m_use = m_ref == -INFINITY ? 0.f : m_ref;
                 float l4[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-                for (int c = 0; c < 4; c++) {
-                    unsigned packed[16];
+                // the weights of 32 keys into 16 columns, over scores that have been read: P of the first 64 keys lies in the columns 0-31
+                // of S, that of the others in 64-95
+                auto weigh = [&](unsigned to) {
+                    unsigned packed[8];
 #pragma unroll
                     for (int i = 0; i < 32; i += 2) {
-                        const float a = fast_exp2(fmaf(__uint_as_float(s[c][i]), sc, -m_use)), b = fast_exp2(fmaf(__uint_as_float(s[c][i + 1]), sc, -m_use));
+                        const float a = fast_exp2(fmaf(__uint_as_float(s[i]), sc, -m_use)), b = fast_exp2(fmaf(__uint_as_float(s[i + 1]), sc, -m_use));
                         l4[i & 2] += a;
                         l4[(i & 2) + 1] += b;
                         __nv_bfloat162 w = __floats2bfloat162_rn(a, b);
-                        packed[i >> 1] = *reinterpret_cast<unsigned*>(&w);
+                        packed[(i >> 1) & 7] = *reinterpret_cast<unsigned*>(&w);
+                        if (i % 16 == 14) tc_st8(to + (i / 16) * 8, packed);
                     }
-                    tc_st16(s_addr + c * 16, packed);
-                }
+                };
+                weigh(s_addr);
+                scores(32);
+                weigh(s_addr + 16);
                 tc_wait_st();
                 l_run += (l4[0] + l4[1]) + (l4[2] + l4[3]);
                 tc_fence_before();                                                   // S has been read, P and O written
@@ -521,54 +599,51 @@ __global__ void __launch_bounds__(THREADS, 1) attn_prefill_kv8_kernel(const __gr
                 if (lane == 0) mbar_arrive(&p_ready[grp]);
             }
             if (!ok) break;
-            // ---- the item's end: with two tiles each group has its own, with one the two groups' results are joined
+            // ---- the item's end: the sum of the row's threads; with one tile for both groups their results are joined
             const bool both = !t.pair && t.nb > 1;
-            if (!t.pair) {
-                xsum[grp * 128 + r] = l_run;
-                xref[grp * 128 + r] = m_ref;
-            }
+            xsum[(grp * 2 + side) * 128 + r] = l_run;
+            if (side == 0) xref[grp * 128 + r] = m_ref;
             for (int g = 0; g < 2; g++)
                 if ((t.pair ? g == grp : g < t.nb) && ok) ok = !*abort_flag && mbar_wait(&o_full[g], ph_o >> g & 1);
             ph_o ^= t.pair || t.nb > 1 ? 3u : 1u;
-            ok = t.pair ? (bool)__all_sync(0xffffffffu, ok) : all_agree(ok, 1 + quad, 64);
+            ok = t.pair ? all_agree(ok, bar_grp, 64) : all_agree(ok, bar_row, 128);
             if (!ok) break;
             tc_fence_after();
             const bool live = r < t.rows(grp);
             bf16* orow = p.out + ((size_t)(t.row0 + (t.pair ? grp * BM : 0) + r) * p.nh + t.h) * p.hd;
             // a group without a key for this row counts 0 (and a row that is no number stays one: 0 * NaN)
+            const int g0 = t.pair ? grp : 0;
             const float m0 = t.pair ? m_ref : xref[r], m1 = both ? xref[128 + r] : -INFINITY, m_all = fmaxf(m0, m1);
             const float f0 = m0 == -INFINITY ? 0.f : fast_exp2(m0 - m_all), f1 = m1 == -INFINITY ? 0.f : fast_exp2(m1 - m_all);
-            float l = f0 * (t.pair ? l_run : xsum[r]);
-            if (both) l += f1 * xsum[128 + r];
+            float l = f0 * (xsum[g0 * 256 + r] + xsum[g0 * 256 + 128 + r]);
+            if (both) l += f1 * (xsum[256 + r] + xsum[384 + r]);
             const float inv = l == 0.f ? 0.f : 1.f / l;
-            const int col0 = t.pair ? 0 : grp * (HD / 2), cols = t.pair ? HD : HD / 2;      // what this thread writes
+            const int cols = t.pair ? HD / 2 : HD / 4, col0 = (t.pair ? side : grp * 2 + side) * cols;   // what this thread writes
             const unsigned from = t.pair ? o_addr : tm_o + lane_sel;
 #pragma unroll 1
-            for (int col = col0; col < col0 + cols; col += 16) {
-                float o[16];
-                tc_ld16(from + col, o);
+            for (int col = col0; col < col0 + cols; col += 8) {
+                unsigned x[8];
+                tc_ld8(from + col, x);
+                float o[8];
+#pragma unroll
+                for (int i = 0; i < 8; i++) o[i] = __uint_as_float(x[i]) * f0;
                 if (both) {
-                    float o1[16];
-                    tc_ld16(tm_o + BN + lane_sel + col, o1);
+                    tc_ld8(tm_o + BN + lane_sel + col, x);
 #pragma unroll
-                    for (int i = 0; i < 16; i++) o[i] = o[i] * f0 + o1[i] * f1;
-                } else {
-#pragma unroll
-                    for (int i = 0; i < 16; i++) o[i] *= f0;
+                    for (int i = 0; i < 8; i++) o[i] += __uint_as_float(x[i]) * f1;
                 }
-#pragma unroll
-                for (int i = 0; i < 16; i += 8) {
-                    if (!live || col + i >= p.hd) break;
+                if (live && col < p.hd) {
                     __nv_bfloat162 w[4];
 #pragma unroll
-                    for (int u = 0; u < 4; u++) w[u] = __floats2bfloat162_rn(o[i + 2 * u] * inv, o[i + 2 * u + 1] * inv);
-                    *reinterpret_cast<uint4*>(orow + col + i) = make_uint4(*reinterpret_cast<unsigned*>(&w[0]), *reinterpret_cast<unsigned*>(&w[1]),
-                                                                           *reinterpret_cast<unsigned*>(&w[2]), *reinterpret_cast<unsigned*>(&w[3]));
+                    for (int u = 0; u < 4; u++) w[u] = __floats2bfloat162_rn(o[2 * u] * inv, o[2 * u + 1] * inv);
+                    *reinterpret_cast<uint4*>(orow + col) = make_uint4(*reinterpret_cast<unsigned*>(&w[0]), *reinterpret_cast<unsigned*>(&w[1]),
+                                                                       *reinterpret_cast<unsigned*>(&w[2]), *reinterpret_cast<unsigned*>(&w[3]));
                 }
             }
             tc_fence_before();
-            if (t.pair) __syncwarp();
-            else named_sync(1 + quad, 64);                                           // both O's and the sums have been read
+            // the sums and O's have been read
+            if (t.pair) named_sync(bar_grp, 64);
+            else named_sync(bar_row, 128);
             if (lane == 0 && (t.pair || grp < t.nb)) mbar_arrive(&o_free[grp]);
         }
         if (!ok && lane == 0) {
@@ -606,7 +681,7 @@ int make_query_map(CUtensorMap* map, const void* base, long long rows, int nh, i
 
 template <int HD> int launch(const CUtensorMap& map_q, Params p, int device, cudaStream_t stream) {
     constexpr int TILE = HD / 64 * ATOM;
-    const size_t smem = 1024 + (size_t)(2 + 2 * STAGES) * TILE + 256 + 4 * 128 * 4 + LIST * 2;
+    const size_t smem = 1024 + (size_t)(2 + 2 * STAGES) * TILE + 256 + (8 + 4 + 2) * 128 * 4 + AHEAD * sizeof(Entry) + LIST * 2;
     static bool raised[64] = {false};
     static int sm_count[64] = {0};
     if (!raised[device]) {
