@@ -26,7 +26,7 @@ using namespace tc05;
 constexpr int BM = 128, BN = 128, ATOM = 128 * 128;     // ATOM: bytes of a 64-channel slice of 128 rows
 constexpr int STAGES = 2;                               // blocks of keys (and of values) in shared memory as bfloat16
 // warps: 0-7 and 8-15 the groups of row threads (two threads a row), 16-23 codes to bfloat16, 24 MMA, 25 queries, 26 pages and
-// exponents, 27 none.  Registers are moved between them (whole groups of four warps): 512 * 80 + 256 * 64 + 128 * 56 = 64,512,
+// exponents, 27 none.  Registers are moved between them (whole groups of four warps): 512 * 80 + 256 * 56 + 128 * 72 = 64,512,
 // the launch's 896 * 72.
 constexpr int ROW_WARPS = 16, CONV_WARPS = 8, MMA_WARP = 24, Q_WARP = 25, PAGE_WARP = 26, THREADS = 896;
 constexpr int AHEAD = 4;                                // blocks of keys whose pages and exponents are known ahead
@@ -69,6 +69,27 @@ __device__ __forceinline__ float fast_exp2(float x) {
     float y;
     asm("ex2.approx.ftz.f32 %0, %1;\n" : "=f"(y) : "f"(x));
     return y;
+}
+// two numbers by one instruction: (a, b) * m + c, and sum + (a, b)
+__device__ __forceinline__ unsigned long long pair_of(float a, float b) {
+    unsigned long long r;
+    asm("mov.b64 %0, {%1, %2};\n" : "=l"(r) : "f"(a), "f"(b));
+    return r;
+}
+__device__ __forceinline__ float2 parts_of(unsigned long long x) {
+    float2 r;
+    asm("mov.b64 {%0, %1}, %2;\n" : "=f"(r.x), "=f"(r.y) : "l"(x));
+    return r;
+}
+__device__ __forceinline__ unsigned long long fma_pair(unsigned long long a, unsigned long long m, unsigned long long c) {
+    unsigned long long r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;\n" : "=l"(r) : "l"(a), "l"(m), "l"(c));
+    return r;
+}
+__device__ __forceinline__ unsigned long long add_pair(unsigned long long a, unsigned long long b) {
+    unsigned long long r;
+    asm("add.rn.f32x2 %0, %1, %2;\n" : "=l"(r) : "l"(a), "l"(b));
+    return r;
 }
 __device__ __forceinline__ bool all_agree(bool ok, int id, int count) {
     unsigned all;
@@ -227,7 +248,7 @@ __global__ void __launch_bounds__(THREADS, 1) attn_prefill_kv8_kernel(const __gr
     // block b takes the items b, 2G-1-b, 2G+b, ...: a long one is followed by a short one
     auto item_of = [&](int round) { return round * G + ((round & 1) ? G - 1 - (int)blockIdx.x : (int)blockIdx.x); };
 
-    if (warp >= MMA_WARP) asm volatile("setmaxnreg.dec.sync.aligned.u32 56;\n");
+    if (warp >= MMA_WARP) asm volatile("setmaxnreg.dec.sync.aligned.u32 72;\n");
     if (warp == Q_WARP) {
         bool ok = true;
         int issued = 0;
@@ -382,7 +403,7 @@ __global__ void __launch_bounds__(THREADS, 1) attn_prefill_kv8_kernel(const __gr
         // are at an odd row while the others are at an even one.  Keys and values of the blocks in turn; the codes of the next are
         // asked for when one has been converted, all together: a load asked for between two pieces would be waited for with
         // the next piece's, as a warp can tell only a few loads apart (418 cycles a piece).
-        asm volatile("setmaxnreg.dec.sync.aligned.u32 64;\n");
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 56;\n");
         const int t = threadIdx.x - ROW_WARPS * 32;
         constexpr int R = HD == 128 ? 4 : 2;
         const int odd = (t >> 2) & 1, c = HD == 128 ? (t & 3) | ((t >> 1) & 4) : t & 3, row_lo = R * (HD == 128 ? (t >> 4) * 2 + odd : t >> 2);
@@ -574,16 +595,17 @@ __global__ void __launch_bounds__(THREADS, 1) attn_prefill_kv8_kernel(const __gr
                     }
                 }
                 const float m_use = m_ref == -INFINITY ? 0.f : m_ref;
-                float l4[4] = {0.f, 0.f, 0.f, 0.f};
+                unsigned long long l_pair = 0ull;
+                const unsigned long long sc2 = pair_of(sc, sc), m2 = pair_of(-m_use, -m_use);
                 // the weights of 32 keys into 16 columns, over scores that have been read: P of the first 64 keys lies in the columns 0-31
                 // of S, that of the others in 64-95
                 auto weigh = [&](unsigned to) {
                     unsigned packed[8];
 #pragma unroll
                     for (int i = 0; i < 32; i += 2) {
-                        const float a = fast_exp2(fmaf(__uint_as_float(s[i]), sc, -m_use)), b = fast_exp2(fmaf(__uint_as_float(s[i + 1]), sc, -m_use));
-                        l4[i & 2] += a;
-                        l4[(i & 2) + 1] += b;
+                        const float2 x = parts_of(fma_pair(pair_of(__uint_as_float(s[i]), __uint_as_float(s[i + 1])), sc2, m2));
+                        const float a = fast_exp2(x.x), b = fast_exp2(x.y);
+                        l_pair = add_pair(l_pair, pair_of(a, b));
                         __nv_bfloat162 w = __floats2bfloat162_rn(a, b);
                         packed[(i >> 1) & 7] = *reinterpret_cast<unsigned*>(&w);
                         if (i % 16 == 14) tc_st8(to + (i / 16) * 8, packed);
@@ -593,7 +615,8 @@ __global__ void __launch_bounds__(THREADS, 1) attn_prefill_kv8_kernel(const __gr
                 scores(32);
                 weigh(s_addr + 16);
                 tc_wait_st();
-                l_run += (l4[0] + l4[1]) + (l4[2] + l4[3]);
+                const float2 l2 = parts_of(l_pair);
+                l_run += l2.x + l2.y;
                 tc_fence_before();                                                   // S has been read, P and O written
                 __syncwarp();
                 if (lane == 0) mbar_arrive(&p_ready[grp]);
