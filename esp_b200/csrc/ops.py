@@ -1593,6 +1593,9 @@ def kv8_rope_append(qkv, bias, tok_seq, tok_pos, cos, sin, rot, q_out, k, v, exp
         raise Backend(f"kv8_rope_append: cosines and sines are not [positions, {rot // 2}]")
     if n == 0:
         return
+    for name, t in (("projection", qkv), ("bias", bias), ("cosines", cos if rot else None), ("sines", sin if rot else None)):
+        if t is not None and t.data_ptr() % 16:
+            raise Backend(f"kv8_rope_append: the {name} do not start on a multiple of 16 bytes")
     _kv8_check("kv8_rope_append", q_out, k if write_kv else None, v, exps, block_table, page, nh, nkv, hd,
                (("the bias", bias, qkv.shape[1]), ("tok_seq", tok_seq, n), ("tok_pos", tok_pos, n)))
     _check(_fn("kv8", "esp_kv8_append")(
