@@ -488,20 +488,20 @@ bool sizes_fit(int nh, int nkv, int hd) { return nkv > 0 && nh > 0 && nh % nkv =
 }  // namespace
 
 // One token row of the step per block row.  ``split``: key positions a block, a multiple of 64; n_splits * split covers
-// the longest row.  Scratch where n_splits > 1: part_o float [n_tokens, nh, n_splits, hd], part_ml float [n_tokens, nh, n_splits,
-// 2], counters int [n_tokens * nh], zero when the call starts and when it ends.  ``seq_past`` (may be null): per sequence
+// the longest row.  Where n_splits > 1: scratch float [n_tokens * nh * n_splits * (hd + 2)], counters
+// int [n_tokens * nh], zero when the call starts and when it ends.  ``seq_past`` (may be null): per sequence
 // of the step, the positions cached before it.
-ESP_API int esp_attn_decode_kv8(const void* q, const void* k, const void* v, const void* exps, void* out, float* part_o, float* part_ml,
-                                int* counters, const int* tok_seq, const int* tok_pos, const int* seq_past, const int* block_table,
+ESP_API int esp_attn_decode_kv8(const void* q, const void* k, const void* v, const void* exps, void* out, float* scratch, int* counters,
+                                const int* tok_seq, const int* tok_pos, const int* seq_past, const int* block_table,
                                 int table_stride, int n_pages, int n_tokens, int nh, int nkv, int hd, int window, int split, int n_splits,
                                 int* status, cudaStream_t stream) {
     if (n_tokens <= 0) return 0;
     if (!sizes_fit(nh, nkv, hd) || n_splits <= 0 || n_splits > 65535 || split < KV8_PAGE || split % KV8_PAGE || window < 0 ||
-        (n_splits > 1 && (!part_o || !part_ml || !counters)) || (long long)split * n_splits < (long long)table_stride * KV8_PAGE)
+        (n_splits > 1 && (!scratch || !counters)) || (long long)split * n_splits < (long long)table_stride * KV8_PAGE)
         return (int)cudaErrorInvalidValue;
     Params p{};
     p.q = (const bf16*)q, p.k = (const unsigned char*)k, p.v = (const unsigned char*)v, p.exps = (const unsigned char*)exps, p.out = (bf16*)out;
-    p.part_o = part_o, p.part_ml = part_ml, p.counters = counters, p.tok_seq = tok_seq, p.tok_pos = tok_pos, p.seq_past = seq_past;
+    p.part_o = scratch, p.part_ml = scratch ? scratch + (size_t)n_tokens * nh * n_splits * hd : nullptr, p.counters = counters, p.tok_seq = tok_seq, p.tok_pos = tok_pos, p.seq_past = seq_past;
     p.block_table = block_table, p.table_stride = table_stride, p.n_pages = n_pages, p.nh = nh, p.nkv = nkv, p.hd = hd, p.window = window;
     p.split_keys = split, p.n_splits = n_splits, p.status = status;
     p.scale_log2 = (float)(1.4426950408889634 / sqrt((double)hd));

@@ -112,7 +112,7 @@ _SIGNATURES = {
     "esp_attn_decode_diff": [P, P, P, P, P, P, P, P, P, P, P, c_int, c_int, c_int, c_int, c_int, c_int, c_int, c_int, c_int,
                              c_int, c_int, c_float, c_int, c_float, c_float, c_float, c_float, P, c_longlong, P, P],
     "esp_kv8_append": [P, P, P, P, P, P, c_int, c_int, P, P, P, P, P, c_int, c_int, c_int, c_int, c_int, c_int, c_int, P, P],
-    "esp_attn_decode_kv8": [P, P, P, P, P, P, P, P, P, P, P, P, c_int, c_int, c_int, c_int, c_int, c_int, c_int, c_int, c_int, P, P],
+    "esp_attn_decode_kv8": [P, P, P, P, P, P, P, P, P, P, P, c_int, c_int, c_int, c_int, c_int, c_int, c_int, c_int, c_int, P, P],
     "esp_attn_prefill_kv8": [P, c_longlong, P, P, P, P, P, P, P, P, P, c_int, c_int, c_int, c_int, c_int, c_int, c_int, P, P],
     "esp_attn_run_kv8": [P, P, P, P, P, P, P, P, P, P, c_int, c_int, c_int, c_int, c_int, c_int, c_int, P, P],
 }
@@ -1542,14 +1542,12 @@ def kv8_fits(hd: int, page: int = KV8_PAGE) -> bool:
     return hd % 8 == 0 and 0 < hd <= 256 and page == KV8_PAGE
 
 
-@functools.lru_cache(maxsize=64)
-def _sm_count(device: int) -> int:
-    return torch.cuda.get_device_properties(device).multi_processor_count
+_current_device = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)
 
 
-def _kv8_check(what, q, k, v, exps, block_table, page, nh, nkv, hd, vectors):
-    """What the three entry points refuse alike; ``vectors``: (name, tensor or None, least length)."""
-    if nh <= 0 or nkv <= 0 or nh % nkv or nh > 65535:
+def _kv8_refuse(what, q, k, v, exps, block_table, page, nh, nkv, hd, vectors, aligned):
+    """Says what is wrong with a call that an entry point below did not let through (or with one whose tensors live elsewhere)."""
+    if nh <= 0 or nkv <= 0 or nh % nkv or nh + 2 * nkv > 65535:
         raise Backend(f"{what}: {nh} query heads do not divide among {nkv} key/value heads")
     if not kv8_fits(hd, page):
         raise Backend(f"{what}: heads of {hd} channels in pages of {page}; they are multiples of 8 up to 256 in pages of {KV8_PAGE}")
@@ -1565,14 +1563,28 @@ def _kv8_check(what, q, k, v, exps, block_table, page, nh, nkv, hd, vectors):
     for name, t, least in vectors:
         if t is not None and t.numel() < least:
             raise Backend(f"{what}: {name} has {t.numel()} elements, {least} are needed")
-    for name, t, step in (("queries", q, 16), ("keys", k, 16), ("values", v, 16), ("exponents", exps, 16)):
-        if t is not None and t.data_ptr() % step:
-            raise Backend(f"{what}: the {name} do not start on a multiple of {step} bytes")
+    for name, t in aligned:
+        if t is not None and t.data_ptr() % 16:
+            raise Backend(f"{what}: {name} do not start on a multiple of 16 bytes")
     if not q.is_cuda:
         raise Backend(f"{what}: queries must live on the GPU; this library has no CPU path")
-    _stream()
-    if q.get_device() != torch.cuda.current_device() or q.get_device() != _device_index:
-        raise Backend(f"{what}: the queries live on {q.device}, kernels are launched on cuda:{_device_index}")
+    raise Backend(f"{what}: the queries live on {q.device}, kernels are launched on cuda:{_device_index} with cuda:{_current_device()} current")
+
+
+def _kv8_pools_fit(k, v, exps, block_table, page, nh, nkv, hd) -> bool:
+    shape = k.shape
+    return (hd % 8 == 0 and 0 < hd <= 256 and page == KV8_PAGE and nkv > 0 < nh and nh % nkv == 0 and nh + 2 * nkv <= 65535 and len(shape) == 4
+            and shape[1] == nkv and shape[2] == page and shape[3] == hd and v.shape == shape and exps.shape == (shape[0], nkv, 2, page)
+            and block_table.dim() == 2)
+
+
+def _kv8_here(q) -> bool:
+    """Whether a tensor lives on the device that launches go to."""
+    if not q.is_cuda:
+        return False
+    if _device_index is None:
+        _stream()
+    return q.get_device() == _device_index == _current_device()
 
 
 def kv8_rope_append(qkv, bias, tok_seq, tok_pos, cos, sin, rot, q_out, k, v, exps, block_table, page, nh, nkv, hd, write_kv, status):
@@ -1580,8 +1592,8 @@ def kv8_rope_append(qkv, bias, tok_seq, tok_pos, cos, sin, rot, q_out, k, v, exp
     [positions, rot / 2]; ``rot`` 0: no rotation) and stores keys and values as rows of the 8-bit cache, each rounded once.
     qkv float32 [N, (nh + 2 nkv) hd]; q_out bfloat16 [N, nh * hd].  ``write_kv`` false: queries alone, the pools may be None.
     A row whose position has no page is left out and the status says so.  Two tokens of a call must not share a position."""
-    n = qkv.shape[0]
-    if qkv.dim() != 2 or qkv.shape[1] != (nh + 2 * nkv) * hd:
+    n, width = qkv.shape if qkv.dim() == 2 else (0, -1)
+    if width != (nh + 2 * nkv) * hd:
         raise Backend("kv8_rope_append: qkv width disagrees with the head counts")
     if rot < 0 or rot > hd or rot % 2:
         raise Backend(f"kv8_rope_append: {rot} rotated channels of heads of {hd}")
@@ -1593,19 +1605,32 @@ def kv8_rope_append(qkv, bias, tok_seq, tok_pos, cos, sin, rot, q_out, k, v, exp
         raise Backend(f"kv8_rope_append: cosines and sines are not [positions, {rot // 2}]")
     if n == 0:
         return
-    for name, t in (("projection", qkv), ("bias", bias), ("cosines", cos if rot else None), ("sines", sin if rot else None)):
-        if t is not None and t.data_ptr() % 16:
-            raise Backend(f"kv8_rope_append: the {name} do not start on a multiple of 16 bytes")
-    _kv8_check("kv8_rope_append", q_out, k if write_kv else None, v, exps, block_table, page, nh, nkv, hd,
-               (("the bias", bias, qkv.shape[1]), ("tok_seq", tok_seq, n), ("tok_pos", tok_pos, n)))
+    k_ = v_ = e_ = t_ = c_ = s_ = None
+    stride = n_pages = positions = 0
+    fits = (_kv8_here(q_out) and q_out.numel() == n * nh * hd and tok_seq.numel() >= n <= tok_pos.numel() and (bias is None or bias.numel() == width)
+            and (_kv8_pools_fit(k, v, exps, block_table, page, nh, nkv, hd) if write_kv else kv8_fits(hd, page) and nkv > 0 < nh))
+    if fits:
+        x_, q_, b_ = _ptr(qkv, _F32, "qkv"), _ptr(q_out, _BF16, "q_out"), _ptr(bias, _F32, "bias")
+        if rot:
+            c_, s_, positions = _ptr(cos, _F32, "cos"), _ptr(sin, _F32, "sin"), cos.shape[0]
+        if write_kv:
+            k_, v_, e_, t_ = _ptr(k, _E4M3, "keys"), _ptr(v, _E4M3, "values"), _ptr(exps, torch.uint8, "exponents"), _ptr(block_table, torch.int32, "page table")
+            stride, n_pages = block_table.shape[1], k.shape[0]
+        fits = not (x_ | q_ | (b_ or 0) | (c_ or 0) | (s_ or 0) | (k_ or 0) | (v_ or 0) | (e_ or 0)) & 15
+    if not fits:
+        _kv8_refuse("kv8_rope_append", q_out, k if write_kv else None, v, exps, block_table, page, nh, nkv, hd,
+                    (("the bias", bias, width), ("tok_seq", tok_seq, n), ("tok_pos", tok_pos, n)),
+                    (("the projection", qkv), ("the bias", bias), ("the cosines", cos if rot else None), ("the sines", sin if rot else None),
+                     ("the queries", q_out), ("the keys", k if write_kv else None), ("the values", v if write_kv else None),
+                     ("the exponents", exps if write_kv else None)))
     _check(_fn("kv8", "esp_kv8_append")(
-        _ptr(qkv, torch.float32, "qkv"), _ptr(bias, torch.float32, "bias"), _ptr(tok_seq, torch.int32, "tok_seq"),
-        _ptr(tok_pos, torch.int32, "tok_pos"), _ptr(cos, torch.float32, "cos") if rot else None, _ptr(sin, torch.float32, "sin") if rot else None,
-        rot, cos.shape[0] if rot else 0, _ptr(q_out, torch.bfloat16, "q_out"), _ptr(k, _E4M3, "keys") if write_kv else None,
-        _ptr(v, _E4M3, "values") if write_kv else None, _ptr(exps, torch.uint8, "exponents") if write_kv else None,
-        _ptr(block_table, torch.int32, "page table") if write_kv else None, block_table.shape[1] if write_kv else 0,
-        k.shape[0] if write_kv else 0, n, nh, nkv, hd, 1 if write_kv else 0, _ptr(status, torch.int32, "status"), _stream()),
-        "kv8_rope_append")
+        x_, b_, _ptr(tok_seq, torch.int32, "tok_seq"), _ptr(tok_pos, torch.int32, "tok_pos"), c_, s_, rot, positions, q_, k_, v_, e_, t_, stride,
+        n_pages, n, nh, nkv, hd, 1 if write_kv else 0, _ptr(status, torch.int32, "status"), _stream()), "kv8_rope_append")
+
+
+@functools.lru_cache(maxsize=64)
+def _sm_count(device: int) -> int:
+    return torch.cuda.get_device_properties(device).multi_processor_count
 
 
 @functools.lru_cache(maxsize=4096)
@@ -1631,44 +1656,57 @@ def attn_decode_kv8(q, k, v, exps, out, ws, tok_seq, tok_pos, block_table, page,
         raise Backend(f"attn_decode_kv8: a window of {window} positions")
     if n == 0:
         return
-    _kv8_check("attn_decode_kv8", q, k, v, exps, block_table, page, nh, nkv, hd,
-               (("tok_seq", tok_seq, n), ("tok_pos", tok_pos, n), ("seq_past", seq_past, block_table.shape[0])))
-    positions = block_table.shape[1] * page
-    group = nh // nkv
+    fits = (_kv8_here(q) and _kv8_pools_fit(k, v, exps, block_table, page, nh, nkv, hd) and q.numel() == n * nh * hd
+            and tok_seq.numel() >= n <= tok_pos.numel() and (seq_past is None or seq_past.numel() >= block_table.shape[0]))
+    if fits:
+        q_, k_, v_, e_, o_ = (_ptr(q, _BF16, "q"), _ptr(k, _E4M3, "keys"), _ptr(v, _E4M3, "values"), _ptr(exps, torch.uint8, "exponents"),
+                              _ptr(out, _BF16, "out"))
+        fits = not (q_ | k_ | v_ | e_ | o_) & 15
+    if not fits:
+        _kv8_refuse("attn_decode_kv8", q, k, v, exps, block_table, page, nh, nkv, hd,
+                    (("tok_seq", tok_seq, n), ("tok_pos", tok_pos, n), ("seq_past", seq_past, block_table.shape[0])),
+                    (("the queries", q), ("the keys", k), ("the values", v), ("the exponents", exps), ("the results", out)))
+    stride = block_table.shape[1]
+    positions, group = stride * page, nh // nkv
     split = attn_decode_kv8_split(n, nkv * ((group + 15) // 16), min(positions, window + page) if window else positions, _sm_count(_device_index))
     n_splits = max(1, (positions + split - 1) // split)
-    part_o = part_ml = counters = None
+    scratch = counters = None
     if n_splits > 1:
-        part_o = ws.get("attn_kv8_part_o", (n, nh, n_splits, hd), torch.float32)
-        part_ml = ws.get("attn_kv8_part_ml", (n, nh, n_splits, 2), torch.float32)
-        counters = ws.get("attn_kv8_counters", (n * nh,), torch.int32, zeroed=True)
+        scratch = _ptr(ws.get("attn_kv8_parts", (n * nh * n_splits, hd + 2), _F32))
+        counters = _ptr(ws.get("attn_kv8_counters", (n * nh,), torch.int32, zeroed=True))
     _check(_fn("kv8", "esp_attn_decode_kv8")(
-        _ptr(q, torch.bfloat16, "q"), _ptr(k, _E4M3, "keys"), _ptr(v, _E4M3, "values"), _ptr(exps, torch.uint8, "exponents"),
-        _ptr(out, torch.bfloat16, "out"), _ptr(part_o), _ptr(part_ml), _ptr(counters), _ptr(tok_seq, torch.int32, "tok_seq"),
-        _ptr(tok_pos, torch.int32, "tok_pos"), _ptr(seq_past, torch.int32, "seq_past"), _ptr(block_table, torch.int32, "page table"),
-        block_table.shape[1], k.shape[0], n, nh, nkv, hd, int(window or 0), split, n_splits, _ptr(status, torch.int32, "status"), _stream()),
-        "attn_decode_kv8")
+        q_, k_, v_, e_, o_, scratch, counters, _ptr(tok_seq, torch.int32, "tok_seq"), _ptr(tok_pos, torch.int32, "tok_pos"),
+        _ptr(seq_past, torch.int32, "seq_past"), _ptr(block_table, torch.int32, "page table"), stride, k.shape[0], n, nh, nkv, hd, int(window or 0),
+        split, n_splits, _ptr(status, torch.int32, "status"), _stream()), "attn_decode_kv8")
 
 
 def attn_prefill_kv8(q, k, v, exps, out, tile_seq, tile_first, seq_start, seq_past, block_table, page, nh, nkv, hd, window, status):
     """Causal attention of runs of new tokens, packed back to back, over the 8-bit cache that holds their own keys already:
     the step's rows seq_start[i] .. seq_start[i + 1] are sequence i's, behind seq_past[i] cached positions.  ``tile_seq`` and
-    ``tile_first``: the tiles of ATTN_TC05_TILE_ROWS new tokens (sequence, index of the tile's first token among the
+    ``tile_first``: all tiles of ATTN_TC05_TILE_ROWS new tokens (sequence, index of the tile's first token among the
     sequence's new ones), best with those first that see the most keys.  The rest as for ``attn_decode_kv8``."""
     if out.numel() != q.numel():
         raise Backend(f"attn_prefill_kv8: {tuple(out.shape)} for the results of queries {tuple(q.shape)}")
     if window is not None and window < 0:
         raise Backend(f"attn_prefill_kv8: a window of {window} positions")
-    if q.shape[0] == 0 or tile_seq.numel() == 0:
+    n, n_tiles = q.shape[0], tile_seq.numel()
+    if n == 0 or n_tiles == 0:
         return
-    _kv8_check("attn_prefill_kv8", q, k, v, exps, block_table, page, nh, nkv, hd,
-               (("tile_first", tile_first, tile_seq.numel()), ("seq_past", seq_past, block_table.shape[0]),
-                ("seq_start", seq_start, block_table.shape[0] + 1)))
-    pools = (_ptr(k, _E4M3, "keys"), _ptr(v, _E4M3, "values"), _ptr(exps, torch.uint8, "exponents"), _ptr(out, torch.bfloat16, "out"),
-             _ptr(tile_seq, torch.int32, "tile_seq"), _ptr(tile_first, torch.int32, "tile_first"), _ptr(seq_start, torch.int32, "seq_start"),
-             _ptr(seq_past, torch.int32, "seq_past"), _ptr(block_table, torch.int32, "page table"), block_table.shape[1], k.shape[0],
-             tile_seq.numel(), nh, nkv, hd, int(window or 0), _ptr(status, torch.int32, "status"), _stream())
+    fits = (_kv8_here(q) and _kv8_pools_fit(k, v, exps, block_table, page, nh, nkv, hd) and q.numel() == n * nh * hd
+            and tile_first.numel() >= n_tiles and seq_past.numel() >= block_table.shape[0] < seq_start.numel())
+    if fits:
+        q_, k_, v_, e_, o_ = (_ptr(q, _BF16, "q"), _ptr(k, _E4M3, "keys"), _ptr(v, _E4M3, "values"), _ptr(exps, torch.uint8, "exponents"),
+                              _ptr(out, _BF16, "out"))
+        fits = not (q_ | k_ | v_ | e_ | o_) & 15
+    if not fits:
+        _kv8_refuse("attn_prefill_kv8", q, k, v, exps, block_table, page, nh, nkv, hd,
+                    (("tile_first", tile_first, n_tiles), ("seq_past", seq_past, block_table.shape[0]),
+                     ("seq_start", seq_start, block_table.shape[0] + 1)),
+                    (("the queries", q), ("the keys", k), ("the values", v), ("the exponents", exps), ("the results", out)))
+    rest = (k_, v_, e_, o_, _ptr(tile_seq, torch.int32, "tile_seq"), _ptr(tile_first, torch.int32, "tile_first"),
+            _ptr(seq_start, torch.int32, "seq_start"), _ptr(seq_past, torch.int32, "seq_past"), _ptr(block_table, torch.int32, "page table"),
+            block_table.shape[1], k.shape[0], n_tiles, nh, nkv, hd, int(window or 0), _ptr(status, torch.int32, "status"), _stream())
     if hd <= 128:                      # scores and weighted values in tensor memory
-        _check(_fn("kv8", "esp_attn_prefill_kv8")(_ptr(q, torch.bfloat16, "q"), q.shape[0], *pools), "attn_prefill_kv8")
+        _check(_fn("kv8", "esp_attn_prefill_kv8")(q_, n, *rest), "attn_prefill_kv8")
     else:                              # the streaming kernel, sixteen rows a block
-        _check(_fn("kv8", "esp_attn_run_kv8")(_ptr(q, torch.bfloat16, "q"), *pools), "attn_prefill_kv8")
+        _check(_fn("kv8", "esp_attn_run_kv8")(q_, *rest), "attn_prefill_kv8")
