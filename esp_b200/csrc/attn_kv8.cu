@@ -1,40 +1,45 @@
-// Attention over the 8-bit paged cache (kv8.cuh), streaming: one new token of every sequence with the keys split over blocks
-// (decode), or sixteen new tokens of a run (head sizes that the tensor-memory kernel does not take).
+// Attention over the 8-bit paged cache (kv8.cuh), streaming: one new token of every sequence (decode), or sixteen new tokens of a
+// run (head sizes that the tensor-memory kernel does not take).
 //
 //   s_j = q k_j / sqrt(hd),  o = sum_j 2^(s_j log2 e - m) v_j / sum_j 2^(s_j log2 e - m),  m = max_j s_j log2 e
 // over the keys max(0, pos - window + 1) <= j <= pos.
 //
 // A block has four warps and up to 8 * NT rows: the query heads that share one key/value head (decode), or consecutive
-// tokens of one head (RUN).  Every warp is on its own until the end: it takes each fourth chunk of 32 keys, brings the
-// codes of its chunks in by asynchronous copies (a ring of STAGES chunks, 16 bytes a lane, swizzled so that eight rows of an
-// ldmatrix fall into different banks), and keeps a softmax and an output of its own; the warps' and then the splits' results
-// are joined in ascending order.
+// tokens of one head (run).  Keys go by in units of 128, a chunk of 32 to each warp, which brings the codes of its chunks in by
+// asynchronous copies (a ring of STAGES chunks, 16 bytes a lane, swizzled so that eight rows of an ldmatrix fall into
+// different banks) and keeps a softmax and an output of its own; the warps' results are joined in ascending order.
+//
+// Decode is one stream: the units of all (row, key head) pairs, one behind the other, are dealt out evenly over a grid that the
+// device holds at once, so that ragged lengths leave no block idle, and a block's copies run on across the pairs' borders.  A pair
+// whose units fall to several blocks is put together by the last of them to finish, in the order of the blocks, so a result
+// is the same in every run; how a row is divided depends on the lengths of the step's other rows.
 //
 // Both products run on mma.sync m16n8k16 in half precision with the cache as the 16-row operand, so a block of up to eight
 // rows wastes no more than that: S^T = K Q^T, O^T = V^T P^T.  Codes become halfs exactly by one conversion per two codes
 // (through bfloat16 it would be four operations), and the exponents are applied in 32-bit: a key's to its scores, a
 // value's to its weight.  A half has little range, so
 //   * queries are scaled by a power of two that brings the row's largest to 2^14 (bfloat16's 8 bits fit a half's 11),
-//   * the weights 2^(s + e_v) have a running maximum M of their own; the largest weight becomes 2^WEIGHT_TOP and what is
-//     rounded off to a half's 11 bits is below 2^-24 of it at most 2^-25 of it.
+//   * the weights 2^(s + e_v) have a running maximum M of their own, which may lag behind by 2^LAG_TOP; the largest weight lies
+//     between 2^WEIGHT_TOP and 2^(WEIGHT_TOP + LAG_TOP), and what is below 2^-20 of it is rounded to multiples of 2^-30 of it.
 // Sums, maxima and accumulators are 32-bit.
 #include "kv8.cuh"
 
 namespace {
-constexpr int THREADS = 128, WARPS = 4, CHUNK = 32;
-constexpr float WEIGHT_TOP = 10.f;
+constexpr int THREADS = 128, WARPS = 4, CHUNK = 32, UNIT = WARPS * CHUNK, MAX_ROWS = 1024;
+constexpr float WEIGHT_TOP = 6.f, LAG_TOP = 8.f, LAG_SUM = 40.f;
+constexpr int PARTS = 16, MOST_PARTS = 48;     // parts that one block joins; of a pair's, or its groups of PARTS blocks
 
 struct Params {
     const bf16* q;
     const unsigned char *k, *v, *exps;
     bf16* out;
-    float *part_o, *part_ml;
-    int* counters;
+    float* parts;                              // decode: [blocks][2][8 * NT][hd + 2] of the pairs that a block has a part of
+    int* counters;                             // decode: per pair
     const int *tok_seq, *tok_pos;              // decode: per row of the step
     const int *seq_past, *seq_start;           // per sequence (decode: seq_past may be null)
-    const int *tile_seq, *tile_first;          // RUN: tiles of tile_rows new tokens
+    const int *tile_seq, *tile_first;          // run: tiles of 128 new tokens
     const int* block_table;
-    int table_stride, n_pages, nh, nkv, hd, window, split_keys, n_splits, tile_rows;
+    int table_stride, n_pages, n_rows, nh, nkv, hd, window;
     float scale_log2;                          // log2(e) / sqrt(hd)
     int* status;
 };
@@ -91,161 +96,101 @@ template <int HD> __device__ __forceinline__ int piece_at(int r, int c) {
     return r * HD + ((c ^ (HD == 64 ? (r >> 1) & 3 : r & 7)) << 4);
 }
 
-template <int HD, int NT, bool RUN>
-__global__ void __launch_bounds__(THREADS) attn_kv8_kernel(const Params p) {
-    pdl_trigger();
-    constexpr int STAGES = Ring<HD>::STAGES, STAGE = Ring<HD>::STAGE, ROWS = 8 * NT, PP = HD / 16;
-    extern __shared__ __align__(128) unsigned char smem[];
-    __shared__ float m_s[WARPS][ROWS], l_s[WARPS][ROWS];
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g8 = lane >> 2, tg = lane & 3;
-    unsigned char* ring = smem + warp * Ring<HD>::WARP;
 
-    // ---- the block's rows: ``rows`` of them, row r at query row q0 + r * q_step, at position pos0 + (RUN ? r : 0)
-    int seq, kvh, rows, pos0, head0;
-    long long q0, q_step;
-    if constexpr (RUN) {
-        const int subs = p.tile_rows / ROWS, tile = blockIdx.x / subs, first = p.tile_first[tile] + (blockIdx.x % subs) * ROWS;
-        seq = p.tile_seq[tile];
-        const int start = p.seq_start[seq];
-        rows = min(ROWS, p.seq_start[seq + 1] - start - first);
-        if (rows <= 0) return;
-        head0 = blockIdx.y;
-        kvh = head0 / (p.nh / p.nkv);
-        pos0 = p.seq_past[seq] + first;
-        q0 = (long long)(start + first) * p.nh + head0;
-        q_step = p.nh;
-    } else {
-        const int group = p.nh / p.nkv, per_kv = (group + ROWS - 1) / ROWS;
-        kvh = blockIdx.y / per_kv;
-        head0 = kvh * group + (blockIdx.y % per_kv) * ROWS;
-        rows = min(ROWS, (kvh + 1) * group - head0);
-        seq = p.tok_seq[blockIdx.x];
-        pos0 = p.tok_pos[blockIdx.x];
-        q0 = (long long)blockIdx.x * p.nh + head0;
-        q_step = 1;
-    }
-    const int pos_last = pos0 + (RUN ? rows - 1 : 0);
-    if (pos0 < 0 || seq < 0 || pos_last / KV8_PAGE >= p.table_stride) {
-        if (threadIdx.x == 0) atomicOr(p.status, ESP_STATUS_BAD_INDEX);
-        return;
-    }
-    const int lo = first_visible_key(pos0, p.window, 0);
-    const int k0 = RUN ? lo : max(lo, (int)blockIdx.z * p.split_keys);
-    const int k1 = RUN ? pos_last : min(pos_last, ((int)blockIdx.z + 1) * p.split_keys - 1);
-    if (k0 > k1) return;                       // not one of the row's splits
-    const int n_chunks = k1 / CHUNK - k0 / CHUNK + 1, mine = (n_chunks - warp + WARPS - 1) / WARPS;
-    const int* pages = p.block_table + (size_t)seq * p.table_stride;
-    const bool whole_pieces = p.hd % 16 == 0;
-
-    // ---- copies of this warp's i-th chunk (keys chunk * 32 ..) into a stage; ``page`` was read one chunk ahead
-    auto chunk_of = [&](int i) { return k0 / CHUNK + i * WARPS + warp; };
-    auto page_of = [&](int i) { return i < mine ? pages[chunk_of(i) * CHUNK / KV8_PAGE] : -1; };
-    auto load = [&](int i, int page) {
-        if (i < mine) {
-            unsigned char* st = ring + (i % STAGES) * STAGE;
-            const unsigned k_dst = smem_addr(st), v_dst = k_dst + CHUNK * HD, e_dst = v_dst + CHUNK * HD;
-            const int key0 = chunk_of(i) * CHUNK;
-            const bool ok = page >= 0 && page < p.n_pages;
-            if (!ok && lane == 0) atomicOr(p.status, ESP_STATUS_BAD_INDEX);
-            const size_t block = ok ? (size_t)page * p.nkv + kvh : 0;
-            const size_t row0 = (block * KV8_PAGE + key0 % KV8_PAGE) * p.hd;
-            if (whole_pieces) {
-#pragma unroll
-                for (int u = 0; u < PP; u++) {
-                    const int idx = u * 32 + lane, r = idx / PP, c = idx % PP;
-                    const bool live = ok && key0 + r >= k0 && key0 + r <= k1 && c * 16 < p.hd;
-                    const size_t from = row0 + (live ? (size_t)r * p.hd + c * 16 : 0);
-                    const int to = piece_at<HD>(r, c), bytes = live ? 16 : 0;
-                    copy16(k_dst + to, p.k + from, bytes);
-                    copy16(v_dst + to, p.v + from, bytes);
-                }
-            } else {
-                for (int u = 0; u < 2 * PP; u++) {
-                    const int idx = u * 32 + lane, r = idx / (2 * PP), c = idx % (2 * PP);
-                    const bool live = ok && key0 + r >= k0 && key0 + r <= k1 && c * 8 < p.hd;
-                    const size_t from = row0 + (live ? (size_t)r * p.hd + c * 8 : 0);
-                    const int to = piece_at<HD>(r, c >> 1) + (c & 1) * 8, bytes = live ? 8 : 0;
-                    copy8(k_dst + to, p.k + from, bytes);
-                    copy8(v_dst + to, p.v + from, bytes);
-                }
-            }
-            // the exponents: 32 bytes of the keys, 32 of the values (a page that is not one: NaN-free zeros, its keys are hidden)
-            if (lane < 16) copy4(e_dst + lane * 4, p.exps + (block * 2 + (lane >> 3)) * KV8_PAGE + key0 % KV8_PAGE + (lane & 7) * 4, ok ? 4 : 0);
-        }
-        copies_commit();
-    };
-    // Positions that were cached before this step do not depend on the kernel before this one, which writes the step's
-    // own: a decode block all of whose keys are older asks for its first chunks at once and then waits for the queries.
-    const bool early = !RUN && p.seq_past != nullptr && k1 < p.seq_past[seq];
-    if (!early) pdl_wait();
-    int page_next = page_of(0);
-#pragma unroll
-    for (int s = 0; s < STAGES - 1; s++) {
-        const int page = page_next;
-        page_next = page_of(s + 1);
-        load(s, page);
-    }
-    if (early) pdl_wait();
-
-    // ---- the queries as B operands, scaled row by row; row_scale: what a score is multiplied by (before the key's exponent)
-    const bf16* q = behind_wait(p.q);
+// One warp's share: its ring of chunks, and the softmax and the output of the block's rows over the keys it has seen.
+template <int HD, int NT, bool RUN> struct Stream {
+    static constexpr int STAGES = Ring<HD>::STAGES, STAGE = Ring<HD>::STAGE, ROWS = 8 * NT, PP = HD / 16;
     unsigned qf[NT][HD / 16][2];
     float row_scale[NT][2];
+    float o[NT][HD / 16][4], top[NT][2];       // top: M, of the row
+    float m[NT][2], l[NT][2];                  // maximum (lagging by LAG_SUM) and sum of the lane's own keys
+
+    // asks for the chunk of keys key0 .. key0 + 31 in page ``page``; those outside [k0, k1] are filled with zeros
+    static __device__ __forceinline__ void ask(const Params& p, unsigned char* st, int page, int kvh, int key0, int k0, int k1, int lane) {
+        const unsigned k_dst = smem_addr(st), v_dst = k_dst + CHUNK * HD, e_dst = v_dst + CHUNK * HD;
+        const bool wanted = key0 <= k1 && key0 + CHUNK > k0, ok = wanted && page >= 0 && page < p.n_pages;
+        if (wanted && !ok && lane == 0) atomicOr(p.status, ESP_STATUS_BAD_INDEX);
+        const size_t block = ok ? (size_t)page * p.nkv + kvh : 0;
+        const size_t row0 = (block * KV8_PAGE + key0 % KV8_PAGE) * p.hd;
+        if (p.hd % 16 == 0) {
 #pragma unroll
-    for (int nt = 0; nt < NT; nt++) {
-        const int r = nt * 8 + g8;
-        const bf16* row = q + (q0 + r * q_step) * p.hd;
-        float amax = 0.f;
-        uint2 raw[HD / 16];
-#pragma unroll
-        for (int kk = 0; kk < HD / 16; kk++) {
-            const int d = kk * 16 + tg * 4;
-            raw[kk] = r < rows && d < p.hd ? *reinterpret_cast<const uint2*>(row + d) : make_uint2(0u, 0u);
-            const float2 a = __bfloat1622float2(*reinterpret_cast<__nv_bfloat162*>(&raw[kk].x)), b = __bfloat1622float2(*reinterpret_cast<__nv_bfloat162*>(&raw[kk].y));
-            amax = fmaxf(amax, fmaxf(fmaxf(fabsf(a.x), fabsf(a.y)), fmaxf(fabsf(b.x), fabsf(b.y))));
+            for (int u = 0; u < PP; u++) {
+                const int idx = u * 32 + lane, r = idx / PP, c = idx % PP;
+                const bool live = ok && key0 + r >= k0 && key0 + r <= k1 && c * 16 < p.hd;
+                const size_t from = row0 + (live ? (size_t)r * p.hd + c * 16 : 0);
+                const int to = piece_at<HD>(r, c), bytes = live ? 16 : 0;
+                copy16(k_dst + to, p.k + from, bytes);
+                copy16(v_dst + to, p.v + from, bytes);
+            }
+        } else {
+            for (int u = 0; u < 2 * PP; u++) {
+                const int idx = u * 32 + lane, r = idx / (2 * PP), c = idx % (2 * PP);
+                const bool live = ok && key0 + r >= k0 && key0 + r <= k1 && c * 8 < p.hd;
+                const size_t from = row0 + (live ? (size_t)r * p.hd + c * 8 : 0);
+                const int to = piece_at<HD>(r, c >> 1) + (c & 1) * 8, bytes = live ? 8 : 0;
+                copy8(k_dst + to, p.k + from, bytes);
+                copy8(v_dst + to, p.v + from, bytes);
+            }
         }
-        amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
-        amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
-        const int x = max((int)(__float_as_uint(amax) >> 23) - 127, -100);       // the largest lies in [2^x, 2^(x+1))
-        const float f = kv8_pow2(14 - x);
-#pragma unroll
-        for (int kk = 0; kk < HD / 16; kk++) {
-            const float2 a = __bfloat1622float2(*reinterpret_cast<__nv_bfloat162*>(&raw[kk].x)), b = __bfloat1622float2(*reinterpret_cast<__nv_bfloat162*>(&raw[kk].y));
-            qf[nt][kk][0] = pack_half(a.x * f, a.y * f);
-            qf[nt][kk][1] = pack_half(b.x * f, b.y * f);
-        }
-        // a lane's scores belong to rows 2 tg and 2 tg + 1, whose queries the lanes 8 tg and 8 tg + 4 hold
-        const int xa = __shfl_sync(0xffffffffu, x, tg * 8), xb = __shfl_sync(0xffffffffu, x, tg * 8 + 4);
-        row_scale[nt][0] = kv8_pow2(min(xa - 14, 127)) * p.scale_log2;
-        row_scale[nt][1] = kv8_pow2(min(xb - 14, 127)) * p.scale_log2;
+        // the exponents: 32 bytes of the keys, 32 of the values (without a page: zeros, which hide its keys)
+        if (lane < 16) copy4(e_dst + lane * 4, p.exps + (block * 2 + (lane >> 3)) * KV8_PAGE + key0 % KV8_PAGE + (lane & 7) * 4, ok ? 4 : 0);
     }
 
-    float o[NT][HD / 16][4], m[NT][2], l[NT][2], top[NT][2];             // top: M, the running maximum of the weights' exponents
+    // the rows' queries: row r at q + r * step, those from ``rows`` on zero
+    static __device__ __forceinline__ void ask_queries(uint2 (&raw)[NT][HD / 16], const bf16* q, long long step, int rows, int hd, int lane) {
 #pragma unroll
-    for (int nt = 0; nt < NT; nt++) {
+        for (int nt = 0; nt < NT; nt++) {
+            const int r = nt * 8 + (lane >> 2);
 #pragma unroll
-        for (int i = 0; i < HD / 16; i++)
+            for (int kk = 0; kk < HD / 16; kk++) {
+                const int d = kk * 16 + (lane & 3) * 4;
+                raw[nt][kk] = r < rows && d < hd ? *reinterpret_cast<const uint2*>(q + r * step + d) : make_uint2(0u, 0u);
+            }
+        }
+    }
+    // ... as B operands, scaled row by row; row_scale: what a score is multiplied by (before the key's exponent).  Empties the rest.
+    __device__ __forceinline__ void begin(const uint2 (&raw)[NT][HD / 16], float scale_log2, int lane) {
+        const int tg = lane & 3;
 #pragma unroll
-            for (int j = 0; j < 4; j++) o[nt][i][j] = 0.f;
+        for (int nt = 0; nt < NT; nt++) {
+            float amax = 0.f;
 #pragma unroll
-        for (int j = 0; j < 2; j++) {
-            m[nt][j] = top[nt][j] = -INFINITY;
-            l[nt][j] = 0.f;
+            for (int kk = 0; kk < HD / 16; kk++) {
+                const float2 a = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&raw[nt][kk].x)), b = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&raw[nt][kk].y));
+                amax = fmaxf(amax, fmaxf(fmaxf(fabsf(a.x), fabsf(a.y)), fmaxf(fabsf(b.x), fabsf(b.y))));
+            }
+            amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
+            amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
+            const int x = max((int)(__float_as_uint(amax) >> 23) - 127, -100);       // the largest lies in [2^x, 2^(x+1))
+            const float f = kv8_pow2(14 - x);
+#pragma unroll
+            for (int kk = 0; kk < HD / 16; kk++) {
+                const float2 a = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&raw[nt][kk].x)), b = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&raw[nt][kk].y));
+                qf[nt][kk][0] = pack_half(a.x * f, a.y * f);
+                qf[nt][kk][1] = pack_half(b.x * f, b.y * f);
+            }
+            // a lane's scores belong to rows 2 tg and 2 tg + 1, whose queries the lanes 8 tg and 8 tg + 4 hold
+            const int xa = __shfl_sync(0xffffffffu, x, tg * 8), xb = __shfl_sync(0xffffffffu, x, tg * 8 + 4);
+            row_scale[nt][0] = kv8_pow2(min(xa - 14, 127)) * scale_log2;
+            row_scale[nt][1] = kv8_pow2(min(xb - 14, 127)) * scale_log2;
+#pragma unroll
+            for (int i = 0; i < HD / 16; i++)
+#pragma unroll
+                for (int j = 0; j < 4; j++) o[nt][i][j] = 0.f;
+#pragma unroll
+            for (int j = 0; j < 2; j++) {
+                m[nt][j] = top[nt][j] = -INFINITY;
+                l[nt][j] = 0.f;
+            }
         }
     }
 
-    for (int i = 0; i < mine; i++) {
-        copies_wait<STAGES - 2>();
-        __syncwarp();                          // every lane's pieces of chunk i are there, and all have read chunk i - 1
-        {
-            const int page = page_next;
-            page_next = page_of(i + STAGES);
-            load(i + STAGES - 1, page);
-        }
-        const unsigned char* st = ring + (i % STAGES) * STAGE;
+    // the chunk of keys key0 .. key0 + 31 that lies in ``st``; [k0, k1]: the keys that the block's rows see (run: row r sees those up
+    // to pos0 + r, and of them the last ``window``)
+    __device__ __forceinline__ void chunk(const unsigned char* st, int key0, int k0, int k1, int pos0, int window, int lane) {
+        const int g8 = lane >> 2, tg = lane & 3;
         const unsigned k_src = smem_addr(st), v_src = k_src + CHUNK * HD;
         const unsigned char* e_src = st + 2 * CHUNK * HD;
-        const int key0 = chunk_of(i) * CHUNK;
         // ---- S^T: 32 keys (two tiles of 16) by the rows
         float s[NT][2][4];
 #pragma unroll
@@ -291,7 +236,7 @@ __global__ void __launch_bounds__(THREADS) attn_kv8_kernel(const Params p) {
                     bool live = seen[u];
                     if constexpr (RUN) {
                         const int key = key0 + u * 8 + g8, pos = pos0 + nt * 8 + 2 * tg + j;
-                        live = live && key <= pos && (p.window <= 0 || pos - key < p.window);
+                        live = live && key <= pos && (window <= 0 || pos - key < window);
                     }
                     if (!live) x = -INFINITY;
                     s[nt][u >> 1][(u & 1) * 2 + j] = x;
@@ -299,42 +244,33 @@ __global__ void __launch_bounds__(THREADS) attn_kv8_kernel(const Params p) {
                     cm[j] = fmaxf(cm[j], x);
                     ct[j] = fmaxf(ct[j], t[u][j]);
                 }
-            float mu[2], tu[2];
-#pragma unroll
-            for (int j = 0; j < 2; j++) {
-#pragma unroll
-                for (int off = 4; off < 32; off <<= 1) {
-                    cm[j] = fmaxf(cm[j], __shfl_xor_sync(0xffffffffu, cm[j], off));
-                    ct[j] = fmaxf(ct[j], __shfl_xor_sync(0xffffffffu, ct[j], off));
-                }
-                cm[j] = fmaxf(m[nt][j], cm[j]);
-                ct[j] = fmaxf(top[nt][j], ct[j]);
-                mu[j] = cm[j] == -INFINITY ? 0.f : cm[j];
-                tu[j] = ct[j] == -INFINITY ? 0.f : ct[j];
-                l[nt][j] *= exp2_fast(m[nt][j] - mu[j]);
-                m[nt][j] = cm[j];
-            }
-            if (__any_sync(0xffffffffu, ct[0] > top[nt][0] || ct[1] > top[nt][1])) {
-                const float a = exp2_fast(top[nt][0] - tu[0]), b = exp2_fast(top[nt][1] - tu[1]);
-#pragma unroll
-                for (int d = 0; d < HD / 16; d++) {
-                    o[nt][d][0] *= a;
-                    o[nt][d][1] *= b;
-                    o[nt][d][2] *= a;
-                    o[nt][d][3] *= b;
-                }
-                top[nt][0] = ct[0];
-                top[nt][1] = ct[1];
-            }
-#pragma unroll
-            for (int u = 0; u < 4; u++) {
-                float w[2];
+            // what is in use has been outgrown: the first chunk, and seldom after it
+            const bool far = cm[0] > m[nt][0] + LAG_SUM || cm[1] > m[nt][1] + LAG_SUM || ct[0] > top[nt][0] + LAG_TOP || ct[1] > top[nt][1] + LAG_TOP;
+            if (__any_sync(0xffffffffu, far)) {
 #pragma unroll
                 for (int j = 0; j < 2; j++) {
-                    l[nt][j] += exp2_fast(s[nt][u >> 1][(u & 1) * 2 + j] - mu[j]);
-                    w[j] = exp2_fast(t[u][j] - tu[j] + WEIGHT_TOP);
+                    cm[j] = fmaxf(m[nt][j], cm[j]);
+                    if (cm[j] > m[nt][j]) l[nt][j] *= exp2_fast(m[nt][j] - cm[j]);
+                    m[nt][j] = cm[j];
+#pragma unroll
+                    for (int off = 4; off < 32; off <<= 1) ct[j] = fmaxf(ct[j], __shfl_xor_sync(0xffffffffu, ct[j], off));
+                    ct[j] = fmaxf(top[nt][j], ct[j]);
+                    const float f = ct[j] > top[nt][j] ? exp2_fast(top[nt][j] - ct[j]) : 1.f;
+                    top[nt][j] = ct[j];
+#pragma unroll
+                    for (int d = 0; d < HD / 16; d++) {
+                        o[nt][d][j] *= f;
+                        o[nt][d][j + 2] *= f;
+                    }
                 }
-                wf[nt][u] = transpose_8x8(pack_half(w[0], w[1]));
+            }
+            const float mu[2] = {m[nt][0] == -INFINITY ? 0.f : m[nt][0], m[nt][1] == -INFINITY ? 0.f : m[nt][1]};
+            const float tu[2] = {(top[nt][0] == -INFINITY ? 0.f : top[nt][0]) - WEIGHT_TOP, (top[nt][1] == -INFINITY ? 0.f : top[nt][1]) - WEIGHT_TOP};
+#pragma unroll
+            for (int u = 0; u < 4; u++) {
+#pragma unroll
+                for (int j = 0; j < 2; j++) l[nt][j] += exp2_fast(s[nt][u >> 1][(u & 1) * 2 + j] - mu[j]);
+                wf[nt][u] = transpose_8x8(pack_half(exp2_fast(t[u][0] - tu[0]), exp2_fast(t[u][1] - tu[1])));
             }
         }
         // ---- O^T += V^T P^T: row r < 8 of an operand tile is channel 2 r of its 16, row r + 8 channel 2 r + 1
@@ -352,162 +288,417 @@ __global__ void __launch_bounds__(THREADS) attn_kv8_kernel(const Params p) {
             }
         }
     }
+
+    // the result in the form (m, l, sum of weights 2^(s - m) times values): m and l of the rows to the lists, the sum to o_w [ROWS][HD]
+    __device__ __forceinline__ void leave(float* m_w, float* l_w, float* o_w, int lane) {
+        const int g8 = lane >> 2, tg = lane & 3;
+#pragma unroll
+        for (int nt = 0; nt < NT; nt++)
+#pragma unroll
+            for (int j = 0; j < 2; j++) {
+                float most = m[nt][j];
+#pragma unroll
+                for (int off = 4; off < 32; off <<= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, off));
+                // a lane without a key counts 0; one whose keys are no numbers is NaN and stays it
+                float sum = l[nt][j] * (m[nt][j] == -INFINITY ? 0.f : exp2_fast(m[nt][j] - most));
+#pragma unroll
+                for (int off = 4; off < 32; off <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, off);
+                const int r = nt * 8 + 2 * tg + j;
+                const float f = most == -INFINITY ? 1.f : exp2_fast(top[nt][j] - WEIGHT_TOP - most);
+                if (g8 == 0) {
+                    m_w[r] = most;
+                    l_w[r] = sum;
+                }
+#pragma unroll
+                for (int d = 0; d < HD / 16; d++)
+                    *reinterpret_cast<float2*>(o_w + r * HD + d * 16 + 2 * g8) = make_float2(o[nt][d][j] * f, o[nt][d][j + 2] * f);
+            }
+    }
+};
+
+// The warps' results of row r, channels d and d + 1, in ascending order of the warps: (maximum, sum, the two sums of values).  A warp
+// that saw nothing has m = -inf, l = 0, o = 0; one that saw only positions that are not numbers has m = -inf and NaN in l
+// and o, which stay (0 * NaN = NaN).  ``o_s``: the first warp's sums, the others' ``warp_bytes`` behind one another.
+struct Joined {
+    float m, l, a, b;
+};
+template <int ROWS, int HD>
+__device__ __forceinline__ Joined join_warps(const float (*m_s)[ROWS], const float (*l_s)[ROWS], const unsigned char* o_s, int warp_bytes, int r, int d) {
+    Joined x{-INFINITY, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int u = 0; u < WARPS; u++) x.m = fmaxf(x.m, m_s[u][r]);
+#pragma unroll
+    for (int u = 0; u < WARPS; u++) {
+        const float w = m_s[u][r] == -INFINITY ? 0.f : exp2_fast(m_s[u][r] - x.m);
+        const float2 v = *reinterpret_cast<const float2*>(reinterpret_cast<const float*>(o_s + u * warp_bytes) + r * HD + d);
+        x.l += l_s[u][r] * w;
+        x.a += v.x * w;
+        x.b += v.y * w;
+    }
+    return x;
+}
+// the sum is 0 where none of the row's pages was one
+__device__ __forceinline__ float inverse(float sum) { return sum == 0.f ? 0.f : 1.f / sum; }
+__device__ __forceinline__ void store_pair(bf16* to, float a, float b) { *reinterpret_cast<__nv_bfloat162*>(to) = __floats2bfloat162_rn(a, b); }
+
+// ---------------------------------------------------------------------------------------------------- sixteen tokens of a run
+template <int HD, int NT>
+__global__ void __launch_bounds__(THREADS) attn_run_kv8_kernel(const Params p) {
+    pdl_trigger();
+    typedef Stream<HD, NT, true> S;
+    extern __shared__ __align__(128) unsigned char smem[];
+    __shared__ float m_s[WARPS][S::ROWS], l_s[WARPS][S::ROWS];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    unsigned char* ring = smem + warp * Ring<HD>::WARP;
+    pdl_wait();
+    // the block's rows: ``rows`` tokens from ``first`` on, all of head ``head``
+    const int subs = 128 / S::ROWS, tile = blockIdx.x / subs, seq = p.tile_seq[tile], first = p.tile_first[tile] + (blockIdx.x % subs) * S::ROWS;
+    const int start = p.seq_start[seq], rows = min(S::ROWS, p.seq_start[seq + 1] - start - first), head = blockIdx.y, kvh = head / (p.nh / p.nkv);
+    if (rows <= 0) return;
+    const int pos0 = p.seq_past[seq] + first, k0 = first_visible_key(pos0, p.window, 0), k1 = pos0 + rows - 1;
+    if (pos0 < 0 || k1 / KV8_PAGE >= p.table_stride) {
+        if (threadIdx.x == 0) atomicOr(p.status, ESP_STATUS_BAD_INDEX);
+        return;
+    }
+    const long long row0 = (long long)(start + first) * p.nh + head;
+    const int n_chunks = k1 / CHUNK - k0 / CHUNK + 1, mine = (n_chunks - warp + WARPS - 1) / WARPS;
+    const int* pages = p.block_table + (size_t)seq * p.table_stride;
+    auto key_of = [&](int i) { return (k0 / CHUNK + i * WARPS + warp) * CHUNK; };
+    auto page_of = [&](int i) { return i < mine ? pages[key_of(i) / KV8_PAGE] : -1; };
+    auto load = [&](int i, int page) {
+        if (i < mine) S::ask(p, ring + (i % S::STAGES) * S::STAGE, page, kvh, key_of(i), k0, k1, lane);
+        copies_commit();
+    };
+    int page_next = page_of(0);                // read one chunk ahead
+#pragma unroll
+    for (int s = 0; s < S::STAGES - 1; s++) {
+        const int page = page_next;
+        page_next = page_of(s + 1);
+        load(s, page);
+    }
+    S x;
+    {
+        uint2 raw[NT][HD / 16];
+        S::ask_queries(raw, behind_wait(p.q) + row0 * p.hd, (long long)p.nh * p.hd, rows, p.hd, lane);
+        x.begin(raw, p.scale_log2, lane);
+    }
+    for (int i = 0; i < mine; i++) {
+        copies_wait<S::STAGES - 2>();
+        __syncwarp();                          // every lane's pieces of chunk i are there, and all have read chunk i - 1
+        const int page = page_next;
+        page_next = page_of(i + S::STAGES);
+        load(i + S::STAGES - 1, page);
+        x.chunk(ring + (i % S::STAGES) * S::STAGE, key_of(i), k0, k1, pos0, p.window, lane);
+    }
     copies_wait<0>();
     __syncwarp();
-
-    // ---- the warp's result in the form (m, l, sum of weights 2^(s - m) times values), into its part of shared memory
-    float* o_w = reinterpret_cast<float*>(ring);                         // [ROWS][HD]
-#pragma unroll
-    for (int nt = 0; nt < NT; nt++)
-#pragma unroll
-        for (int j = 0; j < 2; j++) {
-            float sum = l[nt][j];
-#pragma unroll
-            for (int off = 4; off < 32; off <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, off);
-            const int r = nt * 8 + 2 * tg + j;
-            const float f = m[nt][j] == -INFINITY ? 1.f : exp2_fast(top[nt][j] - WEIGHT_TOP - m[nt][j]);
-            if (g8 == 0) {
-                m_s[warp][r] = m[nt][j];
-                l_s[warp][r] = sum;
-            }
-#pragma unroll
-            for (int d = 0; d < HD / 16; d++)
-                *reinterpret_cast<float2*>(o_w + r * HD + d * 16 + 2 * g8) = make_float2(o[nt][d][j] * f, o[nt][d][j + 2] * f);
-        }
+    x.leave(m_s[warp], l_s[warp], reinterpret_cast<float*>(ring), lane);
     __syncthreads();
-    // ---- the warps in ascending order.  A warp that saw nothing has m = -inf, l = 0, o = 0; one that saw only rows that are not
-    // numbers has m = -inf and NaN in l and o, which stay (0 * NaN = NaN).
-    const int first_split = lo / p.split_keys, n_live = RUN ? 1 : pos_last / p.split_keys - first_split + 1;
-    auto join = [&](int r, float (&w)[WARPS], float& mx, float& sum) {
-        mx = -INFINITY;
-        sum = 0.f;
-#pragma unroll
-        for (int u = 0; u < WARPS; u++) mx = fmaxf(mx, m_s[u][r]);
-#pragma unroll
-        for (int u = 0; u < WARPS; u++) {
-            w[u] = m_s[u][r] == -INFINITY ? 0.f : exp2_fast(m_s[u][r] - mx);
-            sum += l_s[u][r] * w[u];
-        }
-    };
-    // the sum is 0 where none of the row's pages was one
-    auto inverse = [](float sum) { return sum == 0.f ? 0.f : 1.f / sum; };
     const int pairs = p.hd / 2;
     for (int idx = threadIdx.x; idx < rows * pairs; idx += THREADS) {
         const int r = idx / pairs, d = (idx % pairs) * 2;
-        float w[WARPS], mx, sum, a = 0.f, b = 0.f;
-        join(r, w, mx, sum);
-#pragma unroll
-        for (int u = 0; u < WARPS; u++) {
-            const float2 x = *reinterpret_cast<const float2*>(reinterpret_cast<const float*>(smem + u * Ring<HD>::WARP) + r * HD + d);
-            a += x.x * w[u];
-            b += x.y * w[u];
-        }
-        if (n_live == 1) {
-            const float inv = inverse(sum);
-            *reinterpret_cast<__nv_bfloat162*>(p.out + (q0 + r * q_step) * p.hd + d) = __floats2bfloat162_rn(a * inv, b * inv);
-        } else {
-            const size_t at = ((size_t)blockIdx.x * p.nh + head0 + r) * p.n_splits + blockIdx.z;
-            *reinterpret_cast<float2*>(p.part_o + at * p.hd + d) = make_float2(a, b);
-            if (d == 0) *reinterpret_cast<float2*>(p.part_ml + at * 2) = make_float2(mx, sum);
-        }
-    }
-    if constexpr (RUN) return;
-    if (n_live == 1) return;
-    // ---- the last block of the row to finish joins its splits, in ascending order
-    __shared__ int is_last;
-    __threadfence();
-    __syncthreads();
-    if (threadIdx.x == 0) {
-        int* c = p.counters + (size_t)blockIdx.x * gridDim.y + blockIdx.y;
-        is_last = atomicAdd(c, 1) == n_live - 1;
-        if (is_last) *c = 0;
-    }
-    __syncthreads();
-    if (!is_last) return;
-    __threadfence();
-    constexpr int AT_ONCE = Ring<HD>::WARP / 8;                          // splits whose weights a warp holds at a time
-    float *w_w = reinterpret_cast<float*>(ring), *l_w = w_w + AT_ONCE;
-    constexpr int NV = HD / 64;                                          // pairs of channels a lane: 64 j + 2 lane
-    for (int r = warp; r < rows; r += WARPS) {
-        const size_t at = ((size_t)blockIdx.x * p.nh + head0 + r) * p.n_splits + first_split;
-        const float *ml = p.part_ml + at * 2, *po = p.part_o + at * p.hd;
-        float mx = -INFINITY, sum = 0.f, num[NV][2];
-        for (int i = lane; i < n_live; i += 32) mx = fmaxf(mx, __ldcg(ml + 2 * i));
-        mx = warp_max(mx);
-#pragma unroll
-        for (int j = 0; j < NV; j++) num[j][0] = num[j][1] = 0.f;
-        for (int c0 = 0; c0 < n_live; c0 += AT_ONCE) {
-            const int cn = min(AT_ONCE, n_live - c0);
-            __syncwarp();
-            for (int i = lane; i < cn; i += 32) {
-                const float2 v = __ldcg(reinterpret_cast<const float2*>(ml + 2 * (c0 + i)));
-                w_w[i] = v.x == -INFINITY ? 0.f : exp2_fast(v.x - mx);
-                l_w[i] = v.y;
-            }
-            __syncwarp();
-#pragma unroll 8
-            for (int i = 0; i < cn; i++) {
-                const float w = w_w[i];
-                sum += l_w[i] * w;
-#pragma unroll
-                for (int j = 0; j < NV; j++)
-                    if (j * 64 + 2 * lane < p.hd) {
-                        const float2 v = __ldcg(reinterpret_cast<const float2*>(po + (size_t)(c0 + i) * p.hd + j * 64 + 2 * lane));
-                        num[j][0] += v.x * w;
-                        num[j][1] += v.y * w;
-                    }
-            }
-        }
-        const float inv = inverse(sum);
-#pragma unroll
-        for (int j = 0; j < NV; j++)
-            if (j * 64 + 2 * lane < p.hd)
-                *reinterpret_cast<__nv_bfloat162*>(p.out + (q0 + r) * p.hd + j * 64 + 2 * lane) = __floats2bfloat162_rn(num[j][0] * inv, num[j][1] * inv);
+        const Joined y = join_warps<S::ROWS, HD>(m_s, l_s, smem, Ring<HD>::WARP, r, d);
+        store_pair(p.out + (row0 + (long long)r * p.nh) * p.hd + d, y.a * inverse(y.l), y.b * inverse(y.l));
     }
 }
 
-template <int HD, int NT, bool RUN> int launch(const Params& p, dim3 grid, cudaStream_t stream) {
-    const size_t smem = (size_t)WARPS * Ring<HD>::WARP;
-    static bool raised[64] = {false};                                    // per device
+// ---------------------------------------------------------------------------------------------------- one token of every sequence
+// What a unit of the stream belongs to.
+struct Cursor {
+    int row, kvb, unit, last;                  // the step's row, its block of heads, the unit's place among absolute 128 keys; the pair's last
+    int seq, pos, lo;                          // of the row; pos < 0: no row
+};
+
+template <int HD, int NT>
+__global__ void __launch_bounds__(THREADS) attn_decode_kv8_kernel(const Params p) {
+    pdl_trigger();
+    typedef Stream<HD, NT, false> S;
+    extern __shared__ __align__(128) unsigned char smem[];
+    __shared__ float m_s[WARPS][S::ROWS], l_s[WARPS][S::ROWS];
+    __shared__ int before[MAX_ROWS + 1];       // units of one key head ahead of each row
+    __shared__ int warp_sum_s[WARPS], is_last;
+    __shared__ float2 ml_s[S::ROWS][MOST_PARTS];                         // of the parts that are joined
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    unsigned char* ring = smem + warp * Ring<HD>::WARP;
+    const int group = p.nh / p.nkv, per_kv = (group + S::ROWS - 1) / S::ROWS, kv_blocks = p.nkv * per_kv;
+
+    // a row's units; one whose position is not in the table has none
+    auto units_of = [&](int pos) {
+        return pos < 0 || pos / KV8_PAGE >= p.table_stride ? 0 : pos / UNIT - first_visible_key(pos, p.window, 0) / UNIT + 1;
+    };
+    // ---- how many units lie ahead of each row (every block works it out for itself; rows and positions were there before this step's
+    // kernels began)
+    int carry = 0;
+    for (int r0 = 0; r0 < p.n_rows; r0 += THREADS) {
+        const int r = r0 + threadIdx.x;
+        int mine = 0;
+        if (r < p.n_rows) {
+            const int pos = p.tok_pos[r];
+            mine = p.tok_seq[r] < 0 ? 0 : units_of(pos);
+            if (mine == 0 && blockIdx.x == 0) atomicOr(p.status, ESP_STATUS_BAD_INDEX);
+        }
+        int sum = mine;
+#pragma unroll
+        for (int off = 1; off < 32; off <<= 1) {
+            const int v = __shfl_up_sync(0xffffffffu, sum, off);
+            if (lane >= off) sum += v;
+        }
+        if (lane == 31) warp_sum_s[warp] = sum;
+        __syncthreads();
+        int ahead = carry, all = carry;
+#pragma unroll
+        for (int u = 0; u < WARPS; u++) {
+            if (u < warp) ahead += warp_sum_s[u];
+            all += warp_sum_s[u];
+        }
+        if (r < p.n_rows) before[r] = ahead + sum - mine;
+        carry = all;
+        __syncthreads();
+    }
+    if (threadIdx.x == 0) before[p.n_rows] = carry;
+    __syncthreads();
+    const long long total = (long long)carry * kv_blocks;
+    const int blocks = (int)min((long long)gridDim.x, total);            // that have units: each of them one at least
+    if ((int)blockIdx.x >= blocks) return;
+    const long long u0 = total * blockIdx.x / blocks, u1 = total * (blockIdx.x + 1) / blocks;
+
+    // ---- cursors through the stream: pairs row by row, of a row its blocks of heads one behind the other
+    auto open_row = [&](Cursor& c) {
+        c.seq = p.tok_seq[c.row];
+        c.pos = p.tok_pos[c.row];
+        c.lo = first_visible_key(c.pos, p.window, 0);
+        c.last = c.pos / UNIT;
+    };
+    auto advance = [&](Cursor& c) {
+        if (c.unit < c.last) {
+            c.unit++;
+        } else if (c.kvb + 1 < kv_blocks) {
+            c.kvb++;
+            c.unit = c.lo / UNIT;
+        } else {
+            do c.row++;
+            while (c.row < p.n_rows && before[c.row] == before[c.row + 1]);   // rows without units
+            c.kvb = 0;
+            if (c.row < p.n_rows) {
+                open_row(c);
+                c.unit = c.lo / UNIT;
+            }
+        }
+    };
+    Cursor now;
+    {
+        int a = 0, b = p.n_rows;               // the last row whose units begin at or ahead of u0, and that has some
+        while (b - a > 1) {
+            const int mid = (a + b) / 2;
+            if ((long long)before[mid] * kv_blocks <= u0) a = mid;
+            else b = mid;
+        }
+        now.row = a;
+        open_row(now);
+        const long long in_row = u0 - (long long)before[a] * kv_blocks;
+        const int each = before[a + 1] - before[a];
+        now.kvb = (int)(in_row / each);
+        now.unit = now.lo / UNIT + (int)(in_row % each);
+    }
+    const int n_units = (int)(u1 - u0);
+    Cursor ahead = now;                        // of the next chunk that is asked for
+    int asked = 0;
+    auto page_of = [&](const Cursor& c) { return p.block_table[(size_t)c.seq * p.table_stride + min(c.unit * UNIT + warp * CHUNK, c.pos) / KV8_PAGE]; };
+    int page_next = page_of(ahead);
+    auto load = [&]() {                        // the next chunk of this warp, into the ring's next stage
+        if (asked < n_units) {
+            S::ask(p, ring + (asked % S::STAGES) * S::STAGE, page_next, ahead.kvb / per_kv, ahead.unit * UNIT + warp * CHUNK, ahead.lo, ahead.pos, lane);
+            advance(ahead);
+            if (asked + 1 < n_units) page_next = page_of(ahead);
+        }
+        asked++;
+        copies_commit();
+    };
+    // Positions that were cached before this step do not depend on the kernel before this one, which writes the step's own: where
+    // the first chunks are older, they are asked for at once, and only then come the wait and the queries.
+    const bool early = p.seq_past != nullptr && now.unit + S::STAGES - 2 <= now.last && min((now.unit + S::STAGES - 1) * UNIT - 1, now.pos) < p.seq_past[now.seq];
+    if (!early) pdl_wait();
+#pragma unroll
+    for (int s = 0; s < S::STAGES - 1; s++) load();
+    if (early) pdl_wait();
+
+    const bf16* q = behind_wait(p.q);
+    const int pairs = p.hd / 2, part = S::ROWS * (p.hd + 2);             // floats of a part: the sums, then (m, l) of the rows
+    auto head_of = [&](const Cursor& c) { return c.kvb / per_kv * group + c.kvb % per_kv * S::ROWS; };
+    auto rows_of = [&](const Cursor& c) { return min(S::ROWS, group - c.kvb % per_kv * S::ROWS); };
+    S x;
+    uint2 raw[NT][HD / 16];
+    S::ask_queries(raw, q + ((size_t)now.row * p.nh + head_of(now)) * p.hd, p.hd, rows_of(now), p.hd, lane);
+    int began = now.unit;                      // the first of the pair's units that is this block's
+    x.begin(raw, p.scale_log2, lane);
+    for (int i = 0; i < n_units; i++) {
+        copies_wait<S::STAGES - 2>();
+        __syncwarp();                          // every lane's pieces of chunk i are there, and all have read chunk i - 1
+        load();
+        unsigned char* st = ring + (i % S::STAGES) * S::STAGE;
+        x.chunk(st, now.unit * UNIT + warp * CHUNK, now.lo, now.pos, 0, 0, lane);
+        const Cursor done = now;
+        advance(now);
+        if (done.unit < done.last && i + 1 < n_units) continue;
+        // ---- the pair's end, or the block's.  The next pair's queries are on their way meanwhile; the stage that has just been read
+        // takes the warp's sums (its next chunk is asked for behind the second meeting).
+        const int rows = rows_of(done), head = head_of(done);
+        if (i + 1 < n_units) S::ask_queries(raw, q + ((size_t)now.row * p.nh + head_of(now)) * p.hd, p.hd, rows_of(now), p.hd, lane);
+        __syncwarp();
+        x.leave(m_s[warp], l_s[warp], reinterpret_cast<float*>(st), lane);
+        __syncthreads();
+        const bool from_start = began == done.lo / UNIT, to_end = done.unit == done.last;
+        float* mine = p.parts + ((size_t)blockIdx.x * 2 + (from_start ? 1 : 0)) * part;
+        const unsigned char* sums = smem + (i % S::STAGES) * S::STAGE;
+        for (int idx = threadIdx.x; idx < rows * pairs; idx += THREADS) {
+            const int r = idx / pairs, d = (idx % pairs) * 2;
+            const Joined y = join_warps<S::ROWS, HD>(m_s, l_s, sums, Ring<HD>::WARP, r, d);
+            if (from_start && to_end) {
+                store_pair(p.out + ((size_t)done.row * p.nh + head + r) * p.hd + d, y.a * inverse(y.l), y.b * inverse(y.l));
+            } else {
+                *reinterpret_cast<float2*>(mine + r * p.hd + d) = make_float2(y.a, y.b);
+                if (d == 0) *reinterpret_cast<float2*>(mine + S::ROWS * p.hd + 2 * r) = make_float2(y.m, y.l);
+            }
+        }
+        if (!(from_start && to_end)) {
+            // ---- the last of the pair's blocks to finish joins their parts, in the order of the blocks; where they are many, the
+            // last of every PARTS blocks joins theirs first, and the last of all the groups'
+            const int each = before[done.row + 1] - before[done.row];
+            const long long p0 = (long long)before[done.row] * kv_blocks + (long long)done.kvb * each, p1 = p0 + each - 1;
+            // unit u belongs to the last block b with total * b / blocks <= u
+            const int b0 = (int)(((p0 + 1) * blocks - 1) / total), b1 = (int)(((p1 + 1) * blocks - 1) / total);
+            auto part_of = [&](int b) { return p.parts + ((size_t)b * 2 + (b == b0 ? 1 : 0)) * part; };
+            // the parts of the blocks first, first + step, ... (the first of them aligned to ``step``): to ``out`` or, normalised no
+            // further, into the first one's place
+            auto join_parts = [&](int first, int step, int count, bool to_out) {
+                auto nth = [&](int u) { return part_of(u == 0 ? first : first / step * step + u * step); };
+                for (int idx = threadIdx.x; idx < rows * count; idx += THREADS)
+                    ml_s[idx / count][idx % count] = __ldcg(reinterpret_cast<const float2*>(nth(idx % count) + S::ROWS * p.hd + 2 * (idx / count)));
+                __syncthreads();
+                constexpr int MINE = (S::ROWS * HD / 4 + THREADS - 1) / THREADS;           // pieces of four channels of a thread
+                float4 got[MINE];
+                float most[MINE], sum[MINE];
+                const int quads = p.hd / 4;
+#pragma unroll
+                for (int i2 = 0; i2 < MINE; i2++) {
+                    const int idx = threadIdx.x + i2 * THREADS, r = idx / quads, d = idx % quads * 4;
+                    got[i2] = make_float4(0.f, 0.f, 0.f, 0.f);
+                    most[i2] = -INFINITY, sum[i2] = 0.f;
+                    if (r >= rows) continue;
+                    for (int u = 0; u < count; u++) most[i2] = fmaxf(most[i2], ml_s[r][u].x);
+#pragma unroll 8
+                    for (int u = 0; u < count; u++) {
+                        const float4 v = __ldcg(reinterpret_cast<const float4*>(nth(u) + r * p.hd + d));
+                        const float2 ml = ml_s[r][u];
+                        const float w = ml.x == -INFINITY ? 0.f : exp2_fast(ml.x - most[i2]);
+                        sum[i2] += ml.y * w;
+                        got[i2].x += v.x * w, got[i2].y += v.y * w, got[i2].z += v.z * w, got[i2].w += v.w * w;
+                    }
+                }
+                __syncthreads();
+#pragma unroll
+                for (int i2 = 0; i2 < MINE; i2++) {
+                    const int idx = threadIdx.x + i2 * THREADS, r = idx / quads, d = idx % quads * 4;
+                    if (r >= rows) continue;
+                    if (to_out) {
+                        const float inv = inverse(sum[i2]);
+                        bf16* to = p.out + ((size_t)done.row * p.nh + head + r) * p.hd + d;
+                        store_pair(to, got[i2].x * inv, got[i2].y * inv);
+                        store_pair(to + 2, got[i2].z * inv, got[i2].w * inv);
+                    } else {
+                        float* to = part_of(first);
+                        *reinterpret_cast<float4*>(to + r * p.hd + d) = got[i2];
+                        if (d == 0) *reinterpret_cast<float2*>(to + S::ROWS * p.hd + 2 * r) = make_float2(most[i2], sum[i2]);
+                    }
+                }
+            };
+            // whether this block is the last of ``count`` that come to the counter
+            auto am_last = [&](int* c, int count) {
+                __threadfence();
+                __syncthreads();
+                if (threadIdx.x == 0) {
+                    is_last = atomicAdd(c, 1) == count - 1;
+                    if (is_last) *c = 0;
+                }
+                __syncthreads();
+                if (is_last) __threadfence();
+                return is_last != 0;
+            };
+            int* of_pair = p.counters + (size_t)done.row * kv_blocks + done.kvb;
+            if (b1 - b0 < PARTS) {
+                if (am_last(of_pair, b1 - b0 + 1)) join_parts(b0, 1, b1 - b0 + 1, true);
+            } else {
+                const int g = blockIdx.x / PARTS, g0 = b0 / PARTS, g1 = b1 / PARTS, first = max(b0, g * PARTS), last = min(b1, g * PARTS + PARTS - 1);
+                // a group's counter: that of its first block, which no other pair's group shares (two slots a block)
+                if (am_last(p.counters + (size_t)p.n_rows * kv_blocks + 2 * first + (first == b0 ? 1 : 0), last - first + 1)) {
+                    join_parts(first, 1, last - first + 1, false);
+                    if (am_last(of_pair, g1 - g0 + 1)) join_parts(b0, PARTS, g1 - g0 + 1, true);
+                }
+            }
+        }
+        __syncthreads();                       // the lists and the stages may be written again
+        if (i + 1 < n_units) {
+            began = now.unit;
+            x.begin(raw, p.scale_log2, lane);
+        }
+    }
+    copies_wait<0>();
+}
+
+template <typename Kernel> int launch(Kernel kernel, size_t smem, bool (&raised)[64], const Params& p, dim3 grid, cudaStream_t stream) {
     int device = 0;
     if (cudaGetDevice(&device) != cudaSuccess || device < 0 || device >= 64) return (int)cudaErrorInvalidDevice;
-    if (!raised[device]) {
-        const cudaError_t e = cudaFuncSetAttribute(attn_kv8_kernel<HD, NT, RUN>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+    if (!raised[device]) {                                               // per device
+        const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
         if (e != cudaSuccess) return (int)e;
         raised[device] = true;
     }
-    esp_launch_pdl(ESP_PDL_ATTENTION, attn_kv8_kernel<HD, NT, RUN>, grid, dim3(THREADS), smem, stream, p);
+    esp_launch_pdl(ESP_PDL_ATTENTION, kernel, grid, dim3(THREADS), smem, stream, p);
     return esp_launch_status();
 }
-template <int NT, bool RUN> int launch_size(const Params& p, dim3 grid, cudaStream_t stream) {
-    if (p.hd <= 64) return launch<64, NT, RUN>(p, grid, stream);
-    if (p.hd <= 128) return launch<128, NT, RUN>(p, grid, stream);
-    return launch<256, NT, RUN>(p, grid, stream);
+template <int HD, int NT> int launch_decode(const Params& p, int blocks, cudaStream_t stream) {
+    static bool raised[64] = {false};
+    return launch(attn_decode_kv8_kernel<HD, NT>, (size_t)WARPS * Ring<HD>::WARP, raised, p, dim3(blocks), stream);
+}
+template <int HD> int launch_run(const Params& p, int n_tiles, cudaStream_t stream) {
+    static bool raised[64] = {false};
+    return launch(attn_run_kv8_kernel<HD, 2>, (size_t)WARPS * Ring<HD>::WARP, raised, p, dim3((unsigned)n_tiles * 8u, p.nh), stream);
 }
 bool sizes_fit(int nh, int nkv, int hd) { return nkv > 0 && nh > 0 && nh % nkv == 0 && nh <= 65535 && hd > 0 && hd % 8 == 0 && hd <= 256; }
-}  // namespace
-
-// One token row of the step per block row.  ``split``: key positions a block, a multiple of 64; n_splits * split covers
-// the longest row.  Where n_splits > 1: scratch float [n_tokens * nh * n_splits * (hd + 2)], counters
-// int [n_tokens * nh], zero when the call starts and when it ends.  ``seq_past`` (may be null): per sequence
-// of the step, the positions cached before it.
-ESP_API int esp_attn_decode_kv8(const void* q, const void* k, const void* v, const void* exps, void* out, float* scratch, int* counters,
-                                const int* tok_seq, const int* tok_pos, const int* seq_past, const int* block_table,
-                                int table_stride, int n_pages, int n_tokens, int nh, int nkv, int hd, int window, int split, int n_splits,
-                                int* status, cudaStream_t stream) {
-    if (n_tokens <= 0) return 0;
-    if (!sizes_fit(nh, nkv, hd) || n_splits <= 0 || n_splits > 65535 || split < KV8_PAGE || split % KV8_PAGE || window < 0 ||
-        (n_splits > 1 && (!scratch || !counters)) || (long long)split * n_splits < (long long)table_stride * KV8_PAGE)
-        return (int)cudaErrorInvalidValue;
+Params make_params(const void* q, const void* k, const void* v, const void* exps, void* out, const int* block_table, int table_stride, int n_pages, int nh,
+                   int nkv, int hd, int window, int* status) {
     Params p{};
     p.q = (const bf16*)q, p.k = (const unsigned char*)k, p.v = (const unsigned char*)v, p.exps = (const unsigned char*)exps, p.out = (bf16*)out;
-    p.part_o = scratch, p.part_ml = scratch ? scratch + (size_t)n_tokens * nh * n_splits * hd : nullptr, p.counters = counters, p.tok_seq = tok_seq, p.tok_pos = tok_pos, p.seq_past = seq_past;
     p.block_table = block_table, p.table_stride = table_stride, p.n_pages = n_pages, p.nh = nh, p.nkv = nkv, p.hd = hd, p.window = window;
-    p.split_keys = split, p.n_splits = n_splits, p.status = status;
     p.scale_log2 = (float)(1.4426950408889634 / sqrt((double)hd));
-    const int group = nh / nkv;
-    if (group <= 8) return launch_size<1, false>(p, dim3(n_tokens, nkv, n_splits), stream);
-    return launch_size<2, false>(p, dim3(n_tokens, nkv * ((group + 15) / 16), n_splits), stream);
+    p.status = status;
+    return p;
+}
+}  // namespace
+
+// One token row of a sequence per row of q.  ``blocks``: the size of the grid, best what the device holds at once.  Scratch: parts
+// float [blocks * 2 * 16 * (hd + 2)]; counters int [min(n_tokens, 1024) * nh + 2 * blocks], zero when the call starts and when it ends.  ``seq_past``
+// (may be null): per sequence of the step, the positions cached before it.
+ESP_API int esp_attn_decode_kv8(const void* q, const void* k, const void* v, const void* exps, void* out, float* parts, int* counters,
+                                const int* tok_seq, const int* tok_pos, const int* seq_past, const int* block_table, int table_stride, int n_pages,
+                                int n_tokens, int nh, int nkv, int hd, int window, int blocks, int* status, cudaStream_t stream) {
+    if (n_tokens <= 0) return 0;
+    if (!sizes_fit(nh, nkv, hd) || blocks <= 0 || blocks > PARTS * (MOST_PARTS - 2) || window < 0 || table_stride <= 0 || table_stride > (1 << 25) || !parts || !counters)
+        return (int)cudaErrorInvalidValue;
+    Params p = make_params(q, k, v, exps, out, block_table, table_stride, n_pages, nh, nkv, hd, window, status);
+    p.parts = parts, p.counters = counters, p.seq_past = seq_past;
+    const bool wide = nh / nkv > 8;
+    for (int at = 0; at < n_tokens; at += MAX_ROWS) {                    // more rows than a block's list holds: one call behind the other
+        p.n_rows = n_tokens - at < MAX_ROWS ? n_tokens - at : MAX_ROWS;
+        p.tok_seq = tok_seq + at, p.tok_pos = tok_pos + at;
+        p.q = (const bf16*)q + (size_t)at * nh * hd, p.out = (bf16*)out + (size_t)at * nh * hd;
+        int rc;
+        if (hd <= 64) rc = wide ? launch_decode<64, 2>(p, blocks, stream) : launch_decode<64, 1>(p, blocks, stream);
+        else if (hd <= 128) rc = wide ? launch_decode<128, 2>(p, blocks, stream) : launch_decode<128, 1>(p, blocks, stream);
+        else rc = wide ? launch_decode<256, 2>(p, blocks, stream) : launch_decode<256, 1>(p, blocks, stream);
+        if (rc) return rc;
+    }
+    return 0;
 }
 
 // Runs of new tokens: tiles of 128 of a sequence (sequence, its first token among the sequence's new ones).
@@ -516,11 +707,9 @@ ESP_API int esp_attn_run_kv8(const void* q, const void* k, const void* v, const 
                              int n_pages, int n_tiles, int nh, int nkv, int hd, int window, int* status, cudaStream_t stream) {
     if (n_tiles <= 0) return 0;
     if (!sizes_fit(nh, nkv, hd) || window < 0 || n_tiles > (1 << 26)) return (int)cudaErrorInvalidValue;
-    Params p{};
-    p.q = (const bf16*)q, p.k = (const unsigned char*)k, p.v = (const unsigned char*)v, p.exps = (const unsigned char*)exps, p.out = (bf16*)out;
+    Params p = make_params(q, k, v, exps, out, block_table, table_stride, n_pages, nh, nkv, hd, window, status);
     p.tile_seq = tile_seq, p.tile_first = tile_first, p.seq_start = seq_start, p.seq_past = seq_past;
-    p.block_table = block_table, p.table_stride = table_stride, p.n_pages = n_pages, p.nh = nh, p.nkv = nkv, p.hd = hd, p.window = window;
-    p.split_keys = 1 << 30, p.n_splits = 1, p.tile_rows = 128, p.status = status;
-    p.scale_log2 = (float)(1.4426950408889634 / sqrt((double)hd));
-    return launch_size<2, true>(p, dim3((unsigned)n_tiles * 8u, nh), stream);
+    if (hd <= 64) return launch_run<64>(p, n_tiles, stream);
+    if (hd <= 128) return launch_run<128>(p, n_tiles, stream);
+    return launch_run<256>(p, n_tiles, stream);
 }

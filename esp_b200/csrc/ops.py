@@ -112,7 +112,7 @@ _SIGNATURES = {
     "esp_attn_decode_diff": [P, P, P, P, P, P, P, P, P, P, P, c_int, c_int, c_int, c_int, c_int, c_int, c_int, c_int, c_int,
                              c_int, c_int, c_float, c_int, c_float, c_float, c_float, c_float, P, c_longlong, P, P],
     "esp_kv8_append": [P, P, P, P, P, P, c_int, c_int, P, P, P, P, P, c_int, c_int, c_int, c_int, c_int, c_int, c_int, P, P],
-    "esp_attn_decode_kv8": [P, P, P, P, P, P, P, P, P, P, P, c_int, c_int, c_int, c_int, c_int, c_int, c_int, c_int, c_int, P, P],
+    "esp_attn_decode_kv8": [P, P, P, P, P, P, P, P, P, P, P, c_int, c_int, c_int, c_int, c_int, c_int, c_int, c_int, P, P],
     "esp_attn_prefill_kv8": [P, c_longlong, P, P, P, P, P, P, P, P, P, c_int, c_int, c_int, c_int, c_int, c_int, c_int, P, P],
     "esp_attn_run_kv8": [P, P, P, P, P, P, P, P, P, P, c_int, c_int, c_int, c_int, c_int, c_int, c_int, P, P],
 }
@@ -1633,18 +1633,13 @@ def _sm_count(device: int) -> int:
     return torch.cuda.get_device_properties(device).multi_processor_count
 
 
-@functools.lru_cache(maxsize=4096)
-def attn_decode_kv8_split(n_rows: int, kv_blocks: int, positions: int, sm_count: int = 148) -> int:
-    """Key positions a block of ``attn_decode_kv8``, whole pages of 64, the same for every row of the step."""
-    pages, room = max(1, (positions + 63) // 64), 2 * sm_count
-    pairs = max(1, n_rows * kv_blocks)
-    parts = max(1, min(pages // 4, room // pairs))
-    return 64 * ((pages + parts - 1) // parts)
+# blocks of the decode kernel that an SM holds at a time, by the width that heads are padded to (shared memory: 66, 99, 131 KB)
+ATTN_DECODE_KV8_BLOCKS_PER_SM = {64: 3, 128: 2, 256: 1}
 
 
 def attn_decode_kv8(q, k, v, exps, out, ws, tok_seq, tok_pos, block_table, page, nh, nkv, hd, window, status, seq_past=None):
-    """Attention of one token row per sequence (or of any rows, each on its own) over the 8-bit cache, split over the keys:
-    scores over sqrt(hd), keys max(0, pos - window + 1) .. pos (``window`` None or 0: all).  q and out bfloat16 [N, nh * hd];
+    """Attention of one token row per sequence (or of any rows, each on its own) over the 8-bit cache, the keys of all rows
+    dealt out evenly over the device: scores over sqrt(hd), keys max(0, pos - window + 1) .. pos (``window`` None or 0: all).  q and out bfloat16 [N, nh * hd];
     query head i reads key/value head i // (nh / nkv).  ``ws``: the ``Workspace`` that holds the scratch; calls that may
     overlap on the device (other streams, captured graphs replayed beside each other) need one each.  ``seq_past``
     (int32 per sequence of the step: positions that were cached before the step's copies to the device): blocks whose
@@ -1667,17 +1662,13 @@ def attn_decode_kv8(q, k, v, exps, out, ws, tok_seq, tok_pos, block_table, page,
                     (("tok_seq", tok_seq, n), ("tok_pos", tok_pos, n), ("seq_past", seq_past, block_table.shape[0])),
                     (("the queries", q), ("the keys", k), ("the values", v), ("the exponents", exps), ("the results", out)))
     stride = block_table.shape[1]
-    positions, group = stride * page, nh // nkv
-    split = attn_decode_kv8_split(n, nkv * ((group + 15) // 16), min(positions, window + page) if window else positions, _sm_count(_device_index))
-    n_splits = max(1, (positions + split - 1) // split)
-    scratch = counters = None
-    if n_splits > 1:
-        scratch = _ptr(ws.get("attn_kv8_parts", (n * nh * n_splits, hd + 2), _F32))
-        counters = _ptr(ws.get("attn_kv8_counters", (n * nh,), torch.int32, zeroed=True))
+    blocks = ATTN_DECODE_KV8_BLOCKS_PER_SM[64 if hd <= 64 else 128 if hd <= 128 else 256] * _sm_count(_device_index)
+    parts = _ptr(ws.get("attn_kv8_parts", (blocks * 32, hd + 2), _F32))
+    counters = _ptr(ws.get("attn_kv8_counters", (min(n, 1024) * nh + 2 * blocks,), torch.int32, zeroed=True))
     _check(_fn("kv8", "esp_attn_decode_kv8")(
-        q_, k_, v_, e_, o_, scratch, counters, _ptr(tok_seq, torch.int32, "tok_seq"), _ptr(tok_pos, torch.int32, "tok_pos"),
+        q_, k_, v_, e_, o_, parts, counters, _ptr(tok_seq, torch.int32, "tok_seq"), _ptr(tok_pos, torch.int32, "tok_pos"),
         _ptr(seq_past, torch.int32, "seq_past"), _ptr(block_table, torch.int32, "page table"), stride, k.shape[0], n, nh, nkv, hd, int(window or 0),
-        split, n_splits, _ptr(status, torch.int32, "status"), _stream()), "attn_decode_kv8")
+        blocks, _ptr(status, torch.int32, "status"), _stream()), "attn_decode_kv8")
 
 
 def attn_prefill_kv8(q, k, v, exps, out, tile_seq, tile_first, seq_start, seq_past, block_table, page, nh, nkv, hd, window, status):

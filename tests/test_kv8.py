@@ -97,10 +97,3 @@ def append(**change):
 def test_append_refuses(change, why):
     with pytest.raises(Backend, match=why):
         append(**change)
-
-
-def test_split_covers_every_length():
-    for rows in (1, 3, 64, 500):
-        for positions in (1, 64, 65, 777, 8192, 131072):
-            split = ops.attn_decode_kv8_split(rows, 4, positions)
-            assert split % 64 == 0 and split > 0
