@@ -27,7 +27,7 @@
 namespace {
 constexpr int THREADS = 128, WARPS = 4, CHUNK = 32, UNIT = WARPS * CHUNK, MAX_ROWS = 1024;
 constexpr float WEIGHT_TOP = 6.f, LAG_TOP = 8.f, LAG_SUM = 40.f;
-constexpr int PARTS = 16, MOST_PARTS = 48;     // parts that one block joins; of a pair's, or its groups of PARTS blocks
+constexpr int PARTS = 16;                      // of a pair, that one block joins
 
 struct Params {
     const bf16* q;
@@ -417,7 +417,7 @@ __global__ void __launch_bounds__(THREADS) attn_decode_kv8_kernel(const Params p
     __shared__ float m_s[WARPS][S::ROWS], l_s[WARPS][S::ROWS];
     __shared__ int before[MAX_ROWS + 1];       // units of one key head ahead of each row
     __shared__ int warp_sum_s[WARPS], is_last;
-    __shared__ float2 ml_s[S::ROWS][MOST_PARTS];                         // of the parts that are joined
+    __shared__ float2 joined_ml[S::ROWS];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     unsigned char* ring = smem + warp * Ring<HD>::WARP;
     const int group = p.nh / p.nkv, per_kv = (group + S::ROWS - 1) / S::ROWS, kv_blocks = p.nkv * per_kv;
@@ -501,40 +501,56 @@ __global__ void __launch_bounds__(THREADS) attn_decode_kv8_kernel(const Params p
         now.unit = now.lo / UNIT + (int)(in_row % each);
     }
     const int n_units = (int)(u1 - u0);
-    Cursor ahead = now;                        // of the next chunk that is asked for
+    Cursor ahead = now;                        // of the chunk behind the one that is asked for next
     int asked = 0;
     auto page_of = [&](const Cursor& c) { return p.block_table[(size_t)c.seq * p.table_stride + min(c.unit * UNIT + warp * CHUNK, c.pos) / KV8_PAGE]; };
-    int page_next = page_of(ahead);
-    auto load = [&]() {                        // the next chunk of this warp, into the ring's next stage
-        if (asked < n_units) {
-            S::ask(p, ring + (asked % S::STAGES) * S::STAGE, page_next, ahead.kvb / per_kv, ahead.unit * UNIT + warp * CHUNK, ahead.lo, ahead.pos, lane);
-            advance(ahead);
-            if (asked + 1 < n_units) page_next = page_of(ahead);
-        }
+    // the next chunk of this warp, into the ring's next stage
+    auto load = [&](const Cursor& c, int page) {
+        if (asked < n_units) S::ask(p, ring + (asked % S::STAGES) * S::STAGE, page, c.kvb / per_kv, c.unit * UNIT + warp * CHUNK, c.lo, c.pos, lane);
         asked++;
         copies_commit();
     };
+    // the first chunks' pages are looked up at once, the later ones' one chunk ahead
+    Cursor first[S::STAGES];
+    int first_page[S::STAGES];
+#pragma unroll
+    for (int i = 0; i < S::STAGES; i++) {
+        first[i] = ahead;
+        first_page[i] = page_of(ahead);
+        if (i + 1 < n_units) advance(ahead);
+    }
+    auto head_of = [&](const Cursor& c) { return c.kvb / per_kv * group + c.kvb % per_kv * S::ROWS; };
+    auto rows_of = [&](const Cursor& c) { return min(S::ROWS, group - c.kvb % per_kv * S::ROWS); };
     // Positions that were cached before this step do not depend on the kernel before this one, which writes the step's own: where
     // the first chunks are older, they are asked for at once, and only then come the wait and the queries.
     const bool early = p.seq_past != nullptr && now.unit + S::STAGES - 2 <= now.last && min((now.unit + S::STAGES - 1) * UNIT - 1, now.pos) < p.seq_past[now.seq];
-    if (!early) pdl_wait();
-#pragma unroll
-    for (int s = 0; s < S::STAGES - 1; s++) load();
-    if (early) pdl_wait();
-
-    const bf16* q = behind_wait(p.q);
-    const int pairs = p.hd / 2, part = S::ROWS * (p.hd + 2);             // floats of a part: the sums, then (m, l) of the rows
-    auto head_of = [&](const Cursor& c) { return c.kvb / per_kv * group + c.kvb % per_kv * S::ROWS; };
-    auto rows_of = [&](const Cursor& c) { return min(S::ROWS, group - c.kvb % per_kv * S::ROWS); };
-    S x;
     uint2 raw[NT][HD / 16];
-    S::ask_queries(raw, q + ((size_t)now.row * p.nh + head_of(now)) * p.hd, p.hd, rows_of(now), p.hd, lane);
+    const bf16* q;
+    auto ask_first = [&]() {
+        pdl_wait();
+        q = behind_wait(p.q);
+        S::ask_queries(raw, q + ((size_t)now.row * p.nh + head_of(now)) * p.hd, p.hd, rows_of(now), p.hd, lane);
+    };
+    if (!early) ask_first();
+#pragma unroll
+    for (int i = 0; i < S::STAGES - 1; i++) load(first[i], first_page[i]);
+    if (early) ask_first();
+    Cursor next = first[S::STAGES - 1];
+    int page_next = first_page[S::STAGES - 1];
+
+    const int pairs = p.hd / 2, part = S::ROWS * (p.hd + 2);             // floats of a part: the sums, then (m, l) of the rows
+    S x;
     int began = now.unit;                      // the first of the pair's units that is this block's
     x.begin(raw, p.scale_log2, lane);
     for (int i = 0; i < n_units; i++) {
         copies_wait<S::STAGES - 2>();
         __syncwarp();                          // every lane's pieces of chunk i are there, and all have read chunk i - 1
-        load();
+        load(next, page_next);
+        if (asked < n_units) {
+            next = ahead;
+            page_next = page_of(next);
+            if (asked + 1 < n_units) advance(ahead);
+        }
         unsigned char* st = ring + (i % S::STAGES) * S::STAGE;
         x.chunk(st, now.unit * UNIT + warp * CHUNK, now.lo, now.pos, 0, 0, lane);
         const Cursor done = now;
@@ -568,60 +584,67 @@ __global__ void __launch_bounds__(THREADS) attn_decode_kv8_kernel(const Params p
             // unit u belongs to the last block b with total * b / blocks <= u
             const int b0 = (int)(((p0 + 1) * blocks - 1) / total), b1 = (int)(((p1 + 1) * blocks - 1) / total);
             auto part_of = [&](int b) { return p.parts + ((size_t)b * 2 + (b == b0 ? 1 : 0)) * part; };
-            // the parts of the blocks first, first + step, ... (the first of them aligned to ``step``): to ``out`` or, normalised no
-            // further, into the first one's place
+            // the parts of the blocks first, first + step, ... (those behind the first aligned to ``step``): to the output or, not
+            // normalised, into the first one's place.  Eight parts are on their way at a time.
             auto join_parts = [&](int first, int step, int count, bool to_out) {
                 auto nth = [&](int u) { return part_of(u == 0 ? first : first / step * step + u * step); };
-                for (int idx = threadIdx.x; idx < rows * count; idx += THREADS)
-                    ml_s[idx / count][idx % count] = __ldcg(reinterpret_cast<const float2*>(nth(idx % count) + S::ROWS * p.hd + 2 * (idx / count)));
-                __syncthreads();
-                constexpr int MINE = (S::ROWS * HD / 4 + THREADS - 1) / THREADS;           // pieces of four channels of a thread
-                float4 got[MINE];
-                float most[MINE], sum[MINE];
                 const int quads = p.hd / 4;
+                for (int idx = threadIdx.x; idx < rows * quads; idx += THREADS) {
+                    const int r = idx / quads, d = idx % quads * 4;
+                    float4 got = make_float4(0.f, 0.f, 0.f, 0.f);
+                    float most = -INFINITY, sum = 0.f;
+                    for (int u0 = 0; u0 < count; u0 += 8) {
+                        float4 v[8];
+                        float2 ml[8];
 #pragma unroll
-                for (int i2 = 0; i2 < MINE; i2++) {
-                    const int idx = threadIdx.x + i2 * THREADS, r = idx / quads, d = idx % quads * 4;
-                    got[i2] = make_float4(0.f, 0.f, 0.f, 0.f);
-                    most[i2] = -INFINITY, sum[i2] = 0.f;
-                    if (r >= rows) continue;
-                    for (int u = 0; u < count; u++) most[i2] = fmaxf(most[i2], ml_s[r][u].x);
-#pragma unroll 8
-                    for (int u = 0; u < count; u++) {
-                        const float4 v = __ldcg(reinterpret_cast<const float4*>(nth(u) + r * p.hd + d));
-                        const float2 ml = ml_s[r][u];
-                        const float w = ml.x == -INFINITY ? 0.f : exp2_fast(ml.x - most[i2]);
-                        sum[i2] += ml.y * w;
-                        got[i2].x += v.x * w, got[i2].y += v.y * w, got[i2].z += v.z * w, got[i2].w += v.w * w;
+                        for (int u = 0; u < 8; u++) {
+                            ml[u] = make_float2(-INFINITY, 0.f);
+                            v[u] = make_float4(0.f, 0.f, 0.f, 0.f);
+                            if (u0 + u < count) {
+                                ml[u] = __ldcg(reinterpret_cast<const float2*>(nth(u0 + u) + S::ROWS * p.hd + 2 * r));
+                                v[u] = __ldcg(reinterpret_cast<const float4*>(nth(u0 + u) + r * p.hd + d));
+                            }
+                        }
+                        float m8 = most;
+#pragma unroll
+                        for (int u = 0; u < 8; u++) m8 = fmaxf(m8, ml[u].x);
+                        const float f = most == -INFINITY ? (m8 == -INFINITY ? 1.f : 0.f) : exp2_fast(most - m8);
+                        sum *= f;
+                        got.x *= f, got.y *= f, got.z *= f, got.w *= f;
+#pragma unroll
+                        for (int u = 0; u < 8; u++) {
+                            const float w = ml[u].x == -INFINITY ? 0.f : exp2_fast(ml[u].x - m8);
+                            sum += ml[u].y * w;
+                            got.x += v[u].x * w, got.y += v[u].y * w, got.z += v[u].z * w, got.w += v[u].w * w;
+                        }
+                        most = m8;
+                    }
+                    if (to_out) {
+                        const float inv = inverse(sum);
+                        bf16* to = p.out + ((size_t)done.row * p.nh + head + r) * p.hd + d;
+                        store_pair(to, got.x * inv, got.y * inv);
+                        store_pair(to + 2, got.z * inv, got.w * inv);
+                    } else {                   // nobody but this thread reads this piece of the first part
+                        float* to = part_of(first);
+                        *reinterpret_cast<float4*>(to + r * p.hd + d) = got;
+                        if (d == 0) joined_ml[r] = make_float2(most, sum);
                     }
                 }
-                __syncthreads();
-#pragma unroll
-                for (int i2 = 0; i2 < MINE; i2++) {
-                    const int idx = threadIdx.x + i2 * THREADS, r = idx / quads, d = idx % quads * 4;
-                    if (r >= rows) continue;
-                    if (to_out) {
-                        const float inv = inverse(sum[i2]);
-                        bf16* to = p.out + ((size_t)done.row * p.nh + head + r) * p.hd + d;
-                        store_pair(to, got[i2].x * inv, got[i2].y * inv);
-                        store_pair(to + 2, got[i2].z * inv, got[i2].w * inv);
-                    } else {
-                        float* to = part_of(first);
-                        *reinterpret_cast<float4*>(to + r * p.hd + d) = got[i2];
-                        if (d == 0) *reinterpret_cast<float2*>(to + S::ROWS * p.hd + 2 * r) = make_float2(most[i2], sum[i2]);
-                    }
+                if (!to_out) {                 // (m, l) of the first part are read by all of a row's threads
+                    __syncthreads();
+                    if (threadIdx.x < rows) *reinterpret_cast<float2*>(part_of(first) + S::ROWS * p.hd + 2 * threadIdx.x) = joined_ml[threadIdx.x];
                 }
             };
             // whether this block is the last of ``count`` that come to the counter
             auto am_last = [&](int* c, int count) {
-                __threadfence();
                 __syncthreads();
                 if (threadIdx.x == 0) {
+                    __threadfence();           // the block's parts are there before its count (the fence covers what the barrier has ordered)
                     is_last = atomicAdd(c, 1) == count - 1;
                     if (is_last) *c = 0;
+                    __threadfence();
                 }
                 __syncthreads();
-                if (is_last) __threadfence();
                 return is_last != 0;
             };
             int* of_pair = p.counters + (size_t)done.row * kv_blocks + done.kvb;
@@ -683,7 +706,7 @@ ESP_API int esp_attn_decode_kv8(const void* q, const void* k, const void* v, con
                                 const int* tok_seq, const int* tok_pos, const int* seq_past, const int* block_table, int table_stride, int n_pages,
                                 int n_tokens, int nh, int nkv, int hd, int window, int blocks, int* status, cudaStream_t stream) {
     if (n_tokens <= 0) return 0;
-    if (!sizes_fit(nh, nkv, hd) || blocks <= 0 || blocks > PARTS * (MOST_PARTS - 2) || window < 0 || table_stride <= 0 || table_stride > (1 << 25) || !parts || !counters)
+    if (!sizes_fit(nh, nkv, hd) || blocks <= 0 || window < 0 || table_stride <= 0 || table_stride > (1 << 25) || !parts || !counters)
         return (int)cudaErrorInvalidValue;
     Params p = make_params(q, k, v, exps, out, block_table, table_stride, n_pages, nh, nkv, hd, window, status);
     p.parts = parts, p.counters = counters, p.seq_past = seq_past;
