@@ -17,7 +17,10 @@
 // take the blocks of one tile in turn instead (SPLIT) and join their results.
 //
 // A position that is no number (kv8.cuh) is made a key of NaN with a value of zeros: whoever sees it gets NaN through the score,
-// and a masked score takes nothing of it.  Every wait is bounded.
+// and a masked score takes nothing of it.
+//
+// Every wait is bounded, and a warp whose wait runs out leaves; the waits that hang on it then run out too.  (A flag that every
+// wait looks at first cost 8 of 291 us.)
 #include "kv8.cuh"
 #include "tc05.cuh"
 
@@ -292,7 +295,7 @@ __global__ void __launch_bounds__(THREADS, 1) attn_prefill_kv8_kernel(const __gr
             unsigned begun = 0;                                           // a bit a group: its O holds something of this item
             auto issue_s = [&](const int g, int j, bool last_use, bool last) {
                 const int st = (b0 + j) % STAGES;
-                if (!__all_sync(0xffffffffu, !*abort_flag && mbar_wait(&k_full[st], ((b0 + j) / STAGES) & 1))) return false;
+                if (!__all_sync(0xffffffffu, mbar_wait(&k_full[st], ((b0 + j) / STAGES) & 1))) return false;
                 tc_fence_after();
                 const unsigned qa = dq + (pair ? (unsigned)(g * TILE) >> 4 : 0u), kb = dk + ((unsigned)(st * TILE) >> 4);
                 if (leader) {
@@ -311,7 +314,7 @@ __global__ void __launch_bounds__(THREADS, 1) attn_prefill_kv8_kernel(const __gr
             auto issue_pv = [&](const int g, int j, bool last_use, bool last) {
                 const int st = (b0 + j) % STAGES;
                 // the first P V of an item: the row threads have read the O of the item before
-                bool fine = !*abort_flag && ((begun >> g & 1) || mbar_wait(&o_free[g], (ph_o >> g & 1) ^ 1));
+                bool fine = (begun >> g & 1) || mbar_wait(&o_free[g], (ph_o >> g & 1) ^ 1);
                 fine = fine && mbar_wait(&v_full[st], ((b0 + j) / STAGES) & 1) && mbar_wait(&p_ready[g], ph_p >> g & 1);
                 if (!__all_sync(0xffffffffu, fine)) return false;
                 tc_fence_after();
@@ -485,7 +488,7 @@ __global__ void __launch_bounds__(THREADS, 1) attn_prefill_kv8_kernel(const __gr
                 }
             }
         };
-        auto wait_all = [&](unsigned long long* bar, int parity) { return (bool)__all_sync(0xffffffffu, !*abort_flag && mbar_wait(bar, parity)); };
+        auto wait_all = [&](unsigned long long* bar, int parity) { return (bool)__all_sync(0xffffffffu, mbar_wait(bar, parity)); };
         uint4 codes[R];
         bool ok = wait_all(&e_full[0], 0);
         if (ok && entries[0].hi >= 0) ask(codes, entries[0], p.k);
@@ -540,7 +543,7 @@ __global__ void __launch_bounds__(THREADS, 1) attn_prefill_kv8_kernel(const __gr
             float m_ref = -INFINITY, l_run = 0.f;                                    // the maximum that O and l_run are scaled by
             for (int j = j0; j <= j1; j += step, n_b++) {
                 const int key0 = (t.blk0 + j) * BN;
-                ok = !*abort_flag && mbar_wait(&s_full[grp], n_b & 1);
+                ok = mbar_wait(&s_full[grp], n_b & 1);
                 ok = __all_sync(0xffffffffu, ok);
                 tc_fence_after();
                 // live columns of an edge block: c_lo .. c_lo + c_span, one unsigned comparison each
