@@ -39,7 +39,7 @@ struct Params {
     const int *seq_past, *seq_start;           // per sequence (decode: seq_past may be null)
     const int *tile_seq, *tile_first;          // run: tiles of 128 new tokens
     const int* block_table;
-    int table_stride, n_pages, n_rows, nh, nkv, hd, window;
+    int n_seqs, table_stride, n_pages, n_rows, nh, nkv, hd, window;      // n_seqs: rows of the page table
     float scale_log2;                          // log2(e) / sqrt(hd)
     int* status;
 };
@@ -353,6 +353,10 @@ __global__ void __launch_bounds__(THREADS) attn_run_kv8_kernel(const Params p) {
     pdl_wait();
     // the block's rows: ``rows`` tokens from ``first`` on, all of head ``head``
     const int subs = 128 / S::ROWS, tile = blockIdx.x / subs, seq = p.tile_seq[tile], first = p.tile_first[tile] + (blockIdx.x % subs) * S::ROWS;
+    if (seq < 0 || seq >= p.n_seqs || first < 0) {
+        if (threadIdx.x == 0) atomicOr(p.status, ESP_STATUS_BAD_INDEX);
+        return;
+    }
     const int start = p.seq_start[seq], rows = min(S::ROWS, p.seq_start[seq + 1] - start - first), head = blockIdx.y, kvh = head / (p.nh / p.nkv);
     if (rows <= 0) return;
     const int pos0 = p.seq_past[seq] + first, k0 = first_visible_key(pos0, p.window, 0), k1 = pos0 + rows - 1;
@@ -434,7 +438,7 @@ __global__ void __launch_bounds__(THREADS) attn_decode_kv8_kernel(const Params p
         int mine = 0;
         if (r < p.n_rows) {
             const int pos = p.tok_pos[r];
-            mine = p.tok_seq[r] < 0 ? 0 : units_of(pos);
+            mine = p.tok_seq[r] < 0 || p.tok_seq[r] >= p.n_seqs ? 0 : units_of(pos);
             if (mine == 0 && blockIdx.x == 0) atomicOr(p.status, ESP_STATUS_BAD_INDEX);
         }
         int sum = mine;
@@ -688,11 +692,11 @@ template <int HD> int launch_run(const Params& p, int n_tiles, cudaStream_t stre
     return launch(attn_run_kv8_kernel<HD, 2>, (size_t)WARPS * Ring<HD>::WARP, raised, p, dim3((unsigned)n_tiles * 8u, p.nh), stream);
 }
 bool sizes_fit(int nh, int nkv, int hd) { return nkv > 0 && nh > 0 && nh % nkv == 0 && nh <= 65535 && hd > 0 && hd % 8 == 0 && hd <= 256; }
-Params make_params(const void* q, const void* k, const void* v, const void* exps, void* out, const int* block_table, int table_stride, int n_pages, int nh,
+Params make_params(const void* q, const void* k, const void* v, const void* exps, void* out, const int* block_table, int n_seqs, int table_stride, int n_pages, int nh,
                    int nkv, int hd, int window, int* status) {
     Params p{};
     p.q = (const bf16*)q, p.k = (const unsigned char*)k, p.v = (const unsigned char*)v, p.exps = (const unsigned char*)exps, p.out = (bf16*)out;
-    p.block_table = block_table, p.table_stride = table_stride, p.n_pages = n_pages, p.nh = nh, p.nkv = nkv, p.hd = hd, p.window = window;
+    p.block_table = block_table, p.n_seqs = n_seqs, p.table_stride = table_stride, p.n_pages = n_pages, p.nh = nh, p.nkv = nkv, p.hd = hd, p.window = window;
     p.scale_log2 = (float)(1.4426950408889634 / sqrt((double)hd));
     p.status = status;
     return p;
@@ -703,12 +707,12 @@ Params make_params(const void* q, const void* k, const void* v, const void* exps
 // float [blocks * 2 * 16 * (hd + 2)]; counters int [min(n_tokens, 1024) * nh + 2 * blocks], zero when the call starts and when it ends.  ``seq_past``
 // (may be null): per sequence of the step, the positions cached before it.
 ESP_API int esp_attn_decode_kv8(const void* q, const void* k, const void* v, const void* exps, void* out, float* parts, int* counters,
-                                const int* tok_seq, const int* tok_pos, const int* seq_past, const int* block_table, int table_stride, int n_pages,
+                                const int* tok_seq, const int* tok_pos, const int* seq_past, const int* block_table, int n_seqs, int table_stride, int n_pages,
                                 int n_tokens, int nh, int nkv, int hd, int window, int blocks, int* status, cudaStream_t stream) {
     if (n_tokens <= 0) return 0;
     if (!sizes_fit(nh, nkv, hd) || blocks <= 0 || window < 0 || table_stride <= 0 || table_stride > (1 << 25) || !parts || !counters)
         return (int)cudaErrorInvalidValue;
-    Params p = make_params(q, k, v, exps, out, block_table, table_stride, n_pages, nh, nkv, hd, window, status);
+    Params p = make_params(q, k, v, exps, out, block_table, n_seqs, table_stride, n_pages, nh, nkv, hd, window, status);
     p.parts = parts, p.counters = counters, p.seq_past = seq_past;
     const bool wide = nh / nkv > 8;
     for (int at = 0; at < n_tokens; at += MAX_ROWS) {                    // more rows than a block's list holds: one call behind the other
@@ -726,11 +730,11 @@ ESP_API int esp_attn_decode_kv8(const void* q, const void* k, const void* v, con
 
 // Runs of new tokens: tiles of 128 of a sequence (sequence, its first token among the sequence's new ones).
 ESP_API int esp_attn_run_kv8(const void* q, const void* k, const void* v, const void* exps, void* out, const int* tile_seq,
-                             const int* tile_first, const int* seq_start, const int* seq_past, const int* block_table, int table_stride,
+                             const int* tile_first, const int* seq_start, const int* seq_past, const int* block_table, int n_seqs, int table_stride,
                              int n_pages, int n_tiles, int nh, int nkv, int hd, int window, int* status, cudaStream_t stream) {
     if (n_tiles <= 0) return 0;
     if (!sizes_fit(nh, nkv, hd) || window < 0 || n_tiles > (1 << 26)) return (int)cudaErrorInvalidValue;
-    Params p = make_params(q, k, v, exps, out, block_table, table_stride, n_pages, nh, nkv, hd, window, status);
+    Params p = make_params(q, k, v, exps, out, block_table, n_seqs, table_stride, n_pages, nh, nkv, hd, window, status);
     p.tile_seq = tile_seq, p.tile_first = tile_first, p.seq_start = seq_start, p.seq_past = seq_past;
     if (hd <= 64) return launch_run<64>(p, n_tiles, stream);
     if (hd <= 128) return launch_run<128>(p, n_tiles, stream);

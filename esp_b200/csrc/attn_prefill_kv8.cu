@@ -40,7 +40,7 @@ struct Params {
     const unsigned char *k, *v, *exps;
     bf16* out;
     const int *tile_seq, *tile_first, *seq_start, *seq_past, *block_table;
-    int table_stride, n_pages, nh, nkv, hd, window, n_tiles, pair, smem_bytes;
+    int n_seqs, table_stride, n_pages, nh, nkv, hd, window, n_tiles, pair, smem_bytes;
     float scale_log2;
     int* status;
 };
@@ -236,7 +236,18 @@ __global__ void __launch_bounds__(THREADS, 1) attn_prefill_kv8_kernel(const __gr
         int n = 0;
         for (int i0 = 0; i0 < p.n_tiles; i0 += 32) {
             const int i = i0 + lane;
-            const bool live = i < p.n_tiles && (!p.pair || (p.tile_first[i] / BM) % 2 == 0);
+            bool live = i < p.n_tiles;
+            if (live) {
+                // a tile of a sequence that is not there, without rows, or with positions that the page table does not have is left out
+                const int seq = p.tile_seq[i], first = p.tile_first[i];
+                bool fine = seq >= 0 && seq < p.n_seqs && first >= 0;
+                if (fine) {
+                    const int news = p.seq_start[seq + 1] - p.seq_start[seq], past = p.seq_past[seq];
+                    fine = first < news && past >= 0 && (past + news - 1) / KV8_PAGE < p.table_stride;
+                }
+                if (!fine && blockIdx.x == 0) atomicOr(p.status, ESP_STATUS_BAD_INDEX);
+                live = fine && (!p.pair || (first / BM) % 2 == 0);
+            }
             const unsigned mask = __ballot_sync(0xffffffffu, live);
             if (live) list[n + __popc(mask & ((1u << lane) - 1u))] = (unsigned short)i;
             n += __popc(mask);
@@ -736,7 +747,7 @@ template <int HD> int launch(const CUtensorMap& map_q, Params p, int device, cud
 // q and out [n_tokens, nh, hd] bfloat16; tile_seq / tile_first: all tiles of 128 new tokens (sequence, the tile's first token among
 // the sequence's new ones), best listed with those that see the most keys first; hd a multiple of 8 up to 128.
 ESP_API int esp_attn_prefill_kv8(const void* q, long long n_tokens, const void* k, const void* v, const void* exps, void* out, const int* tile_seq,
-                                 const int* tile_first, const int* seq_start, const int* seq_past, const int* block_table, int table_stride,
+                                 const int* tile_first, const int* seq_start, const int* seq_past, const int* block_table, int n_seqs, int table_stride,
                                  int n_pages, int n_tiles, int nh, int nkv, int hd, int window, int* status, cudaStream_t stream) {
     if (n_tiles <= 0 || n_tokens <= 0) return 0;
     if (nkv <= 0 || nh <= 0 || nh % nkv || nh > 65535 || hd <= 0 || hd % 8 || hd > 128 || window < 0 || (long long)n_tiles * nh > 0x7fffffffLL)
@@ -748,7 +759,7 @@ ESP_API int esp_attn_prefill_kv8(const void* q, long long n_tokens, const void* 
     if (rc) return rc;
     Params p{};
     p.k = (const unsigned char*)k, p.v = (const unsigned char*)v, p.exps = (const unsigned char*)exps, p.out = (bf16*)out;
-    p.tile_seq = tile_seq, p.tile_first = tile_first, p.seq_start = seq_start, p.seq_past = seq_past, p.block_table = block_table;
+    p.tile_seq = tile_seq, p.tile_first = tile_first, p.seq_start = seq_start, p.seq_past = seq_past, p.block_table = block_table, p.n_seqs = n_seqs;
     p.table_stride = table_stride, p.n_pages = n_pages, p.nh = nh, p.nkv = nkv, p.hd = hd, p.window = window, p.n_tiles = n_tiles, p.status = status;
     p.scale_log2 = (float)(1.4426950408889634 / sqrt((double)hd));
     if (hd <= 64) return launch<64>(map_q, p, device, stream);

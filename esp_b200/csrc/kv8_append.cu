@@ -21,7 +21,7 @@ struct AppendParams {
     bf16* q_out;
     unsigned char *k_codes, *v_codes, *exps;
     const int* block_table;
-    int table_stride, n_pages, nh, nkv, hd, heads;      // heads: of a token's rows that the call writes (queries alone: nh)
+    int n_seqs, table_stride, n_pages, nh, nkv, hd, heads;      // heads: of a token's rows that the call writes (queries alone: nh)
     int* status;
 };
 
@@ -37,7 +37,7 @@ __device__ __forceinline__ Place find_place(const AppendParams& p, int n) {
     } else if (p.heads > p.nh) {
         const int seq = p.tok_seq[n];
         int page = -1;
-        if (at.pos / KV8_PAGE < p.table_stride && seq >= 0) page = p.block_table[(size_t)seq * p.table_stride + at.pos / KV8_PAGE];
+        if (at.pos / KV8_PAGE < p.table_stride && seq >= 0 && seq < p.n_seqs) page = p.block_table[(size_t)seq * p.table_stride + at.pos / KV8_PAGE];
         if (page >= 0 && page < p.n_pages) at.block = (long long)page * p.nkv;
     }
     return at;
@@ -183,13 +183,13 @@ __global__ void __launch_bounds__(256) kv8_append_kernel(AppendParams p) {
 // ``write_kv`` 0: queries alone.  Rows whose position has no table row or no page are skipped and the status says so.
 ESP_API int esp_kv8_append(const float* qkv, const float* bias, const int* tok_seq, const int* tok_pos, const float* cos_t,
                            const float* sin_t, int rot, int max_pos, void* q_out, void* k_codes, void* v_codes, void* exps,
-                           const int* block_table, int table_stride, int n_pages, int n_tokens, int nh, int nkv, int hd, int write_kv,
+                           const int* block_table, int n_seqs, int table_stride, int n_pages, int n_tokens, int nh, int nkv, int hd, int write_kv,
                            int* status, cudaStream_t stream) {
     if (n_tokens <= 0) return 0;
     if (rot < 0 || rot > hd || (rot & 1) || hd <= 0 || hd % 8 || hd > 256 || nh <= 0 || nkv <= 0 || nh + 2 * nkv > 65535) return (int)cudaErrorInvalidValue;
     const int heads = write_kv ? nh + 2 * nkv : nh;
     const AppendParams p{qkv, bias, tok_seq, tok_pos, cos_t, sin_t, rot, max_pos, (bf16*)q_out, (unsigned char*)k_codes, (unsigned char*)v_codes,
-                         (unsigned char*)exps, block_table, table_stride, n_pages, nh, nkv, hd, heads, status};
+                         (unsigned char*)exps, block_table, n_seqs, table_stride, n_pages, nh, nkv, hd, heads, status};
     if (rot % 8 == 0) {
         int group = 1;
         while (group * 8 < hd) group *= 2;

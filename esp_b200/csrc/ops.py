@@ -111,10 +111,10 @@ _SIGNATURES = {
                            c_float, c_int, c_float, c_float, c_float, P, c_longlong, P, P],
     "esp_attn_decode_diff": [P, P, P, P, P, P, P, P, P, P, P, c_int, c_int, c_int, c_int, c_int, c_int, c_int, c_int, c_int,
                              c_int, c_int, c_float, c_int, c_float, c_float, c_float, c_float, P, c_longlong, P, P],
-    "esp_kv8_append": [P, P, P, P, P, P, c_int, c_int, P, P, P, P, P, c_int, c_int, c_int, c_int, c_int, c_int, c_int, P, P],
-    "esp_attn_decode_kv8": [P, P, P, P, P, P, P, P, P, P, P, c_int, c_int, c_int, c_int, c_int, c_int, c_int, c_int, P, P],
-    "esp_attn_prefill_kv8": [P, c_longlong, P, P, P, P, P, P, P, P, P, c_int, c_int, c_int, c_int, c_int, c_int, c_int, P, P],
-    "esp_attn_run_kv8": [P, P, P, P, P, P, P, P, P, P, c_int, c_int, c_int, c_int, c_int, c_int, c_int, P, P],
+    "esp_kv8_append": [P, P, P, P, P, P, c_int, c_int, P, P, P, P, P, c_int, c_int, c_int, c_int, c_int, c_int, c_int, c_int, P, P],
+    "esp_attn_decode_kv8": [P, P, P, P, P, P, P, P, P, P, P, c_int, c_int, c_int, c_int, c_int, c_int, c_int, c_int, c_int, P, P],
+    "esp_attn_prefill_kv8": [P, c_longlong, P, P, P, P, P, P, P, P, P, c_int, c_int, c_int, c_int, c_int, c_int, c_int, c_int, P, P],
+    "esp_attn_run_kv8": [P, P, P, P, P, P, P, P, P, P, c_int, c_int, c_int, c_int, c_int, c_int, c_int, c_int, P, P],
 }
 
 _bound: dict = {}
@@ -1606,7 +1606,7 @@ def kv8_rope_append(qkv, bias, tok_seq, tok_pos, cos, sin, rot, q_out, k, v, exp
     if n == 0:
         return
     k_ = v_ = e_ = t_ = c_ = s_ = None
-    stride = n_pages = positions = 0
+    n_seqs = stride = n_pages = positions = 0
     fits = (_kv8_here(q_out) and q_out.numel() == n * nh * hd and tok_seq.numel() >= n <= tok_pos.numel() and (bias is None or bias.numel() == width)
             and (_kv8_pools_fit(k, v, exps, block_table, page, nh, nkv, hd) if write_kv else kv8_fits(hd, page) and nkv > 0 < nh))
     if fits:
@@ -1615,7 +1615,8 @@ def kv8_rope_append(qkv, bias, tok_seq, tok_pos, cos, sin, rot, q_out, k, v, exp
             c_, s_, positions = _ptr(cos, _F32, "cos"), _ptr(sin, _F32, "sin"), cos.shape[0]
         if write_kv:
             k_, v_, e_, t_ = _ptr(k, _E4M3, "keys"), _ptr(v, _E4M3, "values"), _ptr(exps, torch.uint8, "exponents"), _ptr(block_table, torch.int32, "page table")
-            stride, n_pages = block_table.shape[1], k.shape[0]
+            n_seqs, stride = block_table.shape
+            n_pages = k.shape[0]
         fits = not (x_ | q_ | (b_ or 0) | (c_ or 0) | (s_ or 0) | (k_ or 0) | (v_ or 0) | (e_ or 0)) & 15
     if not fits:
         _kv8_refuse("kv8_rope_append", q_out, k if write_kv else None, v, exps, block_table, page, nh, nkv, hd,
@@ -1624,8 +1625,8 @@ def kv8_rope_append(qkv, bias, tok_seq, tok_pos, cos, sin, rot, q_out, k, v, exp
                      ("the queries", q_out), ("the keys", k if write_kv else None), ("the values", v if write_kv else None),
                      ("the exponents", exps if write_kv else None)))
     _check(_fn("kv8", "esp_kv8_append")(
-        x_, b_, _ptr(tok_seq, torch.int32, "tok_seq"), _ptr(tok_pos, torch.int32, "tok_pos"), c_, s_, rot, positions, q_, k_, v_, e_, t_, stride,
-        n_pages, n, nh, nkv, hd, 1 if write_kv else 0, _ptr(status, torch.int32, "status"), _stream()), "kv8_rope_append")
+        x_, b_, _ptr(tok_seq, torch.int32, "tok_seq"), _ptr(tok_pos, torch.int32, "tok_pos"), c_, s_, rot, positions, q_, k_, v_, e_, t_, n_seqs,
+        stride, n_pages, n, nh, nkv, hd, 1 if write_kv else 0, _ptr(status, torch.int32, "status"), _stream()), "kv8_rope_append")
 
 
 @functools.lru_cache(maxsize=64)
@@ -1661,13 +1662,13 @@ def attn_decode_kv8(q, k, v, exps, out, ws, tok_seq, tok_pos, block_table, page,
         _kv8_refuse("attn_decode_kv8", q, k, v, exps, block_table, page, nh, nkv, hd,
                     (("tok_seq", tok_seq, n), ("tok_pos", tok_pos, n), ("seq_past", seq_past, block_table.shape[0])),
                     (("the queries", q), ("the keys", k), ("the values", v), ("the exponents", exps), ("the results", out)))
-    stride = block_table.shape[1]
+    n_seqs, stride = block_table.shape
     blocks = ATTN_DECODE_KV8_BLOCKS_PER_SM[64 if hd <= 64 else 128 if hd <= 128 else 256] * _sm_count(_device_index)
     parts = _ptr(ws.get("attn_kv8_parts", (blocks * 32, hd + 2), _F32))
     counters = _ptr(ws.get("attn_kv8_counters", (min(n, 1024) * nh + 2 * blocks,), torch.int32, zeroed=True))
     _check(_fn("kv8", "esp_attn_decode_kv8")(
         q_, k_, v_, e_, o_, parts, counters, _ptr(tok_seq, torch.int32, "tok_seq"), _ptr(tok_pos, torch.int32, "tok_pos"),
-        _ptr(seq_past, torch.int32, "seq_past"), _ptr(block_table, torch.int32, "page table"), stride, k.shape[0], n, nh, nkv, hd, int(window or 0),
+        _ptr(seq_past, torch.int32, "seq_past"), _ptr(block_table, torch.int32, "page table"), n_seqs, stride, k.shape[0], n, nh, nkv, hd, int(window or 0),
         blocks, _ptr(status, torch.int32, "status"), _stream()), "attn_decode_kv8")
 
 
@@ -1696,7 +1697,7 @@ def attn_prefill_kv8(q, k, v, exps, out, tile_seq, tile_first, seq_start, seq_pa
                     (("the queries", q), ("the keys", k), ("the values", v), ("the exponents", exps), ("the results", out)))
     rest = (k_, v_, e_, o_, _ptr(tile_seq, torch.int32, "tile_seq"), _ptr(tile_first, torch.int32, "tile_first"),
             _ptr(seq_start, torch.int32, "seq_start"), _ptr(seq_past, torch.int32, "seq_past"), _ptr(block_table, torch.int32, "page table"),
-            block_table.shape[1], k.shape[0], n_tiles, nh, nkv, hd, int(window or 0), _ptr(status, torch.int32, "status"), _stream())
+            *block_table.shape, k.shape[0], n_tiles, nh, nkv, hd, int(window or 0), _ptr(status, torch.int32, "status"), _stream())
     if hd <= 128:                      # scores and weighted values in tensor memory
         _check(_fn("kv8", "esp_attn_prefill_kv8")(q_, n, *rest), "attn_prefill_kv8")
     else:                              # the streaming kernel, sixteen rows a block

@@ -172,6 +172,9 @@ def test_append_of_queries_alone_and_bad_places():
     ops.kv8_rope_append(qkv, None, seq, pos, cos, sin, hd, q, None, None, None, None, PAGE, nh, nkv, hd, False, st)
     assert st.item() == 0
     assert torch.equal(q, qkv[:, :nh * hd].to(torch.bfloat16))
+    # sequence 2 is not in the table
+    ops.kv8_rope_append(qkv[:1], None, ints([2]), ints([1]), cos, sin, hd, q[:1], k, v, exps, ints([[0], [1]]), PAGE, nh, nkv, hd, True, st)
+    assert st.item() == BAD_INDEX and (exps == 255).all()
     # page 7 and page -1 are not there, position 200 has no angle, position 130 no entry of the table, -1 is no position
     table = ints([[2, 0], [7, -1]])
     for where in ([3, 0, 2, 2, 2], [3, 70, 0, 100, 2]):
@@ -336,7 +339,7 @@ def test_decode_with_pages_that_are_none():
     assert (got[2] == 0).all()                        # not one page: no keys
     st.zero_()
     got.fill_(7)
-    ops.attn_decode_kv8(q, k, v, exps, got, ws, ints([0, 1, -1, 3]), ints([299, -1, 63, 99 + 64 * table.shape[1]]), table, PAGE, nh, nkv, hd, 0, st)
+    ops.attn_decode_kv8(q, k, v, exps, got, ws, ints([0, 1, [-1, 4][hd > 64], 3]), ints([299, -1, 63, 99 + 64 * table.shape[1]]), table, PAGE, nh, nkv, hd, 0, st)
     assert st.item() == BAD_INDEX and torch.equal(got[0], out[0]) and (got[1:] == 7).all()
 
 
@@ -470,7 +473,83 @@ def test_prefill_with_pages_that_are_none(hd):
     assert torch.equal(got[:150], out[:150]) and torch.isfinite(got).all()
 
 
+def test_prefill_tiles_that_are_none():
+    for hd in (128, 192):
+        nh, nkv, news, pasts = 2, 1, [150, 140], [100, 30]
+        table, k, v, exps, q, starts, tile_seq, tile_first = prefill_inputs(nh, nkv, hd, news, pasts, 8)
+        out, st = torch.empty_like(q), status()
+        ops.attn_prefill_kv8(q, k, v, exps, out, tile_seq, tile_first, ints(starts), ints(pasts), table, PAGE, nh, nkv, hd, 0, st)
+        got = torch.full_like(q, 7)
+        bad_seq, bad_first = torch.cat((tile_seq, ints([2, -1, 0]))), torch.cat((tile_first, ints([0, 0, -128])))
+        ops.attn_prefill_kv8(q, k, v, exps, got, bad_seq, bad_first, ints(starts), ints(pasts), table, PAGE, nh, nkv, hd, 0, st)
+        assert st.item() == BAD_INDEX and torch.equal(got, out)
+        # positions that the table does not have: the sequence is left out, the other is not
+        got.fill_(7)
+        st.zero_()
+        ops.attn_prefill_kv8(q, k, v, exps, got, tile_seq, tile_first, ints(starts), ints([64 * table.shape[1], 30]), table, PAGE, nh, nkv, hd, 0, st)
+        assert st.item() == BAD_INDEX and torch.equal(got[150:], out[150:]) and (got[:128] == 7).all()
+
+
+@pytest.mark.parametrize("nh,hd", [(1, 64), (3, 128)])
+def test_prefill_of_more_tiles_than_a_launch_lists(nh, hd):
+    """5,000 sequences of one token: a row sees its own position alone, so the result is its value."""
+    n = 5000
+    k, v, exps = pools(n, 1, hd, 4)
+    q = torch.randn((n, nh * hd), generator=gen(1), device="cuda").to(torch.bfloat16)
+    order = torch.randperm(n, generator=torch.Generator().manual_seed(1)).to(torch.int32).cuda()
+    out, st, seq = torch.full_like(q, math.nan), status(), torch.arange(n, dtype=torch.int32, device="cuda")
+    ops.attn_prefill_kv8(q, k, v, exps, out, seq, ints([0] * n), torch.arange(n + 1, dtype=torch.int32, device="cuda"), ints([0] * n), order[:, None].contiguous(),
+                         PAGE, nh, 1, hd, 0, st)
+    want = plain.stored(v[order.long(), 0, 0], exps[order.long(), 0, 1, 0])
+    assert st.item() == 0
+    assert torch.equal(out.view(n, nh, hd).double(), want[:, None].expand(n, nh, hd))
+
+
 # ------------------------------------------------------------------------------------------------------- together
+def test_pools_past_32_bits_of_bytes():
+    """Pages whose codes lie more than 2^31 bytes into the pool."""
+    nh, nkv, hd, pages = 4, 4, 256, 34000
+    k, v = (torch.empty((pages, nkv, PAGE, hd), dtype=E4M3, device="cuda") for _ in range(2))
+    exps = torch.zeros((pages, nkv, 2, PAGE), dtype=torch.uint8, device="cuda")
+    assert k.numel() > 1 << 31
+    for hd_now in (256, 128):
+        kk, vv = k.view(-1, nkv, PAGE, hd_now)[:2 * pages if hd_now == 128 else pages], v.view(-1, nkv, PAGE, hd_now)
+        ee = exps if hd_now == 256 else torch.zeros((2 * pages, nkv, 2, PAGE), dtype=torch.uint8, device="cuda")
+        last = kk.shape[0]
+        table = ints([[last - 1, last - 3, last - 2, -1]])
+        n, length = 150, 150
+        qkv = torch.randn((n, 3 * nh * hd_now), generator=gen(2), device="cuda")
+        q, st = torch.empty((n, nh * hd_now), dtype=torch.bfloat16, device="cuda"), status()
+        seq, pos = ints([0] * n), torch.arange(n, dtype=torch.int32, device="cuda")
+        ops.kv8_rope_append(qkv, None, seq, pos, None, None, 0, q, kk, vv, ee, table, PAGE, nh, nkv, hd_now, True, st)
+        out, one = torch.empty_like(q), torch.empty_like(q[:1])
+        ops.attn_prefill_kv8(q, kk, vv, ee, out, ints([0, 0]), ints([128, 0]), ints([0, n]), ints([0]), table, PAGE, nh, nkv, hd_now, 0, st)
+        ops.attn_decode_kv8(q[-1:], kk, vv, ee, one, Workspace(q.device), ints([0]), ints([n - 1]), table, PAGE, nh, nkv, hd_now, 0, st)
+        assert st.item() == 0
+        check_prefill(out, q, kk, vv, ee, table, [0, n], [0], nh, hd_now, 0)
+        check_decode(one, q[-1:], kk, vv, ee, table, [length], nh, hd_now, 0)
+
+
+def test_calls_on_two_streams_with_a_workspace_each():
+    """Decode and prefill of two steps at once: nothing is shared but the pools."""
+    nh, nkv, hd, lengths = 8, 2, 128, [3000, 700, 1500]
+    table, k, v, exps, q, seq, pos = decode_inputs(nh, nkv, hd, lengths, 4)
+    want, st = torch.empty_like(q), status()
+    ops.attn_decode_kv8(q, k, v, exps, want, Workspace(q.device), seq, pos, table, PAGE, nh, nkv, hd, 0, st)
+    torch.cuda.synchronize()
+    streams, outs, spaces = [torch.cuda.Stream() for _ in range(2)], [torch.empty_like(q) for _ in range(2)], [Workspace(q.device) for _ in range(2)]
+    for stream, ws in zip(streams, spaces):               # the scratch is made on the stream that uses it
+        with torch.cuda.stream(stream):
+            ops.attn_decode_kv8(q, k, v, exps, outs[0], ws, seq, pos, table, PAGE, nh, nkv, hd, 0, st)
+    torch.cuda.synchronize()
+    for _ in range(20):
+        for stream, out, ws in zip(streams, outs, spaces):
+            with torch.cuda.stream(stream):
+                ops.attn_decode_kv8(q, k, v, exps, out, ws, seq, pos, table, PAGE, nh, nkv, hd, 0, st)
+    torch.cuda.synchronize()
+    assert st.item() == 0 and torch.equal(outs[0], want) and torch.equal(outs[1], want)
+
+
 def test_append_then_attend_is_a_captured_step():
     """A step as it is used, append then decode, on a stream of its own and replayed from a graph over changing inputs."""
     nh, nkv, hd, lengths = 8, 2, 128, [130, 700]
