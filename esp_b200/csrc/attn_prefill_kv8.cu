@@ -735,13 +735,14 @@ template <int HD> int launch(const CUtensorMap& map_q, Params p, int device, cud
         raised[device] = true;
     }
     p.smem_bytes = (int)smem;
+    // Pairs halve the conversions and the number of items: not where the device would not be filled by them.  One rule for all
+    // launches, as a tile is left to its neighbour, which another launch may list.
+    p.pair = (long long)p.n_tiles * p.nh >= 4LL * sm_count[device];
     for (int at = 0; at < p.n_tiles; at += LIST) {
         Params q = p;
         q.tile_seq += at, q.tile_first += at;
         q.n_tiles = p.n_tiles - at < LIST ? p.n_tiles - at : LIST;
         const long long items = (long long)q.n_tiles * p.nh;
-        // pairs halve the conversions and the number of items: not where the device would not be filled by them
-        q.pair = items >= 4LL * sm_count[device];
         const unsigned grid = (unsigned)(items < sm_count[device] ? items : sm_count[device]);
         esp_launch_pdl(ESP_PDL_MANY_ROWS, attn_prefill_kv8_kernel<HD>, dim3(grid), dim3(THREADS), smem, stream, map_q, q);
         const int rc = esp_launch_status();

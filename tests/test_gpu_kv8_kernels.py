@@ -505,6 +505,19 @@ def test_prefill_of_more_tiles_than_a_launch_lists(nh, hd):
     assert torch.equal(out.view(n, nh, hd).double(), want[:, None].expand(n, nh, hd))
 
 
+def test_prefill_of_two_tiles_that_different_launches_list():
+    """The second of a sequence's two tiles heads a list of 4,098, the first ends it."""
+    nh, nkv, hd = 2, 1, 128
+    news = [200] + [1] * 4096
+    pasts = [0] * len(news)
+    table, k, v, exps, q, starts, _, _ = prefill_inputs(nh, nkv, hd, news, pasts, 9)
+    tile_seq, tile_first = ints([0, *range(1, 4097), 0]), ints([128, *[0] * 4096, 0])
+    out, st = torch.full_like(q, math.nan), status()
+    ops.attn_prefill_kv8(q, k, v, exps, out, tile_seq, tile_first, ints(starts), ints(pasts), table, PAGE, nh, nkv, hd, 0, st)
+    assert st.item() == 0 and torch.isfinite(out).all()
+    check_prefill(out[:200], q, k, v, exps, table, starts[:2], pasts[:1], nh, hd, 0)
+
+
 # ------------------------------------------------------------------------------------------------------- together
 def test_pools_past_32_bits_of_bytes():
     """Pages whose codes lie more than 2^31 bytes into the pool."""
