@@ -46,7 +46,7 @@ struct Params {
     const int *seq_past, *seq_start;           // per sequence (decode: seq_past may be null)
     const int *tile_seq, *tile_first;          // run: tiles of 128 new tokens
     const int* block_table;
-    int n_seqs, table_stride, n_pages, n_rows, nh, nkv, hd, window;      // n_seqs: rows of the page table
+    int n_seqs, table_stride, n_pages, n_rows, nh, nkv, hd, window;      // n_seqs: rows of the page table; n_rows: of the queries
     float scale_log2;                          // log2(e) / sqrt(hd)
     int* status;
 };
@@ -364,10 +364,11 @@ __global__ void __launch_bounds__(THREADS) attn_run_kv8_kernel(const Params p) {
         if (threadIdx.x == 0) atomicOr(p.status, ESP_STATUS_BAD_INDEX);
         return;
     }
-    const int start = p.seq_start[seq], rows = min(S::ROWS, p.seq_start[seq + 1] - start - first), head = blockIdx.y, kvh = head / (p.nh / p.nkv);
+    const int start = p.seq_start[seq], end = p.seq_start[seq + 1], rows = min(S::ROWS, end - start - first), head = blockIdx.y, kvh = head / (p.nh / p.nkv);
     if (rows <= 0) return;
-    const int pos0 = p.seq_past[seq] + first, k0 = first_visible_key(pos0, p.window, 0), k1 = pos0 + rows - 1;
-    if (pos0 < 0 || k1 / KV8_PAGE >= p.table_stride) {
+    const int past = p.seq_past[seq], pos0 = past + first, k0 = first_visible_key(pos0, p.window, 0), k1 = pos0 + rows - 1;
+    // rows that the queries do not have, or positions that the page table does not have
+    if (start < 0 || end > p.n_rows || past < 0 || ((long long)past + first + rows - 1) / KV8_PAGE >= p.table_stride) {
         if (threadIdx.x == 0) atomicOr(p.status, ESP_STATUS_BAD_INDEX);
         return;
     }
@@ -733,13 +734,13 @@ ESP_API int esp_attn_decode_kv8(const void* q, const void* k, const void* v, con
 
 // Runs of new tokens: tiles of 128 of a sequence (sequence, its first token among the sequence's new ones).  For heads of more
 // than 128 channels (esp_attn_prefill_kv8 has the others).
-ESP_API int esp_attn_run_kv8(const void* q, const void* k, const void* v, const void* exps, void* out, const int* tile_seq,
+ESP_API int esp_attn_run_kv8(const void* q, long long n_tokens, const void* k, const void* v, const void* exps, void* out, const int* tile_seq,
                              const int* tile_first, const int* seq_start, const int* seq_past, const int* block_table, int n_seqs, int table_stride,
                              int n_pages, int n_tiles, int nh, int nkv, int hd, int window, int* status, cudaStream_t stream) {
     if (n_tiles <= 0) return 0;
-    if (!sizes_fit(nh, nkv, hd) || hd <= 128 || window < 0 || n_tiles > (1 << 26)) return (int)cudaErrorInvalidValue;
+    if (!sizes_fit(nh, nkv, hd) || hd <= 128 || window < 0 || n_tiles > (1 << 26) || n_tokens > 0x7fffffffLL) return (int)cudaErrorInvalidValue;
     Params p = make_params(q, k, v, exps, out, block_table, n_seqs, table_stride, n_pages, nh, nkv, hd, window, status);
-    p.tile_seq = tile_seq, p.tile_first = tile_first, p.seq_start = seq_start, p.seq_past = seq_past;
+    p.n_rows = (int)n_tokens, p.tile_seq = tile_seq, p.tile_first = tile_first, p.seq_start = seq_start, p.seq_past = seq_past;
     static bool raised[64] = {false};
     return launch(attn_run_kv8_kernel<256, 2>, (size_t)WARPS * Ring<256>::WARP, raised, p, dim3((unsigned)n_tiles * 8u, p.nh), stream);
 }

@@ -47,7 +47,7 @@ struct Params {
     const unsigned char *k, *v, *exps;
     bf16* out;
     const int *tile_seq, *tile_first, *seq_start, *seq_past, *block_table;
-    int n_seqs, table_stride, n_pages, nh, nkv, hd, window, n_tiles, pair, smem_bytes;
+    int n_seqs, table_stride, n_pages, nh, nkv, hd, window, n_tiles, pair, smem_bytes, n_tokens;
     float scale_log2;
     int* status;
 };
@@ -245,12 +245,14 @@ __global__ void __launch_bounds__(THREADS, 1) attn_prefill_kv8_kernel(const __gr
             const int i = i0 + lane;
             bool live = i < p.n_tiles;
             if (live) {
-                // a tile of a sequence that is not there, without rows, or with positions that the page table does not have is left out
+                // a tile of a sequence that is not there, without rows or with rows that the queries do not have, or with positions that the
+            // page table does not have is left out
                 const int seq = p.tile_seq[i], first = p.tile_first[i];
                 bool fine = seq >= 0 && seq < p.n_seqs && first >= 0;
                 if (fine) {
-                    const int news = p.seq_start[seq + 1] - p.seq_start[seq], past = p.seq_past[seq];
-                    fine = first < news && past >= 0 && (past + news - 1) / KV8_PAGE < p.table_stride;
+                    const int start = p.seq_start[seq], end = p.seq_start[seq + 1], past = p.seq_past[seq];
+                    fine = start >= 0 && end <= p.n_tokens && first < end - start && past >= 0 &&
+                           ((long long)past + (end - start) - 1) / KV8_PAGE < p.table_stride;
                 }
                 if (!fine && blockIdx.x == 0) atomicOr(p.status, ESP_STATUS_BAD_INDEX);
                 live = fine && (!p.pair || (first / BM) % 2 == 0);
@@ -758,7 +760,7 @@ ESP_API int esp_attn_prefill_kv8(const void* q, long long n_tokens, const void* 
                                  const int* tile_first, const int* seq_start, const int* seq_past, const int* block_table, int n_seqs, int table_stride,
                                  int n_pages, int n_tiles, int nh, int nkv, int hd, int window, int* status, cudaStream_t stream) {
     if (n_tiles <= 0 || n_tokens <= 0) return 0;
-    if (nkv <= 0 || nh <= 0 || nh % nkv || nh > 65535 || hd <= 0 || hd % 8 || hd > 128 || window < 0 || (long long)n_tiles * nh > 0x7fffffffLL)
+    if (nkv <= 0 || nh <= 0 || nh % nkv || nh > 65535 || hd <= 0 || hd % 8 || hd > 128 || window < 0 || (long long)n_tiles * nh > 0x7fffffffLL || n_tokens > 0x7fffffffLL)
         return (int)cudaErrorInvalidValue;
     int device = 0;
     if (cudaGetDevice(&device) != cudaSuccess || device < 0 || device >= 64) return (int)cudaErrorInvalidDevice;
@@ -769,6 +771,7 @@ ESP_API int esp_attn_prefill_kv8(const void* q, long long n_tokens, const void* 
     p.k = (const unsigned char*)k, p.v = (const unsigned char*)v, p.exps = (const unsigned char*)exps, p.out = (bf16*)out;
     p.tile_seq = tile_seq, p.tile_first = tile_first, p.seq_start = seq_start, p.seq_past = seq_past, p.block_table = block_table, p.n_seqs = n_seqs;
     p.table_stride = table_stride, p.n_pages = n_pages, p.nh = nh, p.nkv = nkv, p.hd = hd, p.window = window, p.n_tiles = n_tiles, p.status = status;
+    p.n_tokens = (int)n_tokens;
     p.scale_log2 = (float)(1.4426950408889634 / sqrt((double)hd));
     if (hd <= 64) return launch<64>(map_q, p, device, stream);
     return launch<128>(map_q, p, device, stream);

@@ -114,7 +114,7 @@ _SIGNATURES = {
     "esp_kv8_append": [P, P, P, P, P, P, c_int, c_int, P, P, P, P, P, c_int, c_int, c_int, c_int, c_int, c_int, c_int, c_int, P, P],
     "esp_attn_decode_kv8": [P, P, P, P, P, P, P, P, P, P, P, c_int, c_int, c_int, c_int, c_int, c_int, c_int, c_int, c_int, P, P],
     "esp_attn_prefill_kv8": [P, c_longlong, P, P, P, P, P, P, P, P, P, c_int, c_int, c_int, c_int, c_int, c_int, c_int, c_int, P, P],
-    "esp_attn_run_kv8": [P, P, P, P, P, P, P, P, P, P, c_int, c_int, c_int, c_int, c_int, c_int, c_int, c_int, P, P],
+    "esp_attn_run_kv8": [P, c_longlong, P, P, P, P, P, P, P, P, P, c_int, c_int, c_int, c_int, c_int, c_int, c_int, c_int, P, P],
 }
 
 _bound: dict = {}
@@ -1701,4 +1701,4 @@ def attn_prefill_kv8(q, k, v, exps, out, tile_seq, tile_first, seq_start, seq_pa
     if hd <= 128:                      # scores and weighted values in tensor memory
         _check(_fn("kv8", "esp_attn_prefill_kv8")(q_, n, *rest), "attn_prefill_kv8")
     else:                              # the streaming kernel, sixteen rows a block
-        _check(_fn("kv8", "esp_attn_run_kv8")(q_, *rest), "attn_prefill_kv8")
+        _check(_fn("kv8", "esp_attn_run_kv8")(q_, n, *rest), "attn_prefill_kv8")

@@ -490,6 +490,23 @@ def test_prefill_tiles_that_are_none():
         assert st.item() == BAD_INDEX and torch.equal(got[150:], out[150:]) and (got[:128] == 7).all()
 
 
+@pytest.mark.parametrize("hd", [64, 128, 192])
+@pytest.mark.parametrize("starts", [[0, 150, 291], [0, 150, 2 ** 31 - 1], [0, -5, 140], [-20, 150, 290]])
+def test_prefill_rows_that_are_none(hd, starts):
+    """Sequences whose rows the queries do not have are left out."""
+    nh, nkv, news, pasts = 2, 1, [150, 140], [100, 30]
+    table, k, v, exps, q, good, tile_seq, tile_first = prefill_inputs(nh, nkv, hd, news, pasts, 8)
+    out, got, st = torch.empty_like(q), torch.full_like(q, 7), status()
+    ops.attn_prefill_kv8(q, k, v, exps, out, tile_seq, tile_first, ints(good), ints(pasts), table, PAGE, nh, nkv, hd, 0, st)
+    assert st.item() == 0
+    ops.attn_prefill_kv8(q, k, v, exps, got, tile_seq, tile_first, ints(starts), ints(pasts), table, PAGE, nh, nkv, hd, 0, st)
+    assert st.item() == BAD_INDEX
+    for i in range(2):
+        fine = 0 <= starts[i] < starts[i + 1] <= 290
+        rows = slice(good[i], good[i + 1])
+        assert torch.equal(got[rows], out[rows] if fine else torch.full_like(out[rows], 7))
+
+
 @pytest.mark.parametrize("nh,hd", [(1, 64), (3, 128)])
 def test_prefill_of_more_tiles_than_a_launch_lists(nh, hd):
     """5,000 sequences of one token: a row sees its own position alone, so the result is its value."""
