@@ -169,7 +169,7 @@ template <int HD, int NT, bool RUN> struct Stream {
             amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
             amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
             const int x = max((int)(__float_as_uint(amax) >> 23) - 127, -100);       // the largest lies in [2^x, 2^(x+1))
-            const float f = kv8_pow2(14 - x);
+            const float f = x > 127 ? __int_as_float(0x7fffffff) : kv8_pow2(14 - x);    // an infinite query is no number: 0 / 0 or inf / inf
 #pragma unroll
             for (int kk = 0; kk < HD / 16; kk++) {
                 const float2 a = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&raw[nt][kk].x)), b = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&raw[nt][kk].y));

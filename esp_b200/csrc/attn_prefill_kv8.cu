@@ -663,7 +663,7 @@ __global__ void __launch_bounds__(THREADS, 1) attn_prefill_kv8_kernel(const __gr
             const float f0 = m0 == -INFINITY ? 0.f : fast_exp2(m0 - m_all), f1 = m1 == -INFINITY ? 0.f : fast_exp2(m1 - m_all);
             float l = f0 * (xsum[g0 * 256 + r] + xsum[g0 * 256 + 128 + r]);
             if (both) l += f1 * (xsum[256 + r] + xsum[384 + r]);
-            const float inv = l == 0.f ? 0.f : 1.f / l;
+            const float inv = 1.f / l;                               // 0 where all scores are -inf (an infinite query): 0 * inf is NaN
             const int cols = t.pair ? HD / 2 : HD / 4, col0 = (t.pair ? side : grp * 2 + side) * cols;   // what this thread writes
             const unsigned from = t.pair ? o_addr : tm_o + lane_sel;
 #pragma unroll 1

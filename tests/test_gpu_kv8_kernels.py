@@ -535,6 +535,28 @@ def test_prefill_of_two_tiles_that_different_launches_list():
     check_prefill(out[:200], q, k, v, exps, table, starts[:2], pasts[:1], nh, hd, 0)
 
 
+@pytest.mark.parametrize("hd", [64, 128, 256])
+@pytest.mark.parametrize("value", [math.inf, -math.inf, math.nan])
+def test_queries_that_are_no_numbers(hd, value):
+    """A row whose query holds an infinity or a NaN is NaN, be its scores all the lowest or not; the others are not touched."""
+    nh, nkv, news, pasts = 2, 1, [300], [40]
+    table, k, v, exps, q, starts, tile_seq, tile_first = prefill_inputs(nh, nkv, hd, news, pasts, 6)
+    k = k.view(torch.uint8).clone()
+    k[..., 5] = 0x38                                       # 1: the query's infinity is every score's
+    k = k.view(E4M3)
+    rows, st = torch.tensor([0, 130, 299], device="cuda"), status()
+    want, got, bad = torch.empty_like(q), torch.empty_like(q), q.clone()
+    bad.view(-1, nh, hd)[rows, 1, 5] = value
+    for qq, out in ((q, want), (bad, got)):
+        ops.attn_prefill_kv8(qq, k, v, exps, out, tile_seq, tile_first, ints(starts), ints(pasts), table, PAGE, nh, nkv, hd, 0, st)
+    hit = torch.zeros((300, nh), dtype=torch.bool, device="cuda")
+    hit[rows, 1] = True
+    assert torch.isnan(got.view(-1, nh, hd)[hit]).all() and torch.equal(got.view(-1, nh, hd)[~hit], want.view(-1, nh, hd)[~hit])
+    one, ws = torch.empty_like(q[rows]), Workspace(q.device)
+    ops.attn_decode_kv8(bad[rows], k, v, exps, one, ws, ints([0, 0, 0]), ints([40, 170, 339]), table, PAGE, nh, nkv, hd, 0, st)
+    assert st.item() == 0 and torch.isnan(one.view(3, nh, hd)[:, 1]).all() and torch.isfinite(one.view(3, nh, hd)[:, 0]).all()
+
+
 # ------------------------------------------------------------------------------------------------------- together
 def test_pools_past_32_bits_of_bytes():
     """Pages whose codes lie more than 2^31 bytes into the pool."""
