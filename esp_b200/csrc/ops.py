@@ -1578,6 +1578,11 @@ def _kv8_pools_fit(k, v, exps, block_table, page, nh, nkv, hd) -> bool:
             and block_table.dim() == 2)
 
 
+def _kv8_window(window, block_table, page) -> int:
+    """0 (all keys) for a window that no position of the table reaches beyond; such a number may not fit an int."""
+    return window if window and window < block_table.shape[1] * page else 0
+
+
 def _kv8_here(q) -> bool:
     """Whether a tensor lives on the device that launches go to."""
     if not q.is_cuda:
@@ -1668,7 +1673,7 @@ def attn_decode_kv8(q, k, v, exps, out, ws, tok_seq, tok_pos, block_table, page,
     counters = _ptr(ws.get("attn_kv8_counters", (min(n, 1024) * nh + 2 * blocks,), torch.int32, zeroed=True))
     _check(_fn("kv8", "esp_attn_decode_kv8")(
         q_, k_, v_, e_, o_, parts, counters, _ptr(tok_seq, torch.int32, "tok_seq"), _ptr(tok_pos, torch.int32, "tok_pos"),
-        _ptr(seq_past, torch.int32, "seq_past"), _ptr(block_table, torch.int32, "page table"), n_seqs, stride, k.shape[0], n, nh, nkv, hd, int(window or 0),
+        _ptr(seq_past, torch.int32, "seq_past"), _ptr(block_table, torch.int32, "page table"), n_seqs, stride, k.shape[0], n, nh, nkv, hd, _kv8_window(window, block_table, page),
         blocks, _ptr(status, torch.int32, "status"), _stream()), "attn_decode_kv8")
 
 
@@ -1697,7 +1702,7 @@ def attn_prefill_kv8(q, k, v, exps, out, tile_seq, tile_first, seq_start, seq_pa
                     (("the queries", q), ("the keys", k), ("the values", v), ("the exponents", exps), ("the results", out)))
     rest = (k_, v_, e_, o_, _ptr(tile_seq, torch.int32, "tile_seq"), _ptr(tile_first, torch.int32, "tile_first"),
             _ptr(seq_start, torch.int32, "seq_start"), _ptr(seq_past, torch.int32, "seq_past"), _ptr(block_table, torch.int32, "page table"),
-            *block_table.shape, k.shape[0], n_tiles, nh, nkv, hd, int(window or 0), _ptr(status, torch.int32, "status"), _stream())
+            *block_table.shape, k.shape[0], n_tiles, nh, nkv, hd, _kv8_window(window, block_table, page), _ptr(status, torch.int32, "status"), _stream())
     if hd <= 128:                      # scores and weighted values in tensor memory
         _check(_fn("kv8", "esp_attn_prefill_kv8")(q_, n, *rest), "attn_prefill_kv8")
     else:                              # the streaming kernel, sixteen rows a block

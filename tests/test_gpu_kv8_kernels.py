@@ -536,6 +536,20 @@ def test_prefill_of_two_tiles_that_different_launches_list():
 
 
 @pytest.mark.parametrize("hd", [64, 128, 256])
+def test_windows_beyond_all_positions(hd):
+    """A window that reaches past the first position hides nothing, whatever its size."""
+    nh, nkv, news, pasts = 2, 1, [140], [100]
+    table, k, v, exps, q, starts, tile_seq, tile_first = prefill_inputs(nh, nkv, hd, news, pasts, 6)
+    outs, ones, st, ws = [], [], status(), Workspace(q.device)
+    for window in (None, 240, 2 ** 31 - 1, 2 ** 31, 2 ** 32 + 5):
+        outs.append(torch.empty_like(q))
+        ops.attn_prefill_kv8(q, k, v, exps, outs[-1], tile_seq, tile_first, ints(starts), ints(pasts), table, PAGE, nh, nkv, hd, window, st)
+        ones.append(torch.empty_like(q[:1]))
+        ops.attn_decode_kv8(q[-1:], k, v, exps, ones[-1], ws, ints([0]), ints([239]), table, PAGE, nh, nkv, hd, window, st)
+    assert st.item() == 0 and all(torch.equal(outs[0], x) for x in outs) and all(torch.equal(ones[0], x) for x in ones)
+
+
+@pytest.mark.parametrize("hd", [64, 128, 256])
 @pytest.mark.parametrize("value", [math.inf, -math.inf, math.nan])
 def test_queries_that_are_no_numbers(hd, value):
     """A row whose query holds an infinity or a NaN is NaN, be its scores all the lowest or not; the others are not touched."""
