@@ -471,7 +471,10 @@ __global__ void __launch_bounds__(THREADS) attn_decode_kv8_kernel(const Params p
     __syncthreads();
     const long long total = (long long)carry * kv_blocks;
     const int blocks = (int)min((long long)gridDim.x, total);            // that have units: each of them one at least
-    if ((int)blockIdx.x >= blocks) return;
+    if ((int)blockIdx.x >= blocks) {
+        pdl_wait();                            // a grid without units ends behind the kernel before it, too
+        return;
+    }
     const long long u0 = total * blockIdx.x / blocks, u1 = total * (blockIdx.x + 1) / blocks;
 
     // ---- cursors through the stream: pairs row by row, of a row its blocks of heads one behind the other
