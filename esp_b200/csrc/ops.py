@@ -1647,7 +1647,9 @@ def attn_decode_kv8(q, k, v, exps, out, ws, tok_seq, tok_pos, block_table, page,
     """Attention of one token row per sequence (or of any rows, each on its own) over the 8-bit cache, the keys of all rows
     dealt out evenly over the device: scores over sqrt(hd), keys max(0, pos - window + 1) .. pos (``window`` None or 0: all).  q and out bfloat16 [N, nh * hd];
     query head i reads key/value head i // (nh / nkv).  ``ws``: the ``Workspace`` that holds the scratch; calls that may
-    overlap on the device (other streams, captured graphs replayed beside each other) need one each.  ``seq_past``
+    overlap on the device (other streams, captured graphs replayed beside each other) need one each.  A call that is to be
+    captured is made once before, and its graph holds ``ws``'s buffers: capture again once ``ws.generation`` has moved on, or
+    set ``ws.frozen``.  ``seq_past``
     (int32 per sequence of the step: positions that were cached before the step's copies to the device): blocks whose
     keys are all older load them without waiting for the kernel before this one."""
     n = q.shape[0]

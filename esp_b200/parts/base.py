@@ -162,7 +162,8 @@ class Workspace:
         self.generation = 0          # bumped whenever a buffer moves; captured graphs check it
 
     def get(self, name: str, shape: tuple, dtype, zeroed: bool = False) -> torch.Tensor:
-        """``zeroed``: a new buffer holds zeros (counters that every kernel leaves at zero)."""
+        """``zeroed``: a new buffer holds zeros (counters that every kernel leaves at zero).  Such a buffer is not made while a
+        graph is captured: its zeros would come with the graph's first replay, and a call before that would not find them."""
         seen = self._views.get((name, dtype, shape))
         if seen is not None:
             return seen
@@ -174,6 +175,8 @@ class Workspace:
         if buf is None or buf.numel() < count:
             if self.frozen:
                 raise Backend(f"workspace buffer {name} would have to grow while a captured graph holds it")
+            if zeroed and torch.device(self.device).type == "cuda" and torch.cuda.is_current_stream_capturing():
+                raise Backend(f"workspace buffer {name} would be made while a graph is captured: make the call once before")
             buf = (torch.zeros if zeroed else torch.empty)(max(count, 1), dtype=dtype, device=self.device)
             self._bufs[key] = buf
             self.generation += 1

@@ -6,6 +6,7 @@ import torch
 
 import plain_kv8 as plain
 from esp_b200.csrc import ops
+from esp_b200.errors import Backend
 from esp_b200.parts.base import Workspace
 
 pytestmark = pytest.mark.gpu
@@ -614,6 +615,20 @@ def test_calls_on_two_streams_with_a_workspace_each():
                 ops.attn_decode_kv8(q, k, v, exps, out, ws, seq, pos, table, PAGE, nh, nkv, hd, 0, st)
     torch.cuda.synchronize()
     assert st.item() == 0 and torch.equal(outs[0], want) and torch.equal(outs[1], want)
+
+
+def test_a_first_call_is_not_captured():
+    """The counters' zeros would be the graph's; refused, and the same workspace serves an eager call afterwards."""
+    nh, nkv, hd, lengths = 8, 2, 128, [3000, 700]
+    table, k, v, exps, q, seq, pos = decode_inputs(nh, nkv, hd, lengths, 4)
+    out, st, ws, graph = torch.empty_like(q), status(), Workspace(q.device), torch.cuda.CUDAGraph()
+    torch.cuda.synchronize()
+    with pytest.raises(Backend, match="captured"), torch.cuda.graph(graph):
+        ops.attn_decode_kv8(q, k, v, exps, out, ws, seq, pos, table, PAGE, nh, nkv, hd, 0, st)
+    del graph
+    ops.attn_decode_kv8(q, k, v, exps, out, ws, seq, pos, table, PAGE, nh, nkv, hd, 0, st)
+    assert st.item() == 0
+    check_decode(out, q, k, v, exps, table, lengths, nh, hd, 0)
 
 
 def test_append_then_attend_is_a_captured_step():
