@@ -509,12 +509,26 @@ __global__ void __launch_bounds__(THREADS, 1) attn_prefill_kv8_kernel(const __gr
             }
         };
         auto wait_all = [&](unsigned long long* bar, int parity) { return (bool)__all_sync(0xffffffffu, mbar_wait(bar, parity)); };
+        // A block's keys are asked for behind the conversion of the values before them, and only then is it said that those are there.
+        // (No load is on its way at the loop's end: there a warp would wait for it, 1,000 cycles a block.)
         uint4 codes[R];
-        bool ok = wait_all(&e_full[0], 0);
-        if (ok && entries[0].hi >= 0) ask(codes, entries[0], p.k);
-        for (int n = 0; ok; n++) {
+        bool ok = true;
+        auto values_done = [&](int n) {
+            fence_async_smem();
+            __syncwarp();
+            if (lane == 0) {
+                mbar_arrive(&v_full[n % STAGES]);
+                mbar_arrive(&e_empty[n % AHEAD]);
+            }
+        };
+        for (int n = 0;; n++) {
+            ok = wait_all(&e_full[n % AHEAD], (n / AHEAD) & 1);
+            if (!ok) break;
             const Entry& x = entries[n % AHEAD];
-            if (x.hi < 0) break;
+            const bool end = x.hi < 0;
+            if (!end) ask(codes, x, p.k);
+            if (n > 0) values_done(n - 1);
+            if (end) break;
             const int st = n % STAGES, free_parity = ((n / STAGES) & 1) ^ 1;
             ok = wait_all(&k_empty[st], free_parity);
             if (!ok) break;
@@ -526,16 +540,6 @@ __global__ void __launch_bounds__(THREADS, 1) attn_prefill_kv8_kernel(const __gr
             ok = wait_all(&v_empty[st], free_parity);
             if (!ok) break;
             convert(codes, x, true, smem_u32(v_s) + st * TILE + to);
-            const Entry& y = entries[(n + 1) % AHEAD];
-            ok = wait_all(&e_full[(n + 1) % AHEAD], ((n + 1) / AHEAD) & 1);
-            if (!ok) break;
-            if (y.hi >= 0) ask(codes, y, p.k);
-            fence_async_smem();
-            __syncwarp();
-            if (lane == 0) {
-                mbar_arrive(&v_full[st]);
-                mbar_arrive(&e_empty[n % AHEAD]);
-            }
         }
         if (!ok && lane == 0) {
             atomicOr(p.status, ESP_STATUS_WAIT_EXPIRED);
