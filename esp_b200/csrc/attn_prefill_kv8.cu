@@ -574,8 +574,11 @@ __global__ void __launch_bounds__(THREADS, 1) attn_prefill_kv8_kernel(const __gr
                 const bool edge = key0 + BN - 1 > first_pos || key0 < key_first_last;
                 const int c_lo = key_first - key0 - side * 64;
                 const unsigned c_span = (unsigned)(pos - key_first);
-                // 32 scores at a time: the second half for its maximum, then the first, which stays; the second is read again when its
-                // weights are made.  (All 64 in registers would spill, and what shared memory leaves of L1 does not hold spills.)
+                // 32 scores at a time (all 64 in registers would spill, and what shared memory leaves of L1 does not hold spills), each read
+                // once: their weights are taken by the maximum in use, ``ref``, unless they have outgrown it by 2^LAZY.  The row's threads
+                // meet when their weights are written: seldom has one of them gone over to another maximum, and then both scale what
+                // they have written, and O, to the larger one.  (A row's maxima are whole numbers, so that
+                // scaling a weight is exact.)
                 unsigned s[32];
                 auto scores = [&](int at) {
                     tc_ask32(s_addr + at, s);
@@ -585,65 +588,81 @@ __global__ void __launch_bounds__(THREADS, 1) attn_prefill_kv8_kernel(const __gr
                         for (int i = 0; i < 32; i++)
                             if ((unsigned)(at + i - c_lo) > c_span) s[i] = 0xff800000u;
                     }
-                };
-                float mx = -INFINITY;
-                if (ok) {
                     float m4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-                    for (int half = 1; half >= 0; half--) {
-                        scores(half * 32);
+                    for (int i = 0; i < 32; i += 8)
 #pragma unroll
-                        for (int i = 0; i < 32; i += 8)
-#pragma unroll
-                            for (int u = 0; u < 4; u++) m4[u] = fmaxf(fmaxf(m4[u], __uint_as_float(s[i + u])), __uint_as_float(s[i + u + 4]));
-                    }
-                    mx = fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3]));
-                }
-                float* xp = xmax + (grp * 2 + (n_b & 1)) * 256;                      // by turns: one meeting a block is enough
-                xp[side * 128 + r] = mx;
-                ok = all_agree(ok, bar_grp, 64);                                     // the row's two threads go on or leave together
-                if (!ok) break;
-                mx = fmaxf(mx, xp[(side ^ 1) * 128 + r]);
-                const float m_new = fmaxf(m_ref, mx * sc);
-                const bool grew = m_new > m_ref + LAZY;                              // the same for both threads of the row
-                if (j == j0) {
-                    m_ref = m_new;
-                } else if (__any_sync(0xffffffffu, grew)) {
-                    const float alpha = grew ? fast_exp2(m_ref - m_new) : 1.f;       // m_ref = -inf gives 0
-                    if (grew) m_ref = m_new;
-                    l_run *= alpha;
+                        for (int u = 0; u < 4; u++) m4[u] = fmaxf(fmaxf(m4[u], __uint_as_float(s[i + u])), __uint_as_float(s[i + u + 4]));
+                    return fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3])) * sc;
+                };
+                float ref = m_ref, l_blk = 0.f;
+                auto scale_weights = [&](unsigned at, int columns, float f) {
+                    __nv_bfloat162 f2 = __float2bfloat162_rn(f);
+                    tc_wait_st();
 #pragma unroll 1
-                    for (int u = side * (HD / 2); u < (side + 1) * (HD / 2); u += 8) {
+                    for (int u = 0; u < columns; u += 8) {
                         unsigned x[8];
-                        tc_ld8(o_addr + u, x);
+                        tc_ld8(at + u, x);
 #pragma unroll
-                        for (int i = 0; i < 8; i++) x[i] = __float_as_uint(__uint_as_float(x[i]) * alpha);
-                        tc_st8(o_addr + u, x);
-                    }
-                }
-                const float m_use = m_ref == -INFINITY ? 0.f : m_ref;
-                unsigned long long l_pair = 0ull;
-                const unsigned long long sc2 = pair_of(sc, sc), m2 = pair_of(-m_use, -m_use);
-                // the weights of 32 keys into 16 columns, over scores that have been read: P of the first 64 keys lies in the columns 0-31
-                // of S, that of the others in 64-95
-                auto weigh = [&](unsigned to) {
-                    unsigned packed[8];
-#pragma unroll
-                    for (int i = 0; i < 32; i += 2) {
-                        const float2 x = parts_of(fma_pair(pair_of(__uint_as_float(s[i]), __uint_as_float(s[i + 1])), sc2, m2));
-                        const float a = fast_exp2(x.x), b = fast_exp2(x.y);
-                        l_pair = add_pair(l_pair, pair_of(a, b));
-                        __nv_bfloat162 w = __floats2bfloat162_rn(a, b);
-                        packed[(i >> 1) & 7] = *reinterpret_cast<unsigned*>(&w);
-                        if (i % 16 == 14) tc_st8(to + (i / 16) * 8, packed);
+                        for (int i = 0; i < 8; i++) x[i] = mul_bf16x2(x[i], *reinterpret_cast<const unsigned*>(&f2));
+                        tc_st8(at + u, x);
                     }
                 };
-                weigh(s_addr);
-                scores(32);
-                weigh(s_addr + 16);
+                if (ok) {
+#pragma unroll
+                    for (int half = 0; half < 2; half++) {
+                        const float mx = scores(half * 32);
+                        const bool far = mx > ref + LAZY;
+                        if (__any_sync(0xffffffffu, far)) {
+                            const float now = !far ? ref : ceilf(mx), f = far ? fast_exp2(ref - now) : 1.f;      // ref = -inf gives 0
+                            if (half == 1) scale_weights(s_addr, 16, f);
+                            l_blk *= f;
+                            ref = now;
+                        }
+                        // the weights of 32 keys into 16 columns, over scores that have been read: P of the first 64 keys lies in the columns
+                        // 0-31 of S, that of the others in 64-95
+                        const float m_use = ref == -INFINITY ? 0.f : ref;
+                        unsigned long long l_pair = 0ull;
+                        const unsigned long long sc2 = pair_of(sc, sc), m2 = pair_of(-m_use, -m_use);
+                        unsigned packed[8];
+#pragma unroll
+                        for (int i = 0; i < 32; i += 2) {
+                            const float2 x = parts_of(fma_pair(pair_of(__uint_as_float(s[i]), __uint_as_float(s[i + 1])), sc2, m2));
+                            const float a = fast_exp2(x.x), b = fast_exp2(x.y);
+                            l_pair = add_pair(l_pair, pair_of(a, b));
+                            __nv_bfloat162 w = __floats2bfloat162_rn(a, b);
+                            packed[(i >> 1) & 7] = *reinterpret_cast<unsigned*>(&w);
+                            if (i % 16 == 14) tc_st8(s_addr + half * 16 + (i / 16) * 8, packed);
+                        }
+                        const float2 l2 = parts_of(l_pair);
+                        l_blk += l2.x + l2.y;
+                    }
+                }
+                const bool same = !__any_sync(0xffffffffu, ref != m_ref);
+                if (!all_agree(ok && same, bar_grp, 64)) {                           // the same for both of a row's threads
+                    float* xp = xmax + (grp * 2 + (n_b & 1)) * 256;                  // by turns
+                    xp[side * 128 + r] = ref;
+                    ok = all_agree(ok, bar_grp, 64);                                 // ... which go on or leave together
+                    if (!ok) break;
+                    const float now = fmaxf(ref, xp[(side ^ 1) * 128 + r]);
+                    const float f = ref < now ? fast_exp2(ref - now) : 1.f, alpha = m_ref < now ? fast_exp2(m_ref - now) : 1.f;
+                    scale_weights(s_addr, 32, f);
+                    l_blk *= f;
+                    l_run *= alpha;
+                    m_ref = now;
+                    if (j != j0) {
+#pragma unroll 1
+                        for (int u = side * (HD / 2); u < (side + 1) * (HD / 2); u += 8) {
+                            unsigned x[8];
+                            tc_ld8(o_addr + u, x);
+#pragma unroll
+                            for (int i = 0; i < 8; i++) x[i] = __float_as_uint(__uint_as_float(x[i]) * alpha);
+                            tc_st8(o_addr + u, x);
+                        }
+                    }
+                }
+                l_run += l_blk;
                 tc_wait_st();
-                const float2 l2 = parts_of(l_pair);
-                l_run += l2.x + l2.y;
                 tc_fence_before();                                                   // S has been read, P and O written
                 __syncwarp();
                 if (lane == 0) mbar_arrive(&p_ready[grp]);
@@ -667,6 +686,8 @@ __global__ void __launch_bounds__(THREADS, 1) attn_prefill_kv8_kernel(const __gr
             const float f0 = m0 == -INFINITY ? 0.f : fast_exp2(m0 - m_all), f1 = m1 == -INFINITY ? 0.f : fast_exp2(m1 - m_all);
             float l = f0 * (xsum[g0 * 256 + r] + xsum[g0 * 256 + 128 + r]);
             if (both) l += f1 * (xsum[256 + r] + xsum[384 + r]);
+            // a row of one key: the weight as it was rounded, so that the result is its value
+            if (p.window == 1 || t.pos0(0) + (t.pair ? grp * BM : 0) + r == 0) l = __bfloat162float(__float2bfloat16_rn(l));
             const float inv = 1.f / l;                               // 0 where all scores are -inf (an infinite query): 0 * inf is NaN
             const int cols = t.pair ? HD / 2 : HD / 4, col0 = (t.pair ? side : grp * 2 + side) * cols;   // what this thread writes
             const unsigned from = t.pair ? o_addr : tm_o + lane_sel;
