@@ -41,13 +41,16 @@ constexpr int STAGES = 2;                               // blocks of keys (and o
 constexpr int ROW_WARPS = 16, CONV_WARPS = 8, MMA_WARP = 24, Q_WARP = 25, PAGE_WARP = 26, THREADS = 896;
 constexpr int AHEAD = 4;                                // blocks of keys whose pages and exponents are known ahead
 constexpr int LIST = 4096;                              // tiles of a launch
+constexpr int FEW = 1024;                               // tiles of a launch that looks which way is better
+enum { SINGLY, IN_PAIRS, LOOK };                        // ways of a launch
+constexpr unsigned LIST_PAIR = 0x8000;                  // of a list's entry: the tile takes the next of its sequence along
 constexpr float LAZY = 8.f;
 
 struct Params {
     const unsigned char *k, *v, *exps;
     bf16* out;
     const int *tile_seq, *tile_first, *seq_start, *seq_past, *block_table;
-    int n_seqs, table_stride, n_pages, nh, nkv, hd, window, n_tiles, pair, smem_bytes, n_tokens;
+    int n_seqs, table_stride, n_pages, nh, nkv, hd, window, n_tiles, way, smem_bytes, n_tokens;
     float scale_log2;
     int* status;
 };
@@ -175,7 +178,7 @@ struct Item {
 };
 __device__ __forceinline__ Item load_item(const Params& p, const unsigned short* list, int item) {
     Item t;
-    const int tile = list[item / p.nh];
+    const unsigned entry = list[item / p.nh], tile = entry & (LIST_PAIR - 1);
     t.h = item % p.nh;
     t.kvh = t.h / (p.nh / p.nkv);
     t.seq = p.tile_seq[tile];
@@ -184,7 +187,7 @@ __device__ __forceinline__ Item load_item(const Params& p, const unsigned short*
     t.news = p.seq_start[t.seq + 1] - start;
     t.past = p.seq_past[t.seq];
     t.row0 = start + t.first;
-    t.pair = p.pair && t.first + BM < t.news;
+    t.pair = entry & LIST_PAIR;
     t.key_lo = first_visible_key(t.pos0(0), p.window, 0);
     t.key_hi = t.pos0(1) + t.rows(1) - 1;
     t.blk0 = t.key_lo / BN;
@@ -206,13 +209,16 @@ __global__ void __launch_bounds__(THREADS, 1) attn_prefill_kv8_kernel(const __gr
     constexpr int N_BARS = 12 + 4 * STAGES + 2 * AHEAD;
     unsigned* tmem_slot = reinterpret_cast<unsigned*>(bars + N_BARS);
     volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
-    int* n_active = reinterpret_cast<int*>(tmem_slot + 2);
-    float* xmax = reinterpret_cast<float*>(bars + 32);   // [group][parity][side][row]: maxima of a block
+    int* n_listed = reinterpret_cast<int*>(tmem_slot + 2);       // [2]: pairs, tiles
+    int* longest = n_listed + 2;                         // [2]: the time of the block with the most work, in pairs and singly
+    float* xmax = reinterpret_cast<float*>(bars + 36);   // [group][parity][side][row]: maxima of a block
     float* xsum = xmax + 2 * 2 * 2 * 128;                // [group][side][row]: sums at the item's end
     float* xref = xsum + 2 * 2 * 128;                    // [group][row]: the maxima that they go with
     Entry* entries = reinterpret_cast<Entry*>(xref + 2 * 128);           // [AHEAD]
-    unsigned short* list = reinterpret_cast<unsigned short*>(entries + AHEAD);
-    static_assert(N_BARS <= 30, "the barriers and three words take 256 bytes");
+    unsigned short* list = reinterpret_cast<unsigned short*>(entries + AHEAD);       // of the tiles that begin a pair
+    // where they are few: of all tiles, and [2][FEW] the blocks of keys of both lists' entries (before there are keys)
+    unsigned short *singles = list + FEW, *steps = reinterpret_cast<unsigned short*>(k_s);
+    static_assert(N_BARS <= 32, "the barriers and six words take 288 bytes");
     if (reinterpret_cast<unsigned char*>(list + LIST) > smem_raw + p.smem_bytes) {
         if (threadIdx.x == 0) atomicOr(p.status, ESP_STATUS_SMEM_LAYOUT);
         return;
@@ -230,6 +236,7 @@ __global__ void __launch_bounds__(THREADS, 1) attn_prefill_kv8_kernel(const __gr
         }
         for (int s = 0; s < AHEAD; s++) mbar_init(&e_empty[s], CONV_WARPS);
         *abort_flag = 0;
+        longest[0] = longest[1] = 0;
         asm volatile("fence.mbarrier_init.release.cluster;\n" ::: "memory");
     }
     if (warp == MMA_WARP) {
@@ -238,38 +245,84 @@ __global__ void __launch_bounds__(THREADS, 1) attn_prefill_kv8_kernel(const __gr
     }
     pdl_wait();
     pdl_trigger();
-    // ---- the tiles that begin an item, in the order of the list: with pairs, those whose place in their sequence is even
+    // ---- the tiles that begin an item, in the order of the list: singly all, with pairs those whose place in their sequence is even
     if (warp == Q_WARP) {
-        int n = 0;
+        int n = 0, n_pairs = 0;
         for (int i0 = 0; i0 < p.n_tiles; i0 += 32) {
             const int i = i0 + lane;
-            bool live = i < p.n_tiles;
-            if (live) {
+            bool fine = false, begins = false, goes_on = false;
+            int blocks = 0, both = 0;
+            if (i < p.n_tiles) {
                 // a tile of a sequence that is not there, without rows or with rows that the queries do not have, or with positions that the
-            // page table does not have is left out
+                // page table does not have is left out
                 const int seq = p.tile_seq[i], first = p.tile_first[i];
-                bool fine = seq >= 0 && seq < p.n_seqs && first >= 0;
+                fine = seq >= 0 && seq < p.n_seqs && first >= 0;
                 if (fine) {
                     const int start = p.seq_start[seq], end = p.seq_start[seq + 1], past = p.seq_past[seq];
                     fine = start >= 0 && end <= p.n_tokens && first < end - start && past >= 0 &&
                            ((long long)past + (end - start) - 1) / KV8_PAGE < p.table_stride;
+                    const int pos = past + first, lo = first_visible_key(pos, p.window, 0) / BN, last = past + end - start - 1;
+                    begins = fine && first / BM % 2 == 0;
+                    goes_on = first + BM < end - start;
+                    blocks = min(pos + BM - 1, last) / BN - lo + 1, both = min(pos + 2 * BM - 1, last) / BN - lo + 1;
                 }
                 if (!fine && blockIdx.x == 0) atomicOr(p.status, ESP_STATUS_BAD_INDEX);
-                live = fine && (!p.pair || (first / BM) % 2 == 0);
             }
-            const unsigned mask = __ballot_sync(0xffffffffu, live);
-            if (live) list[n + __popc(mask & ((1u << lane) - 1u))] = (unsigned short)i;
+            const unsigned below = (1u << lane) - 1u, mask = __ballot_sync(0xffffffffu, fine), mask2 = __ballot_sync(0xffffffffu, begins);
+            if (fine && p.way != IN_PAIRS) {
+                const int at = n + __popc(mask & below);
+                (p.way == LOOK ? singles : list)[at] = (unsigned short)i;
+                if (p.way == LOOK) steps[FEW + at] = (unsigned short)min(blocks, 65535);
+            }
+            if (begins && p.way != SINGLY) {
+                const int at = n_pairs + __popc(mask2 & below);
+                list[at] = (unsigned short)(i | (goes_on ? LIST_PAIR : 0u));
+                if (p.way == LOOK) steps[at] = (unsigned short)min(both, 65535);
+            }
             n += __popc(mask);
+            n_pairs += __popc(mask2);
         }
-        if (lane == 0) *n_active = n;
+        if (lane == 0) {
+            n_listed[0] = n_pairs;
+            n_listed[1] = n;
+        }
+    }
+    const int G = gridDim.x;
+    // block b takes the items b, 2G-1-b, 2G+b, ...: a long one is followed by a short one
+    auto nth_item = [&](int b, int round) { return round * G + (round & 1 ? G - 1 - b : b); };
+    // Pairs halve the conversions but are fewer and longer items, for which a step (a block of keys) takes 4/3 of the time.  Every block
+    // works out what the block with the most work has either way, an item counting three steps more than it has.  (210 tiles behind
+    // 4,953 keys: 138 us singly, 109 in pairs; 512 of a prompt of 4,096: 108 and 80; 256 of a prompt of 2,048: 37 and 46; 232 of four
+    // prompts of 3,693: 58 and 81.)
+    if (p.way == LOOK) {
+        __syncthreads();
+        int most[2] = {0, 0};
+        if ((int)threadIdx.x < G) {
+#pragma unroll
+            for (int u = 0; u < 2; u++) {
+                const int items = n_listed[u] * p.nh;
+                for (int round = 0; round * G < items; round++) {
+                    const int item = nth_item(threadIdx.x, round);
+                    if (item < items) most[u] += steps[u * FEW + item / p.nh] + 3;
+                }
+            }
+        }
+#pragma unroll
+        for (int u = 0; u < 2; u++) {
+            most[u] = __reduce_max_sync(0xffffffffu, most[u]);
+            if (lane == 0 && most[u] > 0) atomicMax(&longest[u], most[u]);
+        }
+        __syncthreads();
+        if (4LL * longest[0] >= 3LL * longest[1]) {
+            for (int i = threadIdx.x; i < n_listed[1]; i += THREADS) list[i] = singles[i];
+        }
     }
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
     const unsigned tmem = (unsigned)uniform((int)*tmem_slot), tm_s = tmem, tm_o = tmem + 256;    // S of the groups at columns 0 and 128, O at 256 and 384
-    const int n_items = *n_active * p.nh, G = gridDim.x;
-    // block b takes the items b, 2G-1-b, 2G+b, ...: a long one is followed by a short one
-    auto item_of = [&](int round) { return round * G + ((round & 1) ? G - 1 - (int)blockIdx.x : (int)blockIdx.x); };
+    const int n_items = n_listed[p.way == IN_PAIRS || (p.way == LOOK && 4LL * longest[0] < 3LL * longest[1]) ? 0 : 1] * p.nh;
+    auto item_of = [&](int round) { return nth_item(blockIdx.x, round); };
 
     if (warp >= MMA_WARP) asm volatile("setmaxnreg.dec.sync.aligned.u32 72;\n");
     if (warp == Q_WARP) {
@@ -752,7 +805,7 @@ int make_query_map(CUtensorMap* map, const void* base, long long rows, int nh, i
 
 template <int HD> int launch(const CUtensorMap& map_q, Params p, int device, cudaStream_t stream) {
     constexpr int TILE = HD / 64 * ATOM;
-    const size_t smem = 1024 + (size_t)(2 + 2 * STAGES) * TILE + 256 + (8 + 4 + 2) * 128 * 4 + AHEAD * sizeof(Entry) + LIST * 2;
+    const size_t smem = 1024 + (size_t)(2 + 2 * STAGES) * TILE + 288 + (8 + 4 + 2) * 128 * 4 + AHEAD * sizeof(Entry) + LIST * 2;
     static bool raised[64] = {false};
     static int sm_count[64] = {0};
     if (!raised[device]) {
@@ -762,9 +815,10 @@ template <int HD> int launch(const CUtensorMap& map_q, Params p, int device, cud
         raised[device] = true;
     }
     p.smem_bytes = (int)smem;
-    // Pairs halve the conversions and the number of items: not where the device would not be filled by them.  One rule for all
-    // launches, as a tile is left to its neighbour, which another launch may list.
-    p.pair = (long long)p.n_tiles * p.nh >= 4LL * sm_count[device];
+    // An item for each SM at most: singly.  Many: in pairs, and in all launches, as a tile is left to its neighbour, which another launch may
+    // list.  Between the two the kernel looks at what the tiles see.
+    const long long all_items = (long long)p.n_tiles * p.nh;
+    p.way = all_items <= sm_count[device] ? SINGLY : all_items >= 4LL * sm_count[device] || p.n_tiles > FEW ? IN_PAIRS : LOOK;
     for (int at = 0; at < p.n_tiles; at += LIST) {
         Params q = p;
         q.tile_seq += at, q.tile_first += at;

@@ -380,6 +380,11 @@ PREFILL = [
     (40, 8, 128, [1700, 130, 1, 300], [200, 1000, 64, 0], 260),
     (60, 60, 104, [1281], [0], 1),
     (48, 3, 24, [900, 900], [3, 60], 1000),
+    # between: the kernel looks at what the tiles see (in pairs; singly; tiles of unequal length; with a window)
+    (35, 5, 128, [706], [1953], 0),
+    (16, 8, 64, [2048], [0], 0),
+    (7, 1, 128, [2500, 5, 1, 640], [100, 900, 0, 1], 0),
+    (12, 3, 104, [1500, 300], [0, 700], 150),
 ]
 
 
