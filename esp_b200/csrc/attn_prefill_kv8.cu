@@ -145,6 +145,11 @@ __device__ __forceinline__ void tc_wait_ld(unsigned (&r)[32]) {
           "+r"(r[31])::"memory");
 }
 
+__device__ __forceinline__ unsigned pack_bf16(float a, float b) {
+    __nv_bfloat162 w = __floats2bfloat162_rn(a, b);
+    return *reinterpret_cast<unsigned*>(&w);
+}
+
 // ---- two codes' bits (two bytes of w) in a bfloat16 pair's places: each is its number times 2^-120
 template <unsigned SELECT> __device__ __forceinline__ unsigned spread_codes(unsigned w) {
     unsigned r;                                         // bytes (code, its sign eight times) of two codes
@@ -683,8 +688,7 @@ __global__ void __launch_bounds__(THREADS, 1) attn_prefill_kv8_kernel(const __gr
                             const float2 x = parts_of(fma_pair(pair_of(__uint_as_float(s[i]), __uint_as_float(s[i + 1])), sc2, m2));
                             const float a = fast_exp2(x.x), b = fast_exp2(x.y);
                             l_pair = add_pair(l_pair, pair_of(a, b));
-                            __nv_bfloat162 w = __floats2bfloat162_rn(a, b);
-                            packed[(i >> 1) & 7] = *reinterpret_cast<unsigned*>(&w);
+                            packed[(i >> 1) & 7] = pack_bf16(a, b);
                             if (i % 16 == 14) tc_st8(s_addr + half * 16 + (i / 16) * 8, packed);
                         }
                         const float2 l2 = parts_of(l_pair);
@@ -731,38 +735,56 @@ __global__ void __launch_bounds__(THREADS, 1) attn_prefill_kv8_kernel(const __gr
             ok = t.pair ? all_agree(ok, bar_grp, 64) : all_agree(ok, bar_row, 128);
             if (!ok) break;
             tc_fence_after();
-            const bool live = r < t.rows(grp);
-            bf16* orow = p.out + ((size_t)(t.row0 + (t.pair ? grp * BM : 0) + r) * p.nh + t.h) * p.hd;
             // a group without a key for this row counts 0 (and a row that is no number stays one: 0 * NaN)
             const int g0 = t.pair ? grp : 0;
             const float m0 = t.pair ? m_ref : xref[r], m1 = both ? xref[128 + r] : -INFINITY, m_all = fmaxf(m0, m1);
-            const float f0 = m0 == -INFINITY ? 0.f : fast_exp2(m0 - m_all), f1 = m1 == -INFINITY ? 0.f : fast_exp2(m1 - m_all);
+            float f0 = m0 == -INFINITY ? 0.f : fast_exp2(m0 - m_all), f1 = m1 == -INFINITY ? 0.f : fast_exp2(m1 - m_all);
             float l = f0 * (xsum[g0 * 256 + r] + xsum[g0 * 256 + 128 + r]);
             if (both) l += f1 * (xsum[256 + r] + xsum[384 + r]);
             // a row of one key: the weight as it was rounded, so that the result is its value
             if (p.window == 1 || t.pos0(0) + (t.pair ? grp * BM : 0) + r == 0) l = __bfloat162float(__float2bfloat16_rn(l));
             const float inv = 1.f / l;                               // 0 where all scores are -inf (an infinite query): 0 * inf is NaN
-            const int cols = t.pair ? HD / 2 : HD / 4, col0 = (t.pair ? side : grp * 2 + side) * cols;   // what this thread writes
+            // what this thread takes from tensor memory: 32 columns of its row at a time.  Four lanes then exchange their pieces of eight, so that
+            // a store writes 64 bytes of each of eight rows (of 32 rows it would write 16: 5,000 cycles an item).
+            const int cols = t.pair ? HD / 2 : 32, col0 = (t.pair ? side : grp * 2 + side) * cols;
             const unsigned from = t.pair ? o_addr : tm_o + lane_sel;
+            const int row_g = t.pair ? grp * BM : 0, n_rows = t.rows(grp), piece = lane & 3;
+            f0 *= inv, f1 *= inv;
 #pragma unroll 1
-            for (int col = col0; col < col0 + cols; col += 8) {
-                unsigned x[8];
-                tc_ld8(from + col, x);
-                float o[8];
+            for (int col = col0; col < col0 + cols && col < HD; col += 32) {
+                uint4 w[4];
 #pragma unroll
-                for (int i = 0; i < 8; i++) o[i] = __uint_as_float(x[i]) * f0;
-                if (both) {
-                    tc_ld8(tm_o + BN + lane_sel + col, x);
+                for (int u = 0; u < 4; u++) {
+                    unsigned x[8];
+                    tc_ld8(from + col + u * 8, x);
+                    float o[8];
 #pragma unroll
-                    for (int i = 0; i < 8; i++) o[i] += __uint_as_float(x[i]) * f1;
+                    for (int i = 0; i < 8; i++) o[i] = __uint_as_float(x[i]) * f0;
+                    if (both) {
+                        tc_ld8(tm_o + BN + lane_sel + col + u * 8, x);
+#pragma unroll
+                        for (int i = 0; i < 8; i++) o[i] += __uint_as_float(x[i]) * f1;
+                    }
+                    w[u] = make_uint4(pack_bf16(o[0], o[1]), pack_bf16(o[2], o[3]), pack_bf16(o[4], o[5]), pack_bf16(o[6], o[7]));
                 }
-                if (live && col < p.hd) {
-                    __nv_bfloat162 w[4];
+                // w[u] of the group's lane i becomes piece i of its row u
 #pragma unroll
-                    for (int u = 0; u < 4; u++) w[u] = __floats2bfloat162_rn(o[2 * u] * inv, o[2 * u + 1] * inv);
-                    *reinterpret_cast<uint4*>(orow + col) = make_uint4(*reinterpret_cast<unsigned*>(&w[0]), *reinterpret_cast<unsigned*>(&w[1]),
-                                                                       *reinterpret_cast<unsigned*>(&w[2]), *reinterpret_cast<unsigned*>(&w[3]));
-                }
+                for (int bit = 1; bit <= 2; bit *= 2)
+#pragma unroll
+                    for (int u = 0; u < 4; u++) {
+                        if (u & bit) continue;
+                        const bool up = piece & bit;
+                        uint4 give = up ? w[u] : w[u + bit];
+                        give.x = __shfl_xor_sync(0xffffffffu, give.x, bit), give.y = __shfl_xor_sync(0xffffffffu, give.y, bit);
+                        give.z = __shfl_xor_sync(0xffffffffu, give.z, bit), give.w = __shfl_xor_sync(0xffffffffu, give.w, bit);
+                        if (up) w[u] = give;
+                        else w[u + bit] = give;
+                    }
+                const int c = col + piece * 8, r0 = r - piece;
+                bf16* to = p.out + ((size_t)(t.row0 + row_g + r0) * p.nh + t.h) * p.hd + c;
+#pragma unroll
+                for (int u = 0; u < 4; u++)
+                    if (r0 + u < n_rows && c < p.hd) *reinterpret_cast<uint4*>(to + (size_t)u * p.nh * p.hd) = w[u];
             }
             tc_fence_before();
             // the sums and O's have been read
