@@ -29,6 +29,9 @@
 // a level: a fence, a count, two trips to L2).  A grid of (row, head, split) blocks of one split length took 29.4, 86, 42.5 and
 // 8.9 us, with the best length of each case 29.3, 60, 41 and 8.2.  Three blocks an SM with rings of two stages instead of two
 // with three: 33.4, 53.7, 37.4 and 7.7 us.
+// Heads are padded to 64, 96, 128 or 256 channels (22 sequences of 7,411 keys, 5 heads of 80: 40.2 us in 96, 43.8 in 128; steps over
+// channels that are not there left out at run time instead: 49, as the branches keep the loads of one step from the products of
+// the last).
 #include "kv8.cuh"
 
 namespace {
@@ -94,13 +97,15 @@ __device__ __forceinline__ void copies_commit() { asm volatile("cp.async.commit_
 template <int N> __device__ __forceinline__ void copies_wait() { asm volatile("cp.async.wait_group %0;\n" ::"n"(N) : "memory"); }
 
 template <int HD> struct Ring {
-    static constexpr int STAGES = HD == 64 ? 4 : HD == 128 ? 3 : 2;
-    static constexpr int STAGE = CHUNK * HD * 2 + 2 * CHUNK;             // keys, values, exponents of both
+    static constexpr int STAGES = HD == 64 ? 4 : HD == 256 ? 2 : 3;
+    static constexpr int ROW = HD == 96 ? 112 : HD;                      // bytes from row to row
+    static constexpr int STAGE = CHUNK * ROW * 2 + 2 * CHUNK;            // keys, values, exponents of both
     static constexpr int WARP = (STAGES * STAGE + 127) / 128 * 128;
 };
-// where the 16-byte piece c of row r lies: rows of 64 bytes share 128 bytes with a neighbour
+// where the 16-byte piece c of row r lies: rows of 64 bytes share 128 bytes with a neighbour; rows of 96 bytes lie 112 apart, which keeps
+// eight of them in different banks as they are
 template <int HD> __device__ __forceinline__ int piece_at(int r, int c) {
-    return r * HD + ((c ^ (HD == 64 ? (r >> 1) & 3 : r & 7)) << 4);
+    return HD == 96 ? r * 112 + (c << 4) : r * HD + ((c ^ (HD == 64 ? (r >> 1) & 3 : r & 7)) << 4);
 }
 
 
@@ -114,7 +119,7 @@ template <int HD, int NT, bool RUN> struct Stream {
 
     // asks for the chunk of keys key0 .. key0 + 31 in page ``page``; those outside [k0, k1] are filled with zeros
     static __device__ __forceinline__ void ask(const Params& p, unsigned char* st, int page, int kvh, int key0, int k0, int k1, int lane) {
-        const unsigned k_dst = smem_addr(st), v_dst = k_dst + CHUNK * HD, e_dst = v_dst + CHUNK * HD;
+        const unsigned k_dst = smem_addr(st), v_dst = k_dst + CHUNK * Ring<HD>::ROW, e_dst = v_dst + CHUNK * Ring<HD>::ROW;
         const bool wanted = key0 <= k1 && key0 + CHUNK > k0, ok = wanted && page >= 0 && page < p.n_pages;
         if (wanted && !ok && lane == 0) atomicOr(p.status, ESP_STATUS_BAD_INDEX);
         const size_t block = ok ? (size_t)page * p.nkv + kvh : 0;
@@ -196,8 +201,8 @@ template <int HD, int NT, bool RUN> struct Stream {
     // to pos0 + r, and of them the last ``window``)
     __device__ __forceinline__ void chunk(const unsigned char* st, int key0, int k0, int k1, int pos0, int window, int lane) {
         const int g8 = lane >> 2, tg = lane & 3;
-        const unsigned k_src = smem_addr(st), v_src = k_src + CHUNK * HD;
-        const unsigned char* e_src = st + 2 * CHUNK * HD;
+        const unsigned k_src = smem_addr(st), v_src = k_src + CHUNK * Ring<HD>::ROW;
+        const unsigned char* e_src = st + 2 * CHUNK * Ring<HD>::ROW;
         // ---- S^T: 32 keys (two tiles of 16) by the rows
         float s[NT][2][4];
 #pragma unroll
@@ -728,6 +733,7 @@ ESP_API int esp_attn_decode_kv8(const void* q, const void* k, const void* v, con
         p.q = (const bf16*)q + (size_t)at * nh * hd, p.out = (bf16*)out + (size_t)at * nh * hd;
         int rc;
         if (hd <= 64) rc = wide ? launch_decode<64, 2>(p, blocks, stream) : launch_decode<64, 1>(p, blocks, stream);
+        else if (hd <= 96) rc = wide ? launch_decode<96, 2>(p, blocks, stream) : launch_decode<96, 1>(p, blocks, stream);
         else if (hd <= 128) rc = wide ? launch_decode<128, 2>(p, blocks, stream) : launch_decode<128, 1>(p, blocks, stream);
         else rc = wide ? launch_decode<256, 2>(p, blocks, stream) : launch_decode<256, 1>(p, blocks, stream);
         if (rc) return rc;

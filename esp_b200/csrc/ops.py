@@ -1639,7 +1639,7 @@ def _sm_count(device: int) -> int:
     return torch.cuda.get_device_properties(device).multi_processor_count
 
 
-# blocks of the decode kernel that an SM holds at a time, by the width that heads are padded to (shared memory: 66, 99, 131 KB)
+# blocks of the decode kernel that an SM holds at a time, by the width that heads are padded to (shared memory: 66, 99 (87 for 96 channels), 131 KB)
 ATTN_DECODE_KV8_BLOCKS_PER_SM = {64: 3, 128: 2, 256: 1}
 
 

@@ -228,6 +228,10 @@ DECODE = [
     (16, 16, 128, [130] * 40, 0),
     (2, 2, 128, [3000, 1, 129, 128, 127, 5000] * 5, 0),
     (1, 1, 64, [70 + 13 * i for i in range(1100)], 0),
+    (24, 2, 96, [1, 95, 96, 97, 1500], 0),
+    (7, 7, 96, [2000, 31, 640], 100),
+    (3, 3, 72, [129, 4000], 0),
+    (16, 1, 88, [900], 0),
     (2, 1, 8, [300], 0),
 ]
 
