@@ -31,7 +31,9 @@
 // with three: 33.4, 53.7, 37.4 and 7.7 us.
 // Heads are padded to 64, 96, 128 or 256 channels (22 sequences of 7,411 keys, 5 heads of 80: 40.2 us in 96, 43.8 in 128; steps over
 // channels that are not there left out at run time instead: 49, as the branches keep the loads of one step from the products of
-// the last).
+// the last; 8 of 4,096 keys, 16 heads of 192: 43.7 us in 192, where two blocks fit an SM, 58 in 256).  Query heads of a key
+// head beyond eight go into one block of sixteen rows, but for heads of more than 128 channels into two of eight (their keys come
+// from L2 the second time): 48 heads on 4 of 256 channels, 8 sequences of 4,096: 40.6 us; sixteen rows spill and take 56.
 #include "kv8.cuh"
 
 namespace {
@@ -97,15 +99,15 @@ __device__ __forceinline__ void copies_commit() { asm volatile("cp.async.commit_
 template <int N> __device__ __forceinline__ void copies_wait() { asm volatile("cp.async.wait_group %0;\n" ::"n"(N) : "memory"); }
 
 template <int HD> struct Ring {
-    static constexpr int STAGES = HD == 64 ? 4 : HD == 256 ? 2 : 3;
-    static constexpr int ROW = HD == 96 ? 112 : HD;                      // bytes from row to row
+    static constexpr int STAGES = HD == 64 ? 4 : HD >= 192 ? 2 : 3;
+    static constexpr int ROW = HD == 96 ? 112 : HD == 192 ? 208 : HD;                      // bytes from row to row
     static constexpr int STAGE = CHUNK * ROW * 2 + 2 * CHUNK;            // keys, values, exponents of both
     static constexpr int WARP = (STAGES * STAGE + 127) / 128 * 128;
 };
-// where the 16-byte piece c of row r lies: rows of 64 bytes share 128 bytes with a neighbour; rows of 96 bytes lie 112 apart, which keeps
-// eight of them in different banks as they are
+// where the 16-byte piece c of row r lies: rows of 64 bytes share 128 bytes with a neighbour; rows of 96 and 192 bytes lie 112 and 208
+// apart, which keeps eight of them in different banks as they are
 template <int HD> __device__ __forceinline__ int piece_at(int r, int c) {
-    return HD == 96 ? r * 112 + (c << 4) : r * HD + ((c ^ (HD == 64 ? (r >> 1) & 3 : r & 7)) << 4);
+    return Ring<HD>::ROW != HD ? r * Ring<HD>::ROW + (c << 4) : r * HD + ((c ^ (HD == 64 ? (r >> 1) & 3 : r & 7)) << 4);
 }
 
 
@@ -735,7 +737,8 @@ ESP_API int esp_attn_decode_kv8(const void* q, const void* k, const void* v, con
         if (hd <= 64) rc = wide ? launch_decode<64, 2>(p, blocks, stream) : launch_decode<64, 1>(p, blocks, stream);
         else if (hd <= 96) rc = wide ? launch_decode<96, 2>(p, blocks, stream) : launch_decode<96, 1>(p, blocks, stream);
         else if (hd <= 128) rc = wide ? launch_decode<128, 2>(p, blocks, stream) : launch_decode<128, 1>(p, blocks, stream);
-        else rc = wide ? launch_decode<256, 2>(p, blocks, stream) : launch_decode<256, 1>(p, blocks, stream);
+        else if (hd <= 192) rc = launch_decode<192, 1>(p, blocks, stream);
+        else rc = launch_decode<256, 1>(p, blocks, stream);
         if (rc) return rc;
     }
     return 0;

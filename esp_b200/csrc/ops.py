@@ -1639,8 +1639,8 @@ def _sm_count(device: int) -> int:
     return torch.cuda.get_device_properties(device).multi_processor_count
 
 
-# blocks of the decode kernel that an SM holds at a time, by the width that heads are padded to (shared memory: 66, 99 (87 for 96 channels), 131 KB)
-ATTN_DECODE_KV8_BLOCKS_PER_SM = {64: 3, 128: 2, 256: 1}
+# blocks of the decode kernel that an SM holds at a time, by the width that heads are padded to (shared memory: 66, 99 (87 for 96 channels), 107, 131 KB)
+ATTN_DECODE_KV8_BLOCKS_PER_SM = {64: 3, 128: 2, 192: 2, 256: 1}
 
 
 def attn_decode_kv8(q, k, v, exps, out, ws, tok_seq, tok_pos, block_table, page, nh, nkv, hd, window, status, seq_past=None):
@@ -1670,7 +1670,7 @@ def attn_decode_kv8(q, k, v, exps, out, ws, tok_seq, tok_pos, block_table, page,
                     (("tok_seq", tok_seq, n), ("tok_pos", tok_pos, n), ("seq_past", seq_past, block_table.shape[0])),
                     (("the queries", q), ("the keys", k), ("the values", v), ("the exponents", exps), ("the results", out)))
     n_seqs, stride = block_table.shape
-    blocks = ATTN_DECODE_KV8_BLOCKS_PER_SM[64 if hd <= 64 else 128 if hd <= 128 else 256] * _sm_count(_device_index)
+    blocks = ATTN_DECODE_KV8_BLOCKS_PER_SM[64 if hd <= 64 else 128 if hd <= 128 else 192 if hd <= 192 else 256] * _sm_count(_device_index)
     parts = _ptr(ws.get("attn_kv8_parts", (blocks * 32, hd + 2), _F32))
     counters = _ptr(ws.get("attn_kv8_counters", (min(n, 1024) * nh + 2 * blocks,), torch.int32, zeroed=True))
     _check(_fn("kv8", "esp_attn_decode_kv8")(
