@@ -29,11 +29,9 @@
 // a level: a fence, a count, two trips to L2).  A grid of (row, head, split) blocks of one split length took 29.4, 86, 42.5 and
 // 8.9 us, with the best length of each case 29.3, 60, 41 and 8.2.  Three blocks an SM with rings of two stages instead of two
 // with three: 33.4, 53.7, 37.4 and 7.7 us.
-// Heads are padded to 64, 96, 128 or 256 channels (22 sequences of 7,411 keys, 5 heads of 80: 40.2 us in 96, 43.8 in 128; steps over
-// channels that are not there left out at run time instead: 49, as the branches keep the loads of one step from the products of
-// the last; 8 of 4,096 keys, 16 heads of 192: 43.7 us in 192, where two blocks fit an SM, 58 in 256).  Query heads of a key
-// head beyond eight go into one block of sixteen rows, but for heads of more than 128 channels into two of eight (their keys come
-// from L2 the second time): 48 heads on 4 of 256 channels, 8 sequences of 4,096: 40.6 us; sixteen rows spill and take 56.
+// Heads are padded to 64, 96, 128, 192 or 256 channels (22 sequences of 7,411 keys, 5 heads of 80: 40.2 us in 96, 43.8 in 128; steps
+// over channels that are not there left out at run time instead: 49, as the branches keep the loads of one step from the products of
+// the last.  8 sequences of 4,096, 16 heads of 192: 43.7 us in 192, where two blocks fit an SM, 58 in 256).
 #include "kv8.cuh"
 
 namespace {
@@ -728,13 +726,18 @@ ESP_API int esp_attn_decode_kv8(const void* q, const void* k, const void* v, con
         return (int)cudaErrorInvalidValue;
     Params p = make_params(q, k, v, exps, out, block_table, n_seqs, table_stride, n_pages, nh, nkv, hd, window, status);
     p.parts = parts, p.counters = counters, p.seq_past = seq_past;
-    const bool wide = nh / nkv > 8;
+    // The query heads of a key head beyond eight: blocks of sixteen rows, or two of eight, whose keys come from L2 the second time.  Sixteen
+    // rows have twice as much to join and, in wide heads, spill; they win where a block has a long way to go (units a block by the
+    // page table's width, sixteen rows and eight: 48 heads on 4, 32 sequences of 2,000: 6.9 units, 29.3 and 31.3 us; 28 on 2 of 96
+    // channels, 20 of 8,000: 8.4, 30.9 and 36.1; 16 on 1, 20 of 8,000: 4.2, 28.6 and 24.9; 32 on 2, 8 of 4,096: 1.7, 24.0 and 17.5; of 64
+    // channels 20 of 8,000: 33.2 and 25.7; 48 on 4 of 256, 8 of 4,096: 56.2 and 40.6).
+    const bool wide = nh / nkv > 8 && (long long)n_tokens * nkv * table_stride * KV8_PAGE / UNIT > 5LL * blocks;
     for (int at = 0; at < n_tokens; at += MAX_ROWS) {                    // more rows than a block's list holds: one call behind the other
         p.n_rows = n_tokens - at < MAX_ROWS ? n_tokens - at : MAX_ROWS;
         p.tok_seq = tok_seq + at, p.tok_pos = tok_pos + at;
         p.q = (const bf16*)q + (size_t)at * nh * hd, p.out = (bf16*)out + (size_t)at * nh * hd;
         int rc;
-        if (hd <= 64) rc = wide ? launch_decode<64, 2>(p, blocks, stream) : launch_decode<64, 1>(p, blocks, stream);
+        if (hd <= 64) rc = launch_decode<64, 1>(p, blocks, stream);
         else if (hd <= 96) rc = wide ? launch_decode<96, 2>(p, blocks, stream) : launch_decode<96, 1>(p, blocks, stream);
         else if (hd <= 128) rc = wide ? launch_decode<128, 2>(p, blocks, stream) : launch_decode<128, 1>(p, blocks, stream);
         else if (hd <= 192) rc = launch_decode<192, 1>(p, blocks, stream);

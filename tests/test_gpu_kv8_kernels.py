@@ -232,6 +232,10 @@ DECODE = [
     (7, 7, 96, [2000, 31, 640], 100),
     (3, 3, 72, [129, 4000], 0),
     (16, 1, 88, [900], 0),
+    # enough keys for blocks of sixteen rows
+    (12, 1, 128, [40000, 33000, 50000, 1], 0),
+    (28, 2, 72, [30000, 25001, 20000], 0),
+    (34, 2, 104, [30000, 25001, 20000], 20000),
     (2, 1, 8, [300], 0),
 ]
 
