@@ -16,12 +16,14 @@
 // of its own, in all 512 columns of tensor memory.  Where there are few items, or a tile has no neighbour, the two groups
 // take the blocks of one tile in turn instead (SPLIT) and join their results.
 //
-// Measured (B200): 8,192 tokens, 16 heads of 128, 283 us = 0.97 PFLOP/s (the kernel for the bfloat16 cache: 335); five ragged chunks
-// of 500 to 1,500 tokens behind contexts of 1,500 to 4,600, 28 heads on 4, 405 us = 0.86.  A step of one block for both tiles takes about
-// 4,400 cycles, of which the tensor core needs 2,050 (counters: tensor pipe 45 %, issue slots 61 %, ALU 47 %).  What bounds it are the converting warps (their loads and stores share
-// shared memory's 128 bytes a cycle with the MMAs' operands) and, close behind, the row threads' chain (scores 850, meeting
-// 570, weights 1,600, then P V and the next scores).  Spills cost more than anything else: beside 200 KB of shared memory
-// they miss L1 (393 us with 17 local loads a warp and block, 296 without).
+// Measured (B200): 8,192 tokens, 16 heads of 128, 276 us = 1.0 PFLOP/s (the kernel for the bfloat16 cache: 335); five ragged chunks
+// of 500 to 1,500 tokens behind contexts of 1,500 to 4,600, 28 heads on 4, 390 us = 0.89.  A step of one block for both tiles takes about
+// 4,000 cycles, of which the tensor core needs 2,050 (counters: tensor pipe 48 %, issue slots 62 %, ALU 49 %, exponentials 50 %).  What
+// bounds it are the converting warps (their loads and stores share shared memory's 128 bytes a cycle with the MMAs' operands, their
+// instructions the issue slots with the row threads) and, close behind, a group's chain: scores, weights and meeting 2,200 cycles, then
+// P V and the next scores 1,024.  An item costs about 5 us besides (its first and last products and its results, which nothing of the
+// same rows overlaps).  Spills cost more than anything else: beside 200 KB of shared memory they miss L1 (17 local loads a warp and
+// block: 393 us for 296).
 //
 // A position that is no number (kv8.cuh) is made a key of NaN with a value of zeros: whoever sees it gets NaN through the score,
 // and a masked score takes nothing of it.
