@@ -364,13 +364,16 @@ __global__ void __launch_bounds__(THREADS) attn_run_kv8_kernel(const Params p) {
     unsigned char* ring = smem + warp * Ring<HD>::WARP;
     pdl_wait();
     // the block's rows: ``rows`` tokens from ``first`` on, all of head ``head``
-    const int subs = 128 / S::ROWS, tile = blockIdx.x / subs, seq = p.tile_seq[tile], first = p.tile_first[tile] + (blockIdx.x % subs) * S::ROWS;
-    if (seq < 0 || seq >= p.n_seqs || first < 0) {
+    const int subs = 128 / S::ROWS, tile = blockIdx.x / subs, seq = p.tile_seq[tile], tile_first = p.tile_first[tile], first = tile_first + (blockIdx.x % subs) * S::ROWS;
+    if (seq < 0 || seq >= p.n_seqs || tile_first < 0 || tile_first % 128) {
         if (threadIdx.x == 0) atomicOr(p.status, ESP_STATUS_BAD_INDEX);
         return;
     }
     const int start = p.seq_start[seq], end = p.seq_start[seq + 1], rows = min(S::ROWS, end - start - first), head = blockIdx.y, kvh = head / (p.nh / p.nkv);
-    if (rows <= 0) return;
+    if (rows <= 0) {                           // behind the sequence's last token; a whole tile there is none
+        if (threadIdx.x == 0 && first == tile_first) atomicOr(p.status, ESP_STATUS_BAD_INDEX);
+        return;
+    }
     const int past = p.seq_past[seq], pos0 = past + first, k0 = first_visible_key(pos0, p.window, 0), k1 = pos0 + rows - 1;
     // rows that the queries do not have, or positions that the page table does not have
     if (start < 0 || end > p.n_rows || past < 0 || ((long long)past + first + rows - 1) / KV8_PAGE >= p.table_stride) {

@@ -260,10 +260,10 @@ __global__ void __launch_bounds__(THREADS, 1) attn_prefill_kv8_kernel(const __gr
             bool fine = false, begins = false, goes_on = false;
             int blocks = 0, both = 0;
             if (i < p.n_tiles) {
-                // a tile of a sequence that is not there, without rows or with rows that the queries do not have, or with positions that the
+                // a tile of a sequence that is not there, that is none of its tiles, without rows or with rows that the queries do not have, or with positions that the
                 // page table does not have is left out
                 const int seq = p.tile_seq[i], first = p.tile_first[i];
-                fine = seq >= 0 && seq < p.n_seqs && first >= 0;
+                fine = seq >= 0 && seq < p.n_seqs && first >= 0 && first % BM == 0;
                 if (fine) {
                     const int start = p.seq_start[seq], end = p.seq_start[seq + 1], past = p.seq_past[seq];
                     fine = start >= 0 && end <= p.n_tokens && first < end - start && past >= 0 &&
@@ -858,7 +858,7 @@ template <int HD> int launch(const CUtensorMap& map_q, Params p, int device, cud
 }  // namespace
 
 // q and out [n_tokens, nh, hd] bfloat16; tile_seq / tile_first: all tiles of 128 new tokens (sequence, the tile's first token among
-// the sequence's new ones), best listed with those that see the most keys first; hd a multiple of 8 up to 128.
+// the sequence's new ones, a multiple of 128), best listed with those that see the most keys first; hd a multiple of 8 up to 128.
 ESP_API int esp_attn_prefill_kv8(const void* q, long long n_tokens, const void* k, const void* v, const void* exps, void* out, const int* tile_seq,
                                  const int* tile_first, const int* seq_start, const int* seq_past, const int* block_table, int n_seqs, int table_stride,
                                  int n_pages, int n_tiles, int nh, int nkv, int hd, int window, int* status, cudaStream_t stream) {

@@ -1683,7 +1683,7 @@ def attn_prefill_kv8(q, k, v, exps, out, tile_seq, tile_first, seq_start, seq_pa
     """Causal attention of runs of new tokens, packed back to back, over the 8-bit cache that holds their own keys already:
     the step's rows seq_start[i] .. seq_start[i + 1] are sequence i's, behind seq_past[i] cached positions.  ``tile_seq`` and
     ``tile_first``: all tiles of ATTN_TC05_TILE_ROWS new tokens (sequence, index of the tile's first token among the
-    sequence's new ones), best with those first that see the most keys.  The rest as for ``attn_decode_kv8``."""
+    sequence's new ones, a multiple of that; a tile may be taken along with the one before it), best with those first that see the most keys.  The rest as for ``attn_decode_kv8``."""
     if out.numel() != q.numel():
         raise Backend(f"attn_prefill_kv8: {tuple(out.shape)} for the results of queries {tuple(q.shape)}")
     if window is not None and window < 0:

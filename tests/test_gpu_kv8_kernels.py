@@ -505,6 +505,20 @@ def test_prefill_tiles_that_are_none():
 
 
 @pytest.mark.parametrize("hd", [64, 128, 192])
+@pytest.mark.parametrize("first", [5, 64, 129, 384, 2 ** 31 - 1])
+def test_prefill_tiles_between_the_tiles(hd, first):
+    """A tile that is none of its sequence's is left out, the others are as without it."""
+    nh, nkv, news, pasts = 2, 1, [300, 140], [100, 30]
+    table, k, v, exps, q, starts, tile_seq, tile_first = prefill_inputs(nh, nkv, hd, news, pasts, 8)
+    out, got, st = torch.empty_like(q), torch.full_like(q, 7), status()
+    ops.attn_prefill_kv8(q, k, v, exps, out, tile_seq, tile_first, ints(starts), ints(pasts), table, PAGE, nh, nkv, hd, 0, st)
+    assert st.item() == 0
+    ops.attn_prefill_kv8(q, k, v, exps, got, torch.cat((ints([0]), tile_seq)), torch.cat((ints([first]), tile_first)), ints(starts), ints(pasts), table, PAGE,
+                         nh, nkv, hd, 0, st)
+    assert st.item() == BAD_INDEX and torch.equal(got, out)
+
+
+@pytest.mark.parametrize("hd", [64, 128, 192])
 @pytest.mark.parametrize("starts", [[0, 150, 291], [0, 150, 2 ** 31 - 1], [0, -5, 140], [-20, 150, 290]])
 def test_prefill_rows_that_are_none(hd, starts):
     """Sequences whose rows the queries do not have are left out."""
