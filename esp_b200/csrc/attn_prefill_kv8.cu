@@ -6,9 +6,9 @@
 //                  product reads it as its A operand
 //   O += P V       tcgen05.mma, accumulated in tensor memory
 //
-// m is the row's running maximum, allowed to lag by 2^LAZY: O and the row's sum are rescaled only when it has outgrown that.
+// m is a whole number near the row's running maximum, which may have outgrown it by 2^LAZY: only then are O and the row's sum scaled anew.
 //
-// The cache's codes cannot be operands beside bfloat16 queries and weights, so four warps turn them into bfloat16 on their way
+// The cache's codes cannot be operands beside bfloat16 queries and weights, so eight warps turn them into bfloat16 on their way
 // from global to shared memory: a code's bits moved into a bfloat16's places are the code times 2^-120, subnormal codes
 // included, and one multiplication by 2^(120 + e) gives the number exactly.  That is four operations for two codes,
 // 2.4 with loads and stores for each, against about 3.5 of the row threads for each score.  A block of keys is therefore made
