@@ -1,5 +1,5 @@
 // Attention over the 8-bit paged cache (kv8.cuh), streaming: one new token of every sequence (decode), or sixteen new tokens of a
-// run (head sizes that the tensor-memory kernel does not take).
+// run (head sizes that the tensor-memory kernel does not take, and sequences of few new tokens).
 //
 //   s_j = q k_j / sqrt(hd),  o = sum_j 2^(s_j log2 e - m) v_j / sum_j 2^(s_j log2 e - m),  m = max_j s_j log2 e
 // over the keys max(0, pos - window + 1) <= j <= pos.
@@ -49,7 +49,7 @@ struct Params {
     const int *seq_past, *seq_start;           // per sequence (decode: seq_past may be null)
     const int *tile_seq, *tile_first;          // run: tiles of 128 new tokens
     const int* block_table;
-    int n_seqs, table_stride, n_pages, n_rows, nh, nkv, hd, window;      // n_seqs: rows of the page table; n_rows: of the queries
+    int n_seqs, table_stride, n_pages, n_rows, nh, nkv, hd, window, most;      // n_seqs: rows of the page table; n_rows: of the queries; run, most: new tokens of the sequences it takes
     float scale_log2;                          // log2(e) / sqrt(hd)
     int* status;
 };
@@ -376,6 +376,7 @@ __global__ void __launch_bounds__(THREADS) attn_run_kv8_kernel(const Params p) {
         if (threadIdx.x == 0 && first == tile_first) atomicOr(p.status, ESP_STATUS_BAD_INDEX);
         return;
     }
+    if (end - start > p.most) return;
     const int past = p.seq_past[seq], pos0 = past + first, k0 = first_visible_key(pos0, p.window, 0), k1 = pos0 + rows - 1;
     // rows that the queries do not have, or positions that the page table does not have
     if (start < 0 || end > p.n_rows || past < 0 || ((long long)past + first + rows - 1) / KV8_PAGE >= p.table_stride) {
@@ -756,14 +757,17 @@ ESP_API int esp_attn_decode_kv8(const void* q, const void* k, const void* v, con
     return 0;
 }
 
-// Runs of new tokens: tiles of 128 of a sequence (sequence, its first token among the sequence's new ones).  For heads of more
-// than 128 channels (esp_attn_prefill_kv8 has the others).
+// Runs of new tokens: tiles of 128 of a sequence (sequence, its first token among the sequence's new ones), of sequences with at
+// most ``most`` new tokens (0: of all).  Heads of 72 to 256 channels.
 ESP_API int esp_attn_run_kv8(const void* q, long long n_tokens, const void* k, const void* v, const void* exps, void* out, const int* tile_seq,
                              const int* tile_first, const int* seq_start, const int* seq_past, const int* block_table, int n_seqs, int table_stride,
-                             int n_pages, int n_tiles, int nh, int nkv, int hd, int window, int* status, cudaStream_t stream) {
+                             int n_pages, int n_tiles, int nh, int nkv, int hd, int window, int most, int* status, cudaStream_t stream) {
     if (n_tiles <= 0) return 0;
-    if (!sizes_fit(nh, nkv, hd) || hd <= 128 || window < 0 || n_tiles > (1 << 26) || n_tokens > 0x7fffffffLL) return (int)cudaErrorInvalidValue;
+    if (!sizes_fit(nh, nkv, hd) || hd <= 64 || window < 0 || n_tiles > (1 << 26) || n_tokens > 0x7fffffffLL) return (int)cudaErrorInvalidValue;
     Params p = make_params(q, k, v, exps, out, block_table, n_seqs, table_stride, n_pages, nh, nkv, hd, window, status);
     p.n_rows = (int)n_tokens, p.tile_seq = tile_seq, p.tile_first = tile_first, p.seq_start = seq_start, p.seq_past = seq_past;
+    p.most = most > 0 ? most : 0x7fffffff;
+    if (hd <= 96) return launch_run<96>(p, n_tiles, stream);
+    if (hd <= 128) return launch_run<128>(p, n_tiles, stream);
     return hd <= 192 ? launch_run<192>(p, n_tiles, stream) : launch_run<256>(p, n_tiles, stream);
 }

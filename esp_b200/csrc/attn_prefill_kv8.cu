@@ -52,7 +52,9 @@ struct Params {
     const unsigned char *k, *v, *exps;
     bf16* out;
     const int *tile_seq, *tile_first, *seq_start, *seq_past, *block_table;
-    int n_seqs, table_stride, n_pages, nh, nkv, hd, window, n_tiles, way, smem_bytes, n_tokens;
+    int n_seqs, table_stride, n_pages, nh, nkv, hd, window, n_tiles;
+    short way, least;                                   // shorts: an int more here and the compiler spills in the row threads' loop (2 %)
+    int smem_bytes, n_tokens;
     float scale_log2;
     int* status;
 };
@@ -269,11 +271,13 @@ __global__ void __launch_bounds__(THREADS, 1) attn_prefill_kv8_kernel(const __gr
                     fine = start >= 0 && end <= p.n_tokens && first < end - start && past >= 0 &&
                            ((long long)past + (end - start) - 1) / KV8_PAGE < p.table_stride;
                     const int pos = past + first, lo = first_visible_key(pos, p.window, 0) / BN, last = past + end - start - 1;
+                    if (!fine && blockIdx.x == 0) atomicOr(p.status, ESP_STATUS_BAD_INDEX);
+                    fine = fine && end - start >= p.least;               // the others are another kernel's
                     begins = fine && first / BM % 2 == 0;
                     goes_on = first + BM < end - start;
                     blocks = min(pos + BM - 1, last) / BN - lo + 1, both = min(pos + 2 * BM - 1, last) / BN - lo + 1;
                 }
-                if (!fine && blockIdx.x == 0) atomicOr(p.status, ESP_STATUS_BAD_INDEX);
+                else if (blockIdx.x == 0) atomicOr(p.status, ESP_STATUS_BAD_INDEX);
             }
             const unsigned below = (1u << lane) - 1u, mask = __ballot_sync(0xffffffffu, fine), mask2 = __ballot_sync(0xffffffffu, begins);
             if (fine && p.way != IN_PAIRS) {
@@ -842,7 +846,7 @@ template <int HD> int launch(const CUtensorMap& map_q, Params p, int device, cud
     // An item for each SM at most: singly.  Many: in pairs, and in all launches, as a tile is left to its neighbour, which another launch may
     // list.  Between the two the kernel looks at what the tiles see.
     const long long all_items = (long long)p.n_tiles * p.nh;
-    p.way = all_items <= sm_count[device] ? SINGLY : all_items >= 4LL * sm_count[device] || p.n_tiles > FEW ? IN_PAIRS : LOOK;
+    p.way = (short)(all_items <= sm_count[device] ? SINGLY : all_items >= 4LL * sm_count[device] || p.n_tiles > FEW ? IN_PAIRS : LOOK);
     for (int at = 0; at < p.n_tiles; at += LIST) {
         Params q = p;
         q.tile_seq += at, q.tile_first += at;
@@ -858,12 +862,13 @@ template <int HD> int launch(const CUtensorMap& map_q, Params p, int device, cud
 }  // namespace
 
 // q and out [n_tokens, nh, hd] bfloat16; tile_seq / tile_first: all tiles of 128 new tokens (sequence, the tile's first token among
-// the sequence's new ones, a multiple of 128), best listed with those that see the most keys first; hd a multiple of 8 up to 128.
+// the sequence's new ones, a multiple of 128), best listed with those that see the most keys first; of sequences with at least ``least``
+// new tokens; hd a multiple of 8 up to 128.
 ESP_API int esp_attn_prefill_kv8(const void* q, long long n_tokens, const void* k, const void* v, const void* exps, void* out, const int* tile_seq,
                                  const int* tile_first, const int* seq_start, const int* seq_past, const int* block_table, int n_seqs, int table_stride,
-                                 int n_pages, int n_tiles, int nh, int nkv, int hd, int window, int* status, cudaStream_t stream) {
+                                 int n_pages, int n_tiles, int nh, int nkv, int hd, int window, int least, int* status, cudaStream_t stream) {
     if (n_tiles <= 0 || n_tokens <= 0) return 0;
-    if (nkv <= 0 || nh <= 0 || nh % nkv || nh > 65535 || hd <= 0 || hd % 8 || hd > 128 || window < 0 || (long long)n_tiles * nh > 0x7fffffffLL || n_tokens > 0x7fffffffLL)
+    if (nkv <= 0 || nh <= 0 || nh % nkv || nh > 65535 || hd <= 0 || hd % 8 || hd > 128 || window < 0 || (long long)n_tiles * nh > 0x7fffffffLL || n_tokens > 0x7fffffffLL || least < 0 || least > BM)
         return (int)cudaErrorInvalidValue;
     int device = 0;
     if (cudaGetDevice(&device) != cudaSuccess || device < 0 || device >= 64) return (int)cudaErrorInvalidDevice;
@@ -874,7 +879,7 @@ ESP_API int esp_attn_prefill_kv8(const void* q, long long n_tokens, const void* 
     p.k = (const unsigned char*)k, p.v = (const unsigned char*)v, p.exps = (const unsigned char*)exps, p.out = (bf16*)out;
     p.tile_seq = tile_seq, p.tile_first = tile_first, p.seq_start = seq_start, p.seq_past = seq_past, p.block_table = block_table, p.n_seqs = n_seqs;
     p.table_stride = table_stride, p.n_pages = n_pages, p.nh = nh, p.nkv = nkv, p.hd = hd, p.window = window, p.n_tiles = n_tiles, p.status = status;
-    p.n_tokens = (int)n_tokens;
+    p.n_tokens = (int)n_tokens, p.least = (short)least;
     p.scale_log2 = (float)(1.4426950408889634 / sqrt((double)hd));
     if (hd <= 64) return launch<64>(map_q, p, device, stream);
     return launch<128>(map_q, p, device, stream);

@@ -113,8 +113,8 @@ _SIGNATURES = {
                              c_int, c_int, c_float, c_int, c_float, c_float, c_float, c_float, P, c_longlong, P, P],
     "esp_kv8_append": [P, P, P, P, P, P, c_int, c_int, P, P, P, P, P, c_int, c_int, c_int, c_int, c_int, c_int, c_int, c_int, P, P],
     "esp_attn_decode_kv8": [P, P, P, P, P, P, P, P, P, P, P, c_int, c_int, c_int, c_int, c_int, c_int, c_int, c_int, c_int, P, P],
-    "esp_attn_prefill_kv8": [P, c_longlong, P, P, P, P, P, P, P, P, P, c_int, c_int, c_int, c_int, c_int, c_int, c_int, c_int, P, P],
-    "esp_attn_run_kv8": [P, c_longlong, P, P, P, P, P, P, P, P, P, c_int, c_int, c_int, c_int, c_int, c_int, c_int, c_int, P, P],
+    "esp_attn_prefill_kv8": [P, c_longlong, P, P, P, P, P, P, P, P, P, c_int, c_int, c_int, c_int, c_int, c_int, c_int, c_int, c_int, P, P],
+    "esp_attn_run_kv8": [P, c_longlong, P, P, P, P, P, P, P, P, P, c_int, c_int, c_int, c_int, c_int, c_int, c_int, c_int, c_int, P, P],
 }
 
 _bound: dict = {}
@@ -1679,6 +1679,10 @@ def attn_decode_kv8(q, k, v, exps, out, ws, tok_seq, tok_pos, block_table, page,
         blocks, _ptr(status, torch.int32, "status"), _stream()), "attn_decode_kv8")
 
 
+# new tokens of the sequences that go to the streaming kernel
+KV8_FEW_TOKENS = 32
+
+
 def attn_prefill_kv8(q, k, v, exps, out, tile_seq, tile_first, seq_start, seq_past, block_table, page, nh, nkv, hd, window, status):
     """Causal attention of runs of new tokens, packed back to back, over the 8-bit cache that holds their own keys already:
     the step's rows seq_start[i] .. seq_start[i + 1] are sequence i's, behind seq_past[i] cached positions.  ``tile_seq`` and
@@ -1704,8 +1708,15 @@ def attn_prefill_kv8(q, k, v, exps, out, tile_seq, tile_first, seq_start, seq_pa
                     (("the queries", q), ("the keys", k), ("the values", v), ("the exponents", exps), ("the results", out)))
     rest = (k_, v_, e_, o_, _ptr(tile_seq, torch.int32, "tile_seq"), _ptr(tile_first, torch.int32, "tile_first"),
             _ptr(seq_start, torch.int32, "seq_start"), _ptr(seq_past, torch.int32, "seq_past"), _ptr(block_table, torch.int32, "page table"),
-            *block_table.shape, k.shape[0], n_tiles, nh, nkv, hd, _kv8_window(window, block_table, page), _ptr(status, torch.int32, "status"), _stream())
-    if hd <= 128:                      # scores and weighted values in tensor memory
-        _check(_fn("kv8", "esp_attn_prefill_kv8")(q_, n, *rest), "attn_prefill_kv8")
-    else:                              # the streaming kernel, sixteen rows a block
-        _check(_fn("kv8", "esp_attn_run_kv8")(q_, n, *rest), "attn_prefill_kv8")
+            *block_table.shape, k.shape[0], n_tiles, nh, nkv, hd, _kv8_window(window, block_table, page))
+    after = (_ptr(status, torch.int32, "status"), _stream())
+    # Scores and weighted values in tensor memory, or (wide heads) the streaming kernel, sixteen rows a block.  That one also takes
+    # the sequences of few new tokens, where tiles of 128 are mostly empty: 6 sequences behind 3,442 keys, 32 heads of 128 on 16, of 16
+    # new tokens 63 us for 108, of 32 95 for 110 (48 would take 112 for 111); 16 behind 2,000, 28 heads on 4, of 16 75 for 118, of 32 122
+    # for 118; heads of 64 gain nothing (19 and 18 us).  Steps whose tiles are half full on average are left to the first kernel
+    # as a whole.
+    few = KV8_FEW_TOKENS if 64 < hd <= 128 and n * 2 < n_tiles * ATTN_TC05_TILE_ROWS else 0
+    if hd <= 128 and (n > few or not few):
+        _check(_fn("kv8", "esp_attn_prefill_kv8")(q_, n, *rest, few + 1, *after), "attn_prefill_kv8")
+    if hd > 128 or few:
+        _check(_fn("kv8", "esp_attn_run_kv8")(q_, n, *rest, few, *after), "attn_prefill_kv8")

@@ -393,6 +393,12 @@ PREFILL = [
     (16, 8, 64, [2048], [0], 0),
     (7, 1, 128, [2500, 5, 1, 640], [100, 900, 0, 1], 0),
     (12, 3, 104, [1500, 300], [0, 700], 150),
+    # sequences of few new tokens among longer ones, and alone
+    (7, 1, 128, [300, 5, 32, 33, 1, 16, 17], [100, 3000, 64, 64, 700, 0, 127], 0),
+    (24, 8, 96, [16, 17, 2, 31], [700, 65, 0, 2000], 0),
+    (4, 2, 104, [32, 33, 1, 1, 1], [300, 300, 5, 64, 1000], 100),
+    (5, 5, 72, [9, 3], [1000, 0], 1),
+    (16, 4, 128, [1000, 7, 7, 7, 7, 7, 7, 7, 7, 7, 7, 7], [0] + [50 * i for i in range(11)], 0),
 ]
 
 
@@ -533,6 +539,30 @@ def test_prefill_rows_that_are_none(hd, starts):
         fine = 0 <= starts[i] < starts[i + 1] <= 290
         rows = slice(good[i], good[i + 1])
         assert torch.equal(got[rows], out[rows] if fine else torch.full_like(out[rows], 7))
+
+
+def test_prefill_bad_tiles_among_sequences_of_few_tokens():
+    """Both kernels that share such a call leave out what is none, and each writes the rows of its own sequences alone."""
+    nh, nkv, hd, news, pasts = 6, 2, 128, [130, 5, 40, 17, 3], [64, 700, 0, 300, 1]
+    table, k, v, exps, q, starts, tile_seq, tile_first = prefill_inputs(nh, nkv, hd, news, pasts, 8)
+    out, got, st = torch.empty_like(q), torch.full_like(q, 7), status()
+    ops.attn_prefill_kv8(q, k, v, exps, out, tile_seq, tile_first, ints(starts), ints(pasts), table, PAGE, nh, nkv, hd, 0, st)
+    assert st.item() == 0
+    check_prefill(out, q, k, v, exps, table, starts, pasts, nh, hd, 0)
+    for seqs, firsts in (([5], [0]), ([-1], [0]), ([1], [128]), ([0], [256]), ([4], [3])):
+        st.zero_(), got.fill_(7)
+        ops.attn_prefill_kv8(q, k, v, exps, got, torch.cat((ints(seqs), tile_seq)), torch.cat((ints(firsts), tile_first)), ints(starts), ints(pasts), table,
+                             PAGE, nh, nkv, hd, 0, st)
+        assert st.item() == BAD_INDEX and torch.equal(got, out)
+    # two sequences' pasts reach beyond the page table
+    st.zero_(), got.fill_(7)
+    far = list(pasts)
+    far[0] = far[3] = 64 * table.shape[1]
+    ops.attn_prefill_kv8(q, k, v, exps, got, tile_seq, tile_first, ints(starts), ints(far), table, PAGE, nh, nkv, hd, 0, st)
+    assert st.item() == BAD_INDEX
+    for i in range(5):
+        rows = slice(starts[i], starts[i + 1])
+        assert torch.equal(got[rows], torch.full_like(out[rows], 7) if i in (0, 3) else out[rows])
 
 
 @pytest.mark.parametrize("nh,hd", [(1, 64), (3, 128)])
