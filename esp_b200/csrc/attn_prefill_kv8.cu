@@ -28,9 +28,11 @@
 // A position that is no number (kv8.cuh) is made a key of NaN with a value of zeros: whoever sees it gets NaN through the score,
 // and a masked score takes nothing of it.
 //
-// Every wait is bounded, and a warp whose wait runs out leaves; the waits that hang on it then run out too.  (A flag that every
-// wait looks at first cost 8 of 291 us.)
+// Every wait is bounded, and a warp whose wait runs out leaves, row threads once they have been at the meetings where others would
+// wait for them without a limit (kv8_walk.cuh); the waits that hang on it then run out too.  (A flag that every wait looks at first
+// cost 8 of 291 us.)
 #include "kv8.cuh"
+#include "kv8_walk.cuh"
 #include "tc05.cuh"
 
 namespace {
@@ -618,17 +620,23 @@ __global__ void __launch_bounds__(THREADS, 1) attn_prefill_kv8_kernel(const __gr
         const float sc = p.scale_log2;
         const unsigned s_addr = tm_s + grp * BN + lane_sel + side * 64;
         const unsigned o_addr = tm_o + grp * BN + lane_sel;
-        bool ok = true;
         unsigned n_b = 0, ph_o = 0;                                       // blocks so far; a bit a group: the phase of its O
-        for (int round = 0; ok; round++) {
+        float m_ref, l_run;                                              // the maximum that O and l_run are scaled by
+        Item t;
+        auto open = [&](int round) {
             const int item = item_of(round);
-            if (item >= n_items) break;
-            const Item t = load_item(p, list, item);
+            if (item < n_items) t = load_item(p, list, item);
+            return item < n_items;
+        };
+        auto two_tiles = [&]() { return t.pair; };
+        auto meet = [&](bool across, bool ok) { return across ? all_agree(ok, bar_row, 128) : all_agree(ok, bar_grp, 64); };
+        auto work = [&]() {
+            bool ok = true;
             const int first_pos = t.pos0(grp), pos = first_pos + r;
             const int key_first = p.window > 0 ? pos - p.window + 1 : 0;             // may lie before the sequence's start
             const int key_first_last = p.window > 0 ? max(0, first_pos + BM - p.window) : 0;   // of the tile's last row
             const int j0 = t.pair ? t.lo(grp, p.window) : grp, j1 = t.pair ? t.hi(grp) : t.nb - 1, step = t.pair ? 1 : 2;
-            float m_ref = -INFINITY, l_run = 0.f;                                    // the maximum that O and l_run are scaled by
+            m_ref = -INFINITY, l_run = 0.f;
             for (int j = j0; j <= j1; j += step, n_b++) {
                 const int key0 = (t.blk0 + j) * BN;
                 ok = mbar_wait(&s_full[grp], n_b & 1);
@@ -730,16 +738,16 @@ __global__ void __launch_bounds__(THREADS, 1) attn_prefill_kv8_kernel(const __gr
                 __syncwarp();
                 if (lane == 0) mbar_arrive(&p_ready[grp]);
             }
-            if (!ok) break;
             // ---- the item's end: the sum of the row's threads; with one tile for both groups their results are joined
-            const bool both = !t.pair && t.nb > 1;
             xsum[(grp * 2 + side) * 128 + r] = l_run;
             if (side == 0) xref[grp * 128 + r] = m_ref;
             for (int g = 0; g < 2; g++)
                 if ((t.pair ? g == grp : g < t.nb) && ok) ok = !*abort_flag && mbar_wait(&o_full[g], ph_o >> g & 1);
             ph_o ^= t.pair || t.nb > 1 ? 3u : 1u;
-            ok = t.pair ? all_agree(ok, bar_grp, 64) : all_agree(ok, bar_row, 128);
-            if (!ok) break;
+            return ok;
+        };
+        auto finish = [&]() {
+            const bool both = !t.pair && t.nb > 1;
             tc_fence_after();
             // a group without a key for this row counts 0 (and a row that is no number stays one: 0 * NaN)
             const int g0 = t.pair ? grp : 0;
@@ -797,8 +805,8 @@ __global__ void __launch_bounds__(THREADS, 1) attn_prefill_kv8_kernel(const __gr
             if (t.pair) named_sync(bar_grp, 64);
             else named_sync(bar_row, 128);
             if (lane == 0 && (t.pair || grp < t.nb)) mbar_arrive(&o_free[grp]);
-        }
-        if (!ok && lane == 0) {
+        };
+        if (!kv8_walk_items(open, two_tiles, work, meet, finish) && lane == 0) {
             atomicOr(p.status, ESP_STATUS_WAIT_EXPIRED);
             *abort_flag = 1;
         }
