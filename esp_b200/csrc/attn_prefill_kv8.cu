@@ -25,6 +25,9 @@
 // same rows overlaps).  Spills cost more than anything else: beside 200 KB of shared memory they miss L1 (17 local loads a warp and
 // block: 393 us for 296).
 //
+// Keys of a page that is none have no weight, as in the streaming kernels: the row threads, each of which has the keys of one page of a
+// block, look it up where the item meets such a page.  A row without keys is zeros.
+//
 // A position that is no number (kv8.cuh) is made a key of NaN with a value of zeros: whoever sees it gets NaN through the score,
 // and a masked score takes nothing of it.
 //
@@ -204,6 +207,25 @@ __device__ __forceinline__ Item load_item(const Params& p, const unsigned short*
     t.blk0 = t.key_lo / BN;
     t.nb = t.key_hi / BN - t.blk0 + 1;
     return t;
+}
+
+// whether the sequence's page of position ``key`` is one; whether that of any of the positions lo .. hi is
+__device__ __forceinline__ bool has_page(const int* table, int table_stride, int n_pages, int seq, int key) {
+    const int i = key / KV8_PAGE, page = i < table_stride ? table[(size_t)seq * table_stride + i] : -1;
+    return page >= 0 && page < n_pages;
+}
+__device__ __noinline__ bool has_pages(const int* table, int table_stride, int n_pages, int seq, int lo, int hi) {
+    for (int i = lo / KV8_PAGE; i <= hi / KV8_PAGE; i++)
+        if (has_page(table, table_stride, n_pages, seq, i * KV8_PAGE)) return true;
+    return false;
+}
+
+// a warp: whether one of them is none
+__device__ __forceinline__ bool misses_page(const int* table, int table_stride, int n_pages, int seq, int lo, int hi, int lane) {
+    bool misses = false;
+#pragma unroll 4
+    for (int i = lo / KV8_PAGE + lane; i <= hi / KV8_PAGE; i += 32) misses |= !has_page(table, table_stride, n_pages, seq, i * KV8_PAGE);
+    return __any_sync(0xffffffffu, misses);
 }
 
 template <int HD>
@@ -634,9 +656,12 @@ __global__ void __launch_bounds__(THREADS, 1) attn_prefill_kv8_kernel(const __gr
             bool ok = true;
             const int first_pos = t.pos0(grp), pos = first_pos + r;
             const int key_first = p.window > 0 ? pos - p.window + 1 : 0;             // may lie before the sequence's start
-            const int key_first_last = p.window > 0 ? max(0, first_pos + BM - p.window) : 0;   // of the tile's last row
+            int key_first_last = p.window > 0 ? max(0, first_pos + BM - p.window) : 0;   // of the tile's last row
             const int j0 = t.pair ? t.lo(grp, p.window) : grp, j1 = t.pair ? t.hi(grp) : t.nb - 1, step = t.pair ? 1 : 2;
             m_ref = -INFINITY, l_run = 0.f;
+            // a page that is none among those of the item's keys (looked for while the first scores are on their way): all blocks are
+            // treated as those at an edge
+            if (misses_page(p.block_table, p.table_stride, p.n_pages, t.seq, t.key_lo, t.key_hi, lane)) key_first_last = INT_MAX;
             for (int j = j0; j <= j1; j += step, n_b++) {
                 const int key0 = (t.blk0 + j) * BN;
                 ok = mbar_wait(&s_full[grp], n_b & 1);
@@ -656,9 +681,13 @@ __global__ void __launch_bounds__(THREADS, 1) attn_prefill_kv8_kernel(const __gr
                     tc_ask32(s_addr + at, s);
                     tc_wait_ld(s);
                     if (edge) {
+                        // this thread's 64 keys are one page's: where it is none, no column
+                        const bool none = key_first_last == INT_MAX && !has_page(p.block_table, p.table_stride, p.n_pages, t.seq, key0 + side * 64);
+                        const int lo = none ? -1 : c_lo;
+                        const unsigned span = none ? 0u : c_span;
 #pragma unroll
                         for (int i = 0; i < 32; i++)
-                            if ((unsigned)(at + i - c_lo) > c_span) s[i] = 0xff800000u;
+                            if ((unsigned)(at + i - lo) > span) s[i] = 0xff800000u;
                     }
                     float m4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
@@ -757,7 +786,11 @@ __global__ void __launch_bounds__(THREADS, 1) attn_prefill_kv8_kernel(const __gr
             if (both) l += f1 * (xsum[256 + r] + xsum[384 + r]);
             // a row of one key: the weight as it was rounded, so that the result is its value
             if (p.window == 1 || t.pos0(0) + (t.pair ? grp * BM : 0) + r == 0) l = __bfloat162float(__float2bfloat16_rn(l));
-            const float inv = 1.f / l;                               // 0 where all scores are -inf (an infinite query): 0 * inf is NaN
+            float inv = 1.f / l;                                     // 0 where all scores are -inf (an infinite query): 0 * inf is NaN
+            if (l == 0.f) {                                          // ... or where the row has no key: zeros
+                const int pos = t.pos0(grp) + r;
+                if (!has_pages(p.block_table, p.table_stride, p.n_pages, t.seq, first_visible_key(pos, p.window, 0), pos)) inv = 0.f;
+            }
             // what this thread takes from tensor memory: 32 columns of its row at a time.  Four lanes then exchange their pieces of eight, so that
             // a store writes 64 bytes of each of eight rows (of 32 rows it would write 16: 5,000 cycles an item).
             const int cols = t.pair ? HD / 2 : 32, col0 = (t.pair ? side : grp * 2 + side) * cols;

@@ -493,6 +493,66 @@ def test_prefill_with_pages_that_are_none(hd):
     assert torch.equal(got[:150], out[:150]) and torch.isfinite(got).all()
 
 
+@pytest.mark.parametrize("nh,nkv,hd,news,pasts,window,missing", [
+    # missing: (sequence, page of it)
+    (4, 2, 128, [150, 150], [100, 30], 0, [(0, 1), (1, 0), (1, 2)]),
+    (4, 2, 64, [300, 129], [0, 64], 0, [(0, 0), (0, 3), (1, 1)]),
+    (2, 2, 104, [400], [100], 77, [(0, 2), (0, 3), (0, 6)]),
+    (32, 4, 64, [1300, 700], [0, 333], 0, [(0, 0), (0, 1), (0, 9), (1, 5)]),
+    (48, 16, 128, [1030, 400], [70, 0], 150, [(0, 4), (0, 5), (0, 6), (0, 7), (1, 2)]),
+    (2, 2, 192, [140, 40], [30, 0], 0, [(0, 1), (1, 0)]),
+    (7, 1, 128, [300, 5, 32], [100, 3000, 64], 0, [(0, 3), (1, 20), (2, 0), (2, 1)]),
+])
+def test_keys_of_pages_that_are_none_have_no_weight(nh, nkv, hd, news, pasts, window, missing):
+    """The same in prompts as in decode: a softmax over the keys that are there, zeros where there are none."""
+    table, k, v, exps, q, starts, tile_seq, tile_first = prefill_inputs(nh, nkv, hd, news, pasts, 17)
+    bad, st, ws = table.clone(), status(), Workspace(q.device)
+    for n, (i, page) in enumerate(missing):
+        bad[i, page] = [-1, k.shape[0], 2 ** 31 - 1][n % 3]
+    out, one = torch.full_like(q, math.nan), torch.full_like(q, math.nan)
+    ops.attn_prefill_kv8(q, k, v, exps, out, tile_seq, tile_first, ints(starts), ints(pasts), bad, PAGE, nh, nkv, hd, window, st)
+    assert st.item() == BAD_INDEX
+    seq = ints([i for i, t in enumerate(news) for _ in range(t)])
+    pos = ints([past + j for past, t in zip(pasts, news) for j in range(t)])
+    ops.attn_decode_kv8(q, k, v, exps, one, ws, seq, pos, bad, PAGE, nh, nkv, hd, window, st)
+    empty = 0
+    for i, past in enumerate(pasts):
+        a, b = starts[i], starts[i + 1]
+        length = past + b - a
+        pages = table[i, :(length + PAGE - 1) // PAGE].long()
+        kk, vv = (sequence_rows(p, exps, w, pages, length) for p, w in ((k, 0), (v, 1)))
+        qq = q[a:b].double().view(b - a, nh, hd)
+        at = torch.arange(past, length, device="cuda")
+        j = torch.arange(length, device="cuda")
+        sees = (j[None] <= at[:, None]) & ((at[:, None] - j[None] < window) if window else True)
+        for page in (page for s, page in missing if s == i):
+            sees = sees & (j // PAGE != page)[None]
+        score = torch.einsum("rhd,hld->rhl", qq, kk.repeat_interleave(nh // nkv, 0)) / math.sqrt(hd)
+        p = torch.nan_to_num(torch.softmax(torch.where(sees[:, None], score, -math.inf), -1))     # a row without keys: zeros
+        want, spread = (torch.einsum("rhl,hld->rhd", p, x.repeat_interleave(nh // nkv, 0)) for x in (vv, vv.abs()))
+        none = ~sees.any(-1)
+        empty += int(none.sum())
+        for got, step in ((out, 2.0 ** -8), (one, 2.0 ** -11)):
+            check_rows(got[a:b].double().view(b - a, nh, hd), want, spread, qq, kk, hd, step)
+            assert (got[a:b][none] == 0).all()
+    assert empty > 0
+
+
+def test_an_infinite_query_among_pages_that_are_none():
+    """All scores the lowest: NaN where the row has a key, zeros where it has none."""
+    nh, nkv, hd, news, pasts = 2, 1, 128, [200], [0]
+    table, k, v, exps, q, starts, tile_seq, tile_first = prefill_inputs(nh, nkv, hd, news, pasts, 6)
+    k.view(torch.uint8)[..., 5] = 0x38
+    q.view(-1, nh, hd)[[10, 70], 1, 5] = -math.inf
+    table[0, 0] = -1
+    out, st = torch.full_like(q, math.nan), status()
+    ops.attn_prefill_kv8(q, k, v, exps, out, tile_seq, tile_first, ints(starts), ints(pasts), table, PAGE, nh, nkv, hd, 0, st)
+    got = out.view(-1, nh, hd)
+    assert st.item() == BAD_INDEX and (got[:64] == 0)[:, 0].all() and torch.isnan(got[70, 1]).all() and (got[:10] == 0).all() and (got[11:64] == 0).all()
+    got[[10, 70], 1] = 0
+    assert torch.isfinite(got).all()
+
+
 def test_prefill_tiles_that_are_none():
     for hd in (128, 192):
         nh, nkv, news, pasts = 2, 1, [150, 140], [100, 30]
