@@ -371,18 +371,20 @@ __global__ void __launch_bounds__(THREADS) attn_run_kv8_kernel(const Params p) {
         if (threadIdx.x == 0) atomicOr(p.status, ESP_STATUS_BAD_INDEX);
         return;
     }
-    const int start = p.seq_start[seq], end = p.seq_start[seq + 1], rows = min(S::ROWS, end - start - first), head = blockIdx.y, kvh = head / (p.nh / p.nkv);
-    if (rows <= 0) {                           // behind the sequence's last token; a whole tile there is none
+    const int start = p.seq_start[seq], end = p.seq_start[seq + 1], past = p.seq_past[seq], head = blockIdx.y, kvh = head / (p.nh / p.nkv);
+    // rows that the queries do not have are looked for first: only where there are none is end - start a number of rows
+    const bool there = start >= 0 && end >= start && end <= p.n_rows;
+    const int rows = there ? min(S::ROWS, end - start - first) : 0;
+    if (rows <= 0) {                           // or behind the sequence's last token; a whole tile there is none
         if (threadIdx.x == 0 && first == tile_first) atomicOr(p.status, ESP_STATUS_BAD_INDEX);
         return;
     }
-    if (end - start > p.most) return;
-    const int past = p.seq_past[seq], pos0 = past + first, k0 = first_visible_key(pos0, p.window, 0), k1 = pos0 + rows - 1;
-    // rows that the queries do not have, or positions that the page table does not have
-    if (start < 0 || end > p.n_rows || past < 0 || ((long long)past + first + rows - 1) / KV8_PAGE >= p.table_stride) {
+    if (past < 0 || ((long long)past + first + rows - 1) / KV8_PAGE >= p.table_stride) {           // positions that the page table does not have
         if (threadIdx.x == 0) atomicOr(p.status, ESP_STATUS_BAD_INDEX);
         return;
     }
+    if (end - start > p.most) return;          // the tensor-memory kernel's
+    const int pos0 = past + first, k0 = first_visible_key(pos0, p.window, 0), k1 = pos0 + rows - 1;
     const long long row0 = (long long)(start + first) * p.nh + head;
     const int n_chunks = k1 / CHUNK - k0 / CHUNK + 1, mine = (n_chunks - warp + WARPS - 1) / WARPS;
     const int* pages = p.block_table + (size_t)seq * p.table_stride;

@@ -292,7 +292,7 @@ __global__ void __launch_bounds__(THREADS, 1) attn_prefill_kv8_kernel(const __gr
                 fine = seq >= 0 && seq < p.n_seqs && first >= 0 && first % BM == 0;
                 if (fine) {
                     const int start = p.seq_start[seq], end = p.seq_start[seq + 1], past = p.seq_past[seq];
-                    fine = start >= 0 && end <= p.n_tokens && first < end - start && past >= 0 &&
+                    fine = start >= 0 && end >= start && end <= p.n_tokens && first < end - start && past >= 0 &&
                            ((long long)past + (end - start) - 1) / KV8_PAGE < p.table_stride;
                     const int pos = past + first, lo = first_visible_key(pos, p.window, 0) / BN, last = past + end - start - 1;
                     if (!fine && blockIdx.x == 0) atomicOr(p.status, ESP_STATUS_BAD_INDEX);

@@ -601,6 +601,23 @@ def test_prefill_rows_that_are_none(hd, starts):
         assert torch.equal(got[rows], out[rows] if fine else torch.full_like(out[rows], 7))
 
 
+@pytest.mark.parametrize("hd", [64, 96, 128, 192])
+@pytest.mark.parametrize("news", [[150, 140], [14, 12]])
+@pytest.mark.parametrize("end", ["one more", 2 ** 31 - 1, -2 ** 31, -1, 3])
+def test_prefill_of_a_sequence_that_ends_nowhere(hd, news, end):
+    """The second sequence's end lies behind the queries or ahead of its start, also where their difference is no 32-bit number, and
+    also in calls that the streaming kernel has to itself (at most 32 rows): it is left out and the status says so."""
+    nh, nkv, pasts = 2, 1, [100, 30]
+    table, k, v, exps, q, good, tile_seq, tile_first = prefill_inputs(nh, nkv, hd, news, pasts, 8)
+    out, got, st = torch.empty_like(q), torch.full_like(q, 7), status()
+    ops.attn_prefill_kv8(q, k, v, exps, out, tile_seq, tile_first, ints(good), ints(pasts), table, PAGE, nh, nkv, hd, 0, st)
+    assert st.item() == 0
+    bad = [*good[:2], good[2] + 1 if end == "one more" else end]
+    ops.attn_prefill_kv8(q, k, v, exps, got, tile_seq, tile_first, ints(bad), ints(pasts), table, PAGE, nh, nkv, hd, 0, st)
+    assert st.item() == BAD_INDEX
+    assert torch.equal(got[:good[1]], out[:good[1]]) and (got[good[1]:] == 7).all()
+
+
 def test_prefill_bad_tiles_among_sequences_of_few_tokens():
     """Both kernels that share such a call leave out what is none, and each writes the rows of its own sequences alone."""
     nh, nkv, hd, news, pasts = 6, 2, 128, [130, 5, 40, 17, 3], [64, 700, 0, 300, 1]
