@@ -36,7 +36,7 @@
 
 namespace {
 constexpr int THREADS = 128, WARPS = 4, CHUNK = 32, UNIT = WARPS * CHUNK, MAX_ROWS = 1024;
-constexpr float WEIGHT_TOP = 6.f, LAG_TOP = 8.f, LAG_SUM = 40.f;
+constexpr float WEIGHT_TOP = 6.f, LAG_TOP = 8.f, LAG_SUM = 40.f, RISE = 60.f;
 constexpr int PARTS = 16;                      // of a pair, that one block joins
 
 struct Params {
@@ -315,6 +315,13 @@ template <int HD, int NT, bool RUN> struct Stream {
                 float sum = l[nt][j] * (m[nt][j] == -INFINITY ? 0.f : exp2_fast(m[nt][j] - most));
 #pragma unroll
                 for (int off = 4; off < 32; off <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, off);
+                // values of large exponents above a maximum that lags: the sums of weights times values would pass 32-bit's range, so
+                // the maximum is moved to where the sum of the weights is between 1 and 2
+                if (most > -INFINITY && top[nt][j] - WEIGHT_TOP - most > RISE && sum < INFINITY) {
+                    const int up = max((int)(__float_as_uint(sum) >> 23) - 127, 0);
+                    most += (float)up;
+                    sum *= kv8_pow2(-up);
+                }
                 const int r = nt * 8 + 2 * tg + j;
                 const float f = most == -INFINITY ? 1.f : exp2_fast(top[nt][j] - WEIGHT_TOP - most);
                 if (g8 == 0) {

@@ -52,6 +52,9 @@ constexpr int FEW = 1024;                               // tiles of a launch tha
 enum { SINGLY, IN_PAIRS, LOOK };                        // ways of a launch
 constexpr unsigned LIST_PAIR = 0x8000;                  // of a list's entry: the tile takes the next of its sequence along
 constexpr float LAZY = 8.f;
+// Values are taken times 2^-V_DOWN and results times 2^V_DOWN, so that sums of weights of up to 2^LAZY times values of up to 448 * 2^100
+// stay in 32-bit's range for 2^23 keys; a value's smallest code, 2^-109, still is a normal bfloat16.
+constexpr int V_DOWN = 12;
 
 struct Params {
     const unsigned char *k, *v, *exps;
@@ -558,8 +561,8 @@ __global__ void __launch_bounds__(THREADS, 1) attn_prefill_kv8_kernel(const __gr
 #pragma unroll
                 for (int i = 0; i < R; i++) {
                     const unsigned word = is_v ? ve : ke;
-                    // the byte of row i ^ odd, and 2^(120 + e) twice
-                    const unsigned f = ((odd ? word >> (8 * (i ^ 1)) : word >> (8 * i)) & 255u) * 0x00800080u + 0x3c003c00u;
+                    // the byte of row i ^ odd, and 2^(120 + e) twice (of values 2^(120 - V_DOWN + e))
+                    const unsigned f = ((odd ? word >> (8 * (i ^ 1)) : word >> (8 * i)) & 255u) * 0x00800080u + (120u - (is_v ? V_DOWN : 0)) * 0x00800080u;
                     const unsigned w[4] = {codes[i].x, codes[i].y, codes[i].z, codes[i].w};
                     unsigned o[8];
 #pragma unroll
@@ -577,7 +580,7 @@ __global__ void __launch_bounds__(THREADS, 1) attn_prefill_kv8_kernel(const __gr
                     const int r = i ^ odd;
                     const unsigned k8 = ke >> (8 * r) & 255u, v8 = ve >> (8 * r) & 255u;
                     const bool bad = (k8 == KV8_NAN || v8 == KV8_NAN) && r >= x.lo - row_lo && r < x.hi - row_lo;
-                    const int up = (int)(is_v ? v8 : k8) + 120, more = max(up - 254, 0);   // two factors
+                    const int up = (int)(is_v ? v8 : k8) + 120 - (is_v ? V_DOWN : 0), more = max(up - 254, 0);   // two factors
                     unsigned f = (unsigned)(up - more) << 7, f2 = (unsigned)(127 + more) << 7;
                     f = bad ? (is_v ? 0u : 0x7fffu) : f;                  // a key of NaN with a value of zeros
                     f2 = bad ? 0x3f80u : f2;
@@ -796,6 +799,7 @@ __global__ void __launch_bounds__(THREADS, 1) attn_prefill_kv8_kernel(const __gr
             const int cols = t.pair ? HD / 2 : 32, col0 = (t.pair ? side : grp * 2 + side) * cols;
             const unsigned from = t.pair ? o_addr : tm_o + lane_sel;
             const int row_g = t.pair ? grp * BM : 0, n_rows = t.rows(grp), piece = lane & 3;
+            inv *= (float)(1 << V_DOWN);
             f0 *= inv, f1 *= inv;
 #pragma unroll 1
             for (int col = col0; col < col0 + cols && col < HD; col += 32) {

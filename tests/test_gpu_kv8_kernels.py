@@ -479,6 +479,34 @@ def test_prefill_with_exponents_far_apart(hd, value_scale):
     check_prefill(out, q, k, v, exps, table, starts, pasts, nh, hd, 0)
 
 
+@pytest.mark.parametrize("nh,hd,rise", [(2, 128, 7.5), (2, 64, 7.5), (40, 128, 7.5), (2, 192, 37.8), (2, 128, 37.8), (12, 128, 37.8), (12, 64, 37.8)])
+def test_the_largest_values_behind_a_maximum_that_lags(nh, hd, rise):
+    """The first 256 values have the largest exponent, and the scores of 12,000 more lie ``rise`` (in units of log2) above theirs, just below
+    where a kernel would go over to a larger maximum (where that looks at weights times 2^exponent: with exponents 30 smaller).  Sums of
+    unnormalised weights times values pass 32-bit's range, the result does not."""
+    past, new, low = 12288 - 130, 130, 256
+    table, total = tables([past + new], 2)
+    k, v, exps = pools(total, 1, hd, 1)
+    k.view(torch.uint8).zero_()
+    k.view(torch.uint8)[..., 0] = 0x40                    # 2
+    first = table[0, :low // PAGE].long()
+    k.view(torch.uint8)[first] = 0
+    v.view(torch.uint8).fill_(0x7D)                       # 416
+    v.view(torch.uint8)[..., 1::2] = 0xFA                 # -320
+    exps[:, :, 0], exps[:, :, 1] = 127, 227 if rise < 8 else 197
+    exps[first, :, 1] = 227
+    q = torch.zeros((new, nh, hd), device="cuda")
+    q[..., 0] = rise / 2 * math.log(2) * math.sqrt(hd)
+    q = q.to(torch.bfloat16).view(new, -1)
+    out, one, st = torch.full_like(q, math.nan), torch.full_like(q, math.nan), status()
+    args = (table, PAGE, nh, 1, hd, 0, st)
+    ops.attn_prefill_kv8(q, k, v, exps, out, ints([0, 0]), ints([128, 0]), ints([0, new]), ints([past]), *args)
+    ops.attn_decode_kv8(q, k, v, exps, one, Workspace(q.device), ints([0] * new), torch.arange(past, past + new, dtype=torch.int32, device="cuda"), *args)
+    assert st.item() == 0
+    check_prefill(out, q, k, v, exps, table, [0, new], [past], nh, hd, 0)
+    check_prefill(one, q, k, v, exps, table, [0, new], [past], nh, hd, 0)
+
+
 @pytest.mark.parametrize("hd", [128, 192])
 def test_prefill_with_pages_that_are_none(hd):
     nh, nkv, news, pasts = 2, 1, [150, 150], [100, 30]
