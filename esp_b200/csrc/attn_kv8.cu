@@ -741,8 +741,10 @@ ESP_API int esp_attn_decode_kv8(const void* q, const void* k, const void* v, con
                                 const int* tok_seq, const int* tok_pos, const int* seq_past, const int* block_table, int n_seqs, int table_stride, int n_pages,
                                 int n_tokens, int nh, int nkv, int hd, int window, int blocks, int* status, cudaStream_t stream) {
     if (n_tokens <= 0) return 0;
-    if (!sizes_fit(nh, nkv, hd) || blocks <= 0 || window < 0 || table_stride <= 0 || table_stride > (1 << 25) || !parts || !counters)
+    if (!sizes_fit(nh, nkv, hd) || blocks <= 0 || window < 0 || table_stride <= 0 || table_stride >= (1 << 25) || !parts || !counters)
         return (int)cudaErrorInvalidValue;
+    // a launch's units are counted in 32 bits
+    if ((long long)(n_tokens < MAX_ROWS ? n_tokens : MAX_ROWS) * (table_stride / 2 + 1) > 0x7fffffffLL) return (int)cudaErrorInvalidValue;
     Params p = make_params(q, k, v, exps, out, block_table, n_seqs, table_stride, n_pages, nh, nkv, hd, window, status);
     p.parts = parts, p.counters = counters, p.seq_past = seq_past;
     // The query heads of a key head beyond eight: blocks of sixteen rows, or two of eight, whose keys come from L2 the second time.  Sixteen
@@ -772,7 +774,7 @@ ESP_API int esp_attn_run_kv8(const void* q, long long n_tokens, const void* k, c
                              const int* tile_first, const int* seq_start, const int* seq_past, const int* block_table, int n_seqs, int table_stride,
                              int n_pages, int n_tiles, int nh, int nkv, int hd, int window, int most, int* status, cudaStream_t stream) {
     if (n_tiles <= 0) return 0;
-    if (!sizes_fit(nh, nkv, hd) || hd <= 64 || window < 0 || n_tiles > (1 << 26) || n_tokens > 0x7fffffffLL) return (int)cudaErrorInvalidValue;
+    if (!sizes_fit(nh, nkv, hd) || hd <= 64 || window < 0 || table_stride >= (1 << 25) || n_tiles > (1 << 26) || n_tokens > 0x7fffffffLL) return (int)cudaErrorInvalidValue;
     Params p = make_params(q, k, v, exps, out, block_table, n_seqs, table_stride, n_pages, nh, nkv, hd, window, status);
     p.n_rows = (int)n_tokens, p.tile_seq = tile_seq, p.tile_first = tile_first, p.seq_start = seq_start, p.seq_past = seq_past;
     p.most = most > 0 ? most : 0x7fffffff;

@@ -913,7 +913,7 @@ ESP_API int esp_attn_prefill_kv8(const void* q, long long n_tokens, const void* 
                                  const int* tile_first, const int* seq_start, const int* seq_past, const int* block_table, int n_seqs, int table_stride,
                                  int n_pages, int n_tiles, int nh, int nkv, int hd, int window, int least, int* status, cudaStream_t stream) {
     if (n_tiles <= 0 || n_tokens <= 0) return 0;
-    if (nkv <= 0 || nh <= 0 || nh % nkv || nh > 65535 || hd <= 0 || hd % 8 || hd > 128 || window < 0 || (long long)n_tiles * nh > 0x7fffffffLL || n_tokens > 0x7fffffffLL || least < 0 || least > BM)
+    if (nkv <= 0 || nh <= 0 || nh % nkv || nh > 65535 || hd <= 0 || hd % 8 || hd > 128 || window < 0 || table_stride >= (1 << 25) || (long long)n_tiles * nh > 0x7fffffffLL || n_tokens > 0x7fffffffLL || least < 0 || least > BM)
         return (int)cudaErrorInvalidValue;
     int device = 0;
     if (cudaGetDevice(&device) != cudaSuccess || device < 0 || device >= 64) return (int)cudaErrorInvalidDevice;

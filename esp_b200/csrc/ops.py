@@ -1545,7 +1545,7 @@ def kv8_fits(hd: int, page: int = KV8_PAGE) -> bool:
 _current_device = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)
 
 
-def _kv8_refuse(what, q, k, v, exps, block_table, page, nh, nkv, hd, vectors, aligned):
+def _kv8_refuse(what, q, k, v, exps, block_table, page, nh, nkv, hd, vectors, aligned, rows=1):
     """Says what is wrong with a call that an entry point below did not let through (or with one whose tensors live elsewhere)."""
     if nh <= 0 or nkv <= 0 or nh % nkv or nh + 2 * nkv > 65535:
         raise Backend(f"{what}: {nh} query heads do not divide among {nkv} key/value heads")
@@ -1560,6 +1560,10 @@ def _kv8_refuse(what, q, k, v, exps, block_table, page, nh, nkv, hd, vectors, al
             raise Backend(f"{what}: exponents of shape {tuple(exps.shape)} are not [pages, {nkv}, 2, {page}]")
         if block_table.dim() != 2:
             raise Backend(f"{what}: the page table has {block_table.dim()} dimensions, not [sequences, pages]")
+        if not _kv8_counts_fit(1, block_table.shape[1]):
+            raise Backend(f"{what}: a page table of {block_table.shape[1]} pages a sequence; positions below 2^31 - {KV8_PAGE} have {KV8_MOST_PAGES}")
+        if not _kv8_counts_fit(rows, block_table.shape[1]):
+            raise Backend(f"{what}: {rows} rows of up to {block_table.shape[1]} pages; 2^38 keys are too many for a launch")
     for name, t, least in vectors:
         if t is not None and t.numel() < least:
             raise Backend(f"{what}: {name} has {t.numel()} elements, {least} are needed")
@@ -1576,6 +1580,15 @@ def _kv8_pools_fit(k, v, exps, block_table, page, nh, nkv, hd) -> bool:
     return (hd % 8 == 0 and 0 < hd <= 256 and page == KV8_PAGE and nkv > 0 < nh and nh % nkv == 0 and nh + 2 * nkv <= 65535 and len(shape) == 4
             and shape[1] == nkv and shape[2] == page and shape[3] == hd and v.shape == shape and exps.shape == (shape[0], nkv, 2, page)
             and block_table.dim() == 2)
+
+
+# pages that a sequence may have: the kernels count its positions, and one chunk more, in 32 bits
+KV8_MOST_PAGES = (1 << 25) - 1
+
+
+def _kv8_counts_fit(rows, pages) -> bool:
+    """Whether positions, and units of 128 keys of all of a launch's rows, are 32-bit numbers (decode: ``rows`` up to 1,024 at a time)."""
+    return pages <= KV8_MOST_PAGES and (rows if rows < 1024 else 1024) * (pages // 2 + 1) < 1 << 31
 
 
 def _kv8_window(window, block_table, page) -> int:
@@ -1664,12 +1677,12 @@ def attn_decode_kv8(q, k, v, exps, out, ws, tok_seq, tok_pos, block_table, page,
     if fits:
         q_, k_, v_, e_, o_ = (_ptr(q, _BF16, "q"), _ptr(k, _E4M3, "keys"), _ptr(v, _E4M3, "values"), _ptr(exps, torch.uint8, "exponents"),
                               _ptr(out, _BF16, "out"))
-        fits = not (q_ | k_ | v_ | e_ | o_) & 15
+        n_seqs, stride = block_table.shape
+        fits = not (q_ | k_ | v_ | e_ | o_) & 15 and _kv8_counts_fit(n, stride)
     if not fits:
         _kv8_refuse("attn_decode_kv8", q, k, v, exps, block_table, page, nh, nkv, hd,
                     (("tok_seq", tok_seq, n), ("tok_pos", tok_pos, n), ("seq_past", seq_past, block_table.shape[0])),
-                    (("the queries", q), ("the keys", k), ("the values", v), ("the exponents", exps), ("the results", out)))
-    n_seqs, stride = block_table.shape
+                    (("the queries", q), ("the keys", k), ("the values", v), ("the exponents", exps), ("the results", out)), n)
     blocks = ATTN_DECODE_KV8_BLOCKS_PER_SM[64 if hd <= 64 else 128 if hd <= 128 else 192 if hd <= 192 else 256] * _sm_count(_device_index)
     parts = _ptr(ws.get("attn_kv8_parts", (blocks * 32, hd + 2), _F32))
     counters = _ptr(ws.get("attn_kv8_counters", (min(n, 1024) * nh + 2 * blocks,), torch.int32, zeroed=True))
@@ -1700,7 +1713,8 @@ def attn_prefill_kv8(q, k, v, exps, out, tile_seq, tile_first, seq_start, seq_pa
     if fits:
         q_, k_, v_, e_, o_ = (_ptr(q, _BF16, "q"), _ptr(k, _E4M3, "keys"), _ptr(v, _E4M3, "values"), _ptr(exps, torch.uint8, "exponents"),
                               _ptr(out, _BF16, "out"))
-        fits = not (q_ | k_ | v_ | e_ | o_) & 15
+        n_seqs, stride = block_table.shape
+        fits = not (q_ | k_ | v_ | e_ | o_) & 15 and _kv8_counts_fit(1, stride)
     if not fits:
         _kv8_refuse("attn_prefill_kv8", q, k, v, exps, block_table, page, nh, nkv, hd,
                     (("tile_first", tile_first, n_tiles), ("seq_past", seq_past, block_table.shape[0]),
@@ -1708,7 +1722,7 @@ def attn_prefill_kv8(q, k, v, exps, out, tile_seq, tile_first, seq_start, seq_pa
                     (("the queries", q), ("the keys", k), ("the values", v), ("the exponents", exps), ("the results", out)))
     rest = (k_, v_, e_, o_, _ptr(tile_seq, torch.int32, "tile_seq"), _ptr(tile_first, torch.int32, "tile_first"),
             _ptr(seq_start, torch.int32, "seq_start"), _ptr(seq_past, torch.int32, "seq_past"), _ptr(block_table, torch.int32, "page table"),
-            *block_table.shape, k.shape[0], n_tiles, nh, nkv, hd, _kv8_window(window, block_table, page))
+            n_seqs, stride, k.shape[0], n_tiles, nh, nkv, hd, _kv8_window(window, block_table, page))
     after = (_ptr(status, torch.int32, "status"), _stream())
     # Scores and weighted values in tensor memory, or (wide heads) the streaming kernel, sixteen rows a block.  That one also takes
     # the sequences of few new tokens, where tiles of 128 are mostly empty: 6 sequences behind 3,442 keys, 32 heads of 128 on 16, of 16

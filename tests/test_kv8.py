@@ -77,6 +77,23 @@ def test_decode_refuses_short_lists():
         prefill({**a, "pos": torch.zeros(2, dtype=torch.int32)})
 
 
+def test_attention_refuses_tables_whose_positions_are_no_32_bit_numbers():
+    """2^25 pages hold 2^31 positions; 1,024 rows of 2^22 pages may see 2^38 keys."""
+    a = {**args(), "table": torch.zeros((1, 1 << 25), dtype=torch.int32)}
+    for call in (decode, prefill):
+        with pytest.raises(Backend, match="pages a sequence"):
+            call(a)
+    n = 1100
+    a = {**args(n=n), "table": torch.zeros((1, 1 << 22), dtype=torch.int32), "seq": torch.zeros(n, dtype=torch.int32), "pos": torch.zeros(n, dtype=torch.int32)}
+    with pytest.raises(Backend, match="too many for a launch"):
+        decode(a)
+    for table, rows in (((1 << 25) - 1, 3), ((1 << 22) - 4, n)):
+        a = {**args(n=rows), "table": torch.zeros((1, table), dtype=torch.int32), "seq": torch.zeros(rows, dtype=torch.int32),
+             "pos": torch.zeros(rows, dtype=torch.int32)}
+        with pytest.raises(Backend, match="no CPU path"):
+            decode(a)
+
+
 def append(**change):
     nh, nkv, hd, n = 4, 2, 64, 3
     a = dict(qkv=torch.zeros((n, (nh + 2 * nkv) * hd)), bias=None, seq=torch.zeros(n, dtype=torch.int32), pos=torch.zeros(n, dtype=torch.int32),
