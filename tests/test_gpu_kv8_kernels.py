@@ -132,6 +132,19 @@ def test_append(nh, nkv, hd, rot, news, pasts, with_bias):
     assert torch.equal(exps.permute(0, 3, 1, 2)[~touched], before[2].permute(0, 3, 1, 2)[~touched])
 
 
+@pytest.mark.parametrize("nh,nkv,hd,rot,news,pasts,with_bias", [
+    (6, 2, 80, 20, [9, 3], [62, 0], True),
+    (5, 5, 104, 100, [3], [127], True),
+    (3, 1, 256, 250, [5, 1], [60, 300], True),
+    (2, 2, 64, 2, [70], [1], False),
+    (7, 1, 128, 126, [300, 33], [0, 64], True),
+    (1, 1, 40, 34, [1], [0], True),
+])
+def test_append_of_rotations_that_are_no_multiple_of_eight(nh, nkv, hd, rot, news, pasts, with_bias):
+    """The kernel whose lanes hold every 32nd number: rotation partners in other slices, more heads than a block has warps."""
+    test_append(nh, nkv, hd, rot, news, pasts, with_bias)
+
+
 @pytest.mark.parametrize("hd,rot", [(128, 128), (128, 0), (80, 40), (256, 256), (64, 0)])
 def test_append_of_rows_at_the_borders(hd, rot):
     """Maxima at and beside 448 * 2^e, ties, subnormal codes, zeros, the smallest and largest exponents, rows that are no numbers.
@@ -777,6 +790,34 @@ def test_calls_on_two_streams_with_a_workspace_each():
                 ops.attn_decode_kv8(q, k, v, exps, out, ws, seq, pos, table, PAGE, nh, nkv, hd, 0, st)
     torch.cuda.synchronize()
     assert st.item() == 0 and torch.equal(outs[0], want) and torch.equal(outs[1], want)
+
+
+@pytest.mark.parametrize("nh,nkv,hd,news,pasts", [(8, 2, 128, [700, 300, 20], [300, 0, 900]), (32, 4, 64, [1300, 129], [0, 333]), (3, 3, 192, [200, 7], [90, 1000])])
+def test_prefill_beside_other_calls_on_streams_of_their_own(nh, nkv, hd, news, pasts):
+    """Prompts on two streams and decode on a third, over the same pools at once: the bits of calls behind one another."""
+    table, k, v, exps, q, starts, tile_seq, tile_first = prefill_inputs(nh, nkv, hd, news, pasts, 14)
+    st, n = status(), len(news)
+    seq, pos = torch.arange(n, dtype=torch.int32, device="cuda"), ints([a + b - 1 for a, b in zip(pasts, news)])
+    rows = torch.tensor([b - 1 for b in starts[1:]], device="cuda")
+    one_q = q[rows].contiguous()
+    args = (tile_seq, tile_first, ints(starts), ints(pasts), table, PAGE, nh, nkv, hd, 0, st)
+    spaces = [Workspace(q.device) for _ in range(3)]
+    calls = [lambda out, ws: ops.attn_prefill_kv8(q, k, v, exps, out, *args), lambda out, ws: ops.attn_prefill_kv8(q, k, v, exps, out, *args),
+             lambda out, ws: ops.attn_decode_kv8(one_q, k, v, exps, out, ws, seq, pos, table, PAGE, nh, nkv, hd, 0, st)]
+    streams, outs = [torch.cuda.Stream() for _ in calls], [torch.empty_like(q), torch.empty_like(q), torch.empty_like(one_q)]
+    wants = [torch.empty_like(x) for x in outs]
+    torch.cuda.synchronize()
+    for call, stream, want, ws in zip(calls, streams, wants, spaces):
+        with torch.cuda.stream(stream):
+            call(want, ws)
+        torch.cuda.synchronize()
+    for _ in range(20):
+        for call, stream, out, ws in zip(calls, streams, outs, spaces):
+            with torch.cuda.stream(stream):
+                call(out, ws)
+    torch.cuda.synchronize()
+    assert st.item() == 0 and all(torch.equal(a, b) for a, b in zip(outs, wants))
+    check_prefill(wants[0], q, k, v, exps, table, starts, pasts, nh, hd, 0)
 
 
 def test_a_first_call_is_not_captured():
