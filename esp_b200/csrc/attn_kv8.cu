@@ -749,10 +749,13 @@ ESP_API int esp_attn_decode_kv8(const void* q, const void* k, const void* v, con
     p.parts = parts, p.counters = counters, p.seq_past = seq_past;
     // The query heads of a key head beyond eight: blocks of sixteen rows, or two of eight, whose keys come from L2 the second time.  Sixteen
     // rows have twice as much to join and, in wide heads, spill; they win where a block has a long way to go (units a block by the
-    // page table's width, sixteen rows and eight: 48 heads on 4, 32 sequences of 2,000: 6.9 units, 29.3 and 31.3 us; 28 on 2 of 96
+    // page table's width, or by the window where that is less, sixteen rows and eight: 48 heads on 4, 32 sequences of 2,000: 6.9 units, 29.3 and 31.3 us; 28 on 2 of 96
     // channels, 20 of 8,000: 8.4, 30.9 and 36.1; 16 on 1, 20 of 8,000: 4.2, 28.6 and 24.9; 32 on 2, 8 of 4,096: 1.7, 24.0 and 17.5; of 64
-    // channels 20 of 8,000: 33.2 and 25.7; 48 on 4 of 256, 8 of 4,096: 56.2 and 40.6).
-    const bool wide = nh / nkv > 8 && (long long)n_tokens * nkv * table_stride * KV8_PAGE / UNIT > 5LL * blocks;
+    // channels 20 of 8,000: 33.2 and 25.7; 48 on 4 of 256, 8 of 4,096: 56.2 and 40.6; with windows 32 on 2, 64 that see 1,000: 3.4, 26.3 and 22.8;
+    // 48 on 4, 32 that see 512: 1.7, 22.6 and 17.7; 28 on 2 of 96 channels, 20 that see 2,000: 2.1, 17.7 and 18.7).
+    long long keys = (long long)table_stride * KV8_PAGE;
+    if (window > 0 && window < keys) keys = window;
+    const bool wide = nh / nkv > 8 && n_tokens * nkv * keys / UNIT > 5LL * blocks;
     for (int at = 0; at < n_tokens; at += MAX_ROWS) {                    // more rows than a block's list holds: one call behind the other
         p.n_rows = n_tokens - at < MAX_ROWS ? n_tokens - at : MAX_ROWS;
         p.tok_seq = tok_seq + at, p.tok_pos = tok_pos + at;

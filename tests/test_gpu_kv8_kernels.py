@@ -285,6 +285,17 @@ def test_decode(nh, nkv, hd, lengths, window):
     assert torch.equal(out, again)
 
 
+@pytest.mark.parametrize("nh,nkv,hd", [(28, 2, 72), (18, 2, 96), (32, 2, 104), (20, 2, 128)])
+@pytest.mark.parametrize("lengths,window", [([30000, 25001, 20000, 35000], 0), ([30000, 25001, 20000, 35000], 33333), ([9000, 1, 8000, 700] * 5, 500)])
+def test_decode_of_more_than_eight_heads_on_one(nh, nkv, hd, lengths, window):
+    """With far to go a block takes sixteen rows, with a short window eight, whatever the page table's width."""
+    table, k, v, exps, q, seq, pos = decode_inputs(nh, nkv, hd, lengths, 13)
+    out, st = torch.full_like(q, math.nan), status()
+    ops.attn_decode_kv8(q, k, v, exps, out, Workspace(q.device), seq, pos, table, PAGE, nh, nkv, hd, window, st)
+    assert st.item() == 0
+    check_decode(out, q, k, v, exps, table, lengths, nh, hd, window)
+
+
 @pytest.mark.parametrize("nh,nkv,hd", [(4, 4, 128), (12, 1, 64)])
 def test_decode_with_rows_that_are_no_numbers(nh, nkv, hd):
     """NaN where the mask hides it (behind the row, ahead of its window) changes nothing; where it is seen the row is NaN."""
