@@ -21,12 +21,13 @@
 //   * queries are scaled by a power of two that brings the row's largest to 2^14 (bfloat16's 8 bits fit a half's 11),
 //   * the weights 2^(s + e_v) have a running maximum M of their own, which may lag behind by 2^LAG_TOP; the largest weight lies
 //     between 2^WEIGHT_TOP and 2^(WEIGHT_TOP + LAG_TOP), and what is below 2^-20 of it is rounded to multiples of 2^-30 of it.
-// Sums, maxima and accumulators are 32-bit.
+// Sums, maxima and accumulators are 32-bit.  Weights and values far apart are held in this form; a warp leaves its result by the maximum of
+// the scores alone, which may lag by 2^LAG_SUM, and moves that where large values' sums would pass 32-bit's range.
 //
 // Measured (B200, one launch behind another): 8 sequences of 4,096 keys, 16 heads of 128, 30.5 us for 135 MB; 64 ragged ones of
 // up to 8,192, 28 heads on 4, 51 us for 231 MB; one of 131,071 34 us; one of 777 7.4 us.  The keys stream at the memory's rate
-// (18 of the 30 us); the rest is a block's start (2.7 us from the wait to its first chunk) and the joining of parts (about 4 us
-// a level: a fence, a count, two trips to L2).  A grid of (row, head, split) blocks of one split length took 29.4, 86, 42.5 and
+// (18 of the 30 us); of the rest a block's start takes 2.7 us (from the wait to its first chunk) and the joining of parts about 4 us
+// a level (a fence, a count, two trips to L2); about 5 us are not accounted for, as a block has 13 or 14 units.  A grid of (row, head, split) blocks of one split length took 29.4, 86, 42.5 and
 // 8.9 us, with the best length of each case 29.3, 60, 41 and 8.2.  Three blocks an SM with rings of two stages instead of two
 // with three: 33.4, 53.7, 37.4 and 7.7 us.
 // Heads are padded to 64, 96, 128, 192 or 256 channels (22 sequences of 7,411 keys, 5 heads of 80: 40.2 us in 96, 43.8 in 128; steps

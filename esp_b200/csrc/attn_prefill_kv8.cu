@@ -16,9 +16,10 @@
 // of its own, in all 512 columns of tensor memory.  Where there are few items, or a tile has no neighbour, the two groups
 // take the blocks of one tile in turn instead (SPLIT) and join their results.
 //
-// Measured (B200): 8,192 tokens, 16 heads of 128, 276 us = 1.0 PFLOP/s (the kernel for the bfloat16 cache: 335); five ragged chunks
-// of 500 to 1,500 tokens behind contexts of 1,500 to 4,600, 28 heads on 4, 390 us = 0.89.  A step of one block for both tiles takes about
-// 4,000 cycles, of which the tensor core needs 2,050 (counters: tensor pipe 48 %, issue slots 62 %, ALU 49 %, exponentials 50 %).  What
+// Measured (B200): 8,192 tokens, 16 heads of 128, 280 to 300 us in runs of 20 calls and 306 in long ones, whose clocks are lower (0.98 to
+// 0.90 PFLOP/s; the kernel for the bfloat16 cache 335 in short runs); five ragged chunks of 500 to 1,500 tokens behind contexts of
+// 1,500 to 4,600, 28 heads on 4, 395 and 415 us (0.88, 0.84).  A step of one block for both tiles takes about
+// 4,000 cycles, of which the tensor core needs 2,050 (counters: tensor pipe 48 %, issue slots 63 %, ALU 49 %, exponentials 50 %).  What
 // bounds it are the converting warps (their loads and stores share shared memory's 128 bytes a cycle with the MMAs' operands, their
 // instructions the issue slots with the row threads) and, close behind, a group's chain: scores, weights and meeting 2,200 cycles, then
 // P V and the next scores 1,024.  An item costs about 5 us besides (its first and last products and its results, which nothing of the
@@ -889,7 +890,9 @@ template <int HD> int launch(const CUtensorMap& map_q, Params p, int device, cud
     }
     p.smem_bytes = (int)smem;
     // An item for each SM at most: singly.  Many: in pairs, and in all launches, as a tile is left to its neighbour, which another launch may
-    // list.  Between the two the kernel looks at what the tiles see.
+    // list.  Between the two the kernel looks at what the tiles see.  Tiles of sequences of few new tokens count although another kernel has
+    // them: looking there as well costs more than it gains (2,048 tokens beside 100 of one, 28 heads on 4, 252 us and 259 with a
+    // look; 700 behind 4,953 beside 60 of four, 32 on 8, 211 and 216; 100 of 33 beside 60 of one 214 and 233).
     const long long all_items = (long long)p.n_tiles * p.nh;
     p.way = (short)(all_items <= sm_count[device] ? SINGLY : all_items >= 4LL * sm_count[device] || p.n_tiles > FEW ? IN_PAIRS : LOOK);
     for (int at = 0; at < p.n_tiles; at += LIST) {

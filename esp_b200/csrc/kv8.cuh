@@ -9,6 +9,7 @@
 // 2^e is a bfloat16 number, so a kernel may work on codes and exponents or on bfloat16 and means the same.
 // A row that holds a NaN, an infinity or a magnitude above 448 * 2^KV8_HIGHEST is stored as codes 0 and the byte KV8_NAN:
 // whoever sees such a position gets NaN, whoever's mask hides it gets nothing of it.
+// Where a sequence's table names no page, attention gives the page's keys no weight (a row without keys is zeros) and the status says so.
 #pragma once
 #include "common.cuh"
 

@@ -8,9 +8,10 @@
 // Columns at or beyond ``rot`` pass through.  A row's exponent comes from its rotated numbers in 32-bit, so a key is rounded
 // once, not to bfloat16 first.
 //
-// Bound by memory where there are many tokens (4 bytes read for every one or two written) and by its launch where there are
-// few.  A row's lanes hold all of its numbers in registers, so the maximum and the rounding need no second pass.  Measured
-// (B200): 8,192 tokens of 48 heads of 128 59 us for 273 MB (4.6 TB/s; a number a lane 300 us), one token 2 to 3 us.
+// Bound by its launch where there are few tokens, and where there are many by its instructions and by how little it has on its way: short
+// blocks that look up position and page first, 73 % of the issue slots.  It is not at the memory's rate, which a copy of as much
+// reading as writing shows to be 6.5 TB/s.  A row's lanes hold all of its numbers in registers, so the maximum and the rounding need no
+// second pass.  Measured (B200): 8,192 tokens of 48 heads of 128 60 us for 273 MB (4.5 TB/s; a number a lane 300 us), one token 2 to 3 us.
 #include "kv8.cuh"
 
 namespace {

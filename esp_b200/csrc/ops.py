@@ -1659,12 +1659,15 @@ ATTN_DECODE_KV8_BLOCKS_PER_SM = {64: 3, 128: 2, 192: 2, 256: 1}
 def attn_decode_kv8(q, k, v, exps, out, ws, tok_seq, tok_pos, block_table, page, nh, nkv, hd, window, status, seq_past=None):
     """Attention of one token row per sequence (or of any rows, each on its own) over the 8-bit cache, the keys of all rows
     dealt out evenly over the device: scores over sqrt(hd), keys max(0, pos - window + 1) .. pos (``window`` None or 0: all).  q and out bfloat16 [N, nh * hd];
-    query head i reads key/value head i // (nh / nkv).  ``ws``: the ``Workspace`` that holds the scratch; calls that may
+    query head i reads key/value head i // (nh / nkv).  Keys of a page that is none have no weight, a row without keys is zeros, one whose
+    position the page table does not have is left as it was, and the status says so.  ``ws``: the ``Workspace`` that holds the scratch; calls that may
     overlap on the device (other streams, captured graphs replayed beside each other) need one each.  A call that is to be
     captured is made once before, and its graph holds ``ws``'s buffers: capture again once ``ws.generation`` has moved on, or
     set ``ws.frozen``.  ``seq_past``
     (int32 per sequence of the step: positions that were cached before the step's copies to the device): blocks whose
-    keys are all older load them without waiting for the kernel before this one."""
+    keys are all older load them without waiting for the kernel before this one.  ``tok_seq``, ``tok_pos``, ``seq_past`` and the page
+    table are read ahead of that wait in any case: the step's copies to the device write them, or work that has ended, not a
+    kernel that may still run."""
     n = q.shape[0]
     if out.numel() != q.numel():
         raise Backend(f"attn_decode_kv8: {tuple(out.shape)} for the results of queries {tuple(q.shape)}")
@@ -1700,7 +1703,8 @@ def attn_prefill_kv8(q, k, v, exps, out, tile_seq, tile_first, seq_start, seq_pa
     """Causal attention of runs of new tokens, packed back to back, over the 8-bit cache that holds their own keys already:
     the step's rows seq_start[i] .. seq_start[i + 1] are sequence i's, behind seq_past[i] cached positions.  ``tile_seq`` and
     ``tile_first``: all tiles of ATTN_TC05_TILE_ROWS new tokens (sequence, index of the tile's first token among the
-    sequence's new ones, a multiple of that; a tile may be taken along with the one before it), best with those first that see the most keys.  The rest as for ``attn_decode_kv8``."""
+    sequence's new ones, a multiple of that; a tile may be taken along with the one before it), best with those first that see the most keys.  Whether tiles go singly or in pairs, and with it a row's last bits, follows from
+    all of the call's tiles.  The rest as for ``attn_decode_kv8``."""
     if out.numel() != q.numel():
         raise Backend(f"attn_prefill_kv8: {tuple(out.shape)} for the results of queries {tuple(q.shape)}")
     if window is not None and window < 0:
@@ -1727,7 +1731,7 @@ def attn_prefill_kv8(q, k, v, exps, out, tile_seq, tile_first, seq_start, seq_pa
     # Scores and weighted values in tensor memory, or (wide heads) the streaming kernel, sixteen rows a block.  That one also takes
     # the sequences of few new tokens, where tiles of 128 are mostly empty: 6 sequences behind 3,442 keys, 32 heads of 128 on 16, of 16
     # new tokens 63 us for 108, of 32 95 for 110 (48 would take 112 for 111); 16 behind 2,000, 28 heads on 4, of 16 75 for 118, of 32 122
-    # for 118; heads of 64 gain nothing (19 and 18 us).  Steps whose tiles are half full on average are left to the first kernel
+    # for 118; heads of 64 gain nothing (19 and 18 us).  (The engine sends steps of at most 128 rows to the decode kernel as a whole.)  Steps whose tiles are half full on average are left to the first kernel
     # as a whole.
     few = KV8_FEW_TOKENS if 64 < hd <= 128 and n * 2 < n_tiles * ATTN_TC05_TILE_ROWS else 0
     if hd <= 128 and (n > few or not few):
