@@ -880,6 +880,81 @@ def test_append_then_attend_is_a_captured_step():
             check_decode(out, q, k, v, exps, table, now, nh, hd, 0)
 
 
+@pytest.mark.parametrize("nh,nkv,hd", [(8, 2, 128), (4, 4, 64), (2, 1, 192)])
+def test_a_captured_prompt_over_changing_inputs(nh, nkv, hd):
+    """Append and attention of many tokens in a graph, replayed over other numbers, pages, lengths and cached positions of as many rows."""
+    n, width, longest = 260, (nh + 2 * nkv) * hd, 700
+    k, v, exps = pools(40, nkv, hd, 2)
+    angle = torch.arange(longest, device="cuda")[:, None] * 1e4 ** (-torch.arange(hd // 2, device="cuda") / (hd // 2))
+    cos, sin = angle.cos().contiguous(), angle.sin().contiguous()
+    qkv, q = torch.empty((n, width), device="cuda"), torch.empty((n, nh * hd), dtype=torch.bfloat16, device="cuda")
+    out, st = torch.empty_like(q), status()
+    # three tiles either way: 200 and 60 new tokens, or 20 and 240
+    lists = {name: torch.zeros(size, dtype=torch.int32, device="cuda") for name, size in
+             (("seq", n), ("pos", n), ("tile_seq", 3), ("tile_first", 3), ("start", 3), ("past", 2))}
+    table = torch.zeros((2, longest // PAGE + 1), dtype=torch.int32, device="cuda")
+
+    def fill(news, pasts, seed):
+        starts = [0, news[0], n]
+        for name, what in (("seq", [i for i, t in enumerate(news) for _ in range(t)]), ("pos", [p + j for p, t in zip(pasts, news) for j in range(t)]),
+                           ("tile_seq", [i for i, t in enumerate(news) for _ in range(0, t, 128)]),
+                           ("tile_first", [f for t in news for f in range(0, t, 128)]), ("start", starts), ("past", pasts)):
+            lists[name].copy_(ints(what))
+        table.copy_(torch.randperm(40, generator=torch.Generator().manual_seed(seed))[:table.numel()].to(torch.int32).view_as(table))
+        qkv.normal_()
+        return starts
+
+    def step():
+        ops.kv8_rope_append(qkv, None, lists["seq"], lists["pos"], cos, sin, hd, q, k, v, exps, table, PAGE, nh, nkv, hd, True, st)
+        ops.attn_prefill_kv8(q, k, v, exps, out, lists["tile_seq"], lists["tile_first"], lists["start"], lists["past"], table, PAGE, nh, nkv, hd, 0, st)
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        fill([200, 60], [0, 100], 1)
+        step()
+        side.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=side):
+            step()
+        for i, (news, pasts) in enumerate([([200, 60], [300, 5]), ([20, 240], [500, 0]), ([240, 20], [1, 640])]):
+            starts = fill(news, pasts, i)
+            out.fill_(math.nan)
+            graph.replay()
+            side.synchronize()
+            assert st.item() == 0
+            check_prefill(out, q, k, v, exps, table, starts, pasts, nh, hd, 0)
+    del graph
+
+
+@pytest.mark.parametrize("nh,nkv,hd,news,pasts", [(2, 1, 128, [150, 20], [0, 70]), (16, 16, 64, [1500, 300], [0, 5]), (2, 2, 192, [40, 17], [9, 0]), (2, 1, 96, [9, 2], [0, 70])])
+def test_rows_behind_the_last_sequence_and_tiles_listed_twice(nh, nkv, hd, news, pasts):
+    table, k, v, exps, q, starts, tile_seq, tile_first = prefill_inputs(nh, nkv, hd, news, pasts, 3)
+    want, st = torch.empty_like(q), status()
+    ops.attn_prefill_kv8(q, k, v, exps, want, tile_seq, tile_first, ints(starts), ints(pasts), table, PAGE, nh, nkv, hd, 0, st)
+    padded = torch.cat((q, torch.full_like(q[:50], math.nan)))
+    out = torch.full_like(padded, 7)
+    ops.attn_prefill_kv8(padded, k, v, exps, out, torch.cat((tile_seq, tile_seq)), torch.cat((tile_first, tile_first)), ints(starts), ints(pasts), table, PAGE,
+                         nh, nkv, hd, 0, st)
+    assert st.item() == 0 and (out[starts[-1]:] == 7).all()
+    check_prefill(out, q, k, v, exps, table, starts, pasts, nh, hd, 0)
+    check_prefill(want, q, k, v, exps, table, starts, pasts, nh, hd, 0)
+
+
+@pytest.mark.parametrize("nh,nkv,hd", [(2, 1, 8), (200, 1, 64), (130, 2, 96), (1, 1, 136)])
+def test_the_smallest_heads_and_the_most_of_them(nh, nkv, hd):
+    news, pasts = [140, 3], [10, 129]
+    table, k, v, exps, q, starts, tile_seq, tile_first = prefill_inputs(nh, nkv, hd, news, pasts, 12)
+    out, one, st = torch.full_like(q, math.nan), torch.full_like(q, math.nan), status()
+    ops.attn_prefill_kv8(q, k, v, exps, out, tile_seq, tile_first, ints(starts), ints(pasts), table, PAGE, nh, nkv, hd, 0, st)
+    seq = ints([i for i, t in enumerate(news) for _ in range(t)])
+    pos = ints([past + j for past, t in zip(pasts, news) for j in range(t)])
+    ops.attn_decode_kv8(q, k, v, exps, one, Workspace(q.device), seq, pos, table, PAGE, nh, nkv, hd, 0, st)
+    assert st.item() == 0
+    check_prefill(out, q, k, v, exps, table, starts, pasts, nh, hd, 0)
+    check_prefill(one, q, k, v, exps, table, starts, pasts, nh, hd, 0)
+
+
 def test_prefill_and_decode_agree():
     """The last row of a run sees what a decode step at its place sees."""
     for hd, weight in ((128, 2.0 ** -8), (192, 2.0 ** -11)):
