@@ -27,9 +27,9 @@
 // Measured (B200, one launch behind another): 8 sequences of 4,096 keys, 16 heads of 128, 30.5 us for 135 MB; 64 ragged ones of
 // up to 8,192, 28 heads on 4, 51 us for 231 MB; one of 131,071 34 us; one of 777 7.4 us.  The keys stream at the memory's rate
 // (18 of the 30 us); of the rest a block's start takes 2.7 us (from the wait to its first chunk) and the joining of parts about 4 us
-// a level (a fence, a count, two trips to L2); about 5 us are not accounted for, as a block has 13 or 14 units.  A grid of (row, head, split) blocks of one split length took 29.4, 86, 42.5 and
-// 8.9 us, with the best length of each case 29.3, 60, 41 and 8.2.  Three blocks an SM with rings of two stages instead of two
-// with three: 33.4, 53.7, 37.4 and 7.7 us.
+// a level (a fence, a count, two trips to L2); about 5 us are not accounted for, as every block has 13 or 14 units.  A grid of (row, head,
+// split) blocks of one split length took 29.4, 86, 42.5 and 8.9 us, with the best length of each case 29.3, 60, 41 and 8.2.  Three blocks an
+// SM with rings of two stages instead of two with three: 33.4, 53.7, 37.4 and 7.7 us.
 // Heads are padded to 64, 96, 128, 192 or 256 channels (22 sequences of 7,411 keys, 5 heads of 80: 40.2 us in 96, 43.8 in 128; steps
 // over channels that are not there left out at run time instead: 49, as the branches keep the loads of one step from the products of
 // the last.  8 sequences of 4,096, 16 heads of 192: 43.7 us in 192, where two blocks fit an SM, 58 in 256).
@@ -317,7 +317,8 @@ template <int HD, int NT, bool RUN> struct Stream {
 #pragma unroll
                 for (int off = 4; off < 32; off <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, off);
                 // values of large exponents above a maximum that lags: the sums of weights times values would pass 32-bit's range, so
-                // the maximum is moved to where the sum of the weights is between 1 and 2
+                // the maximum is moved to where the sum of the weights is between 1 and 2.  (Up to 2^RISE they are in it: o stays below
+                // 2^14 * 448 * 2^24 keys.)
                 if (most > -INFINITY && top[nt][j] - WEIGHT_TOP - most > RISE && sum < INFINITY) {
                     const int up = max((int)(__float_as_uint(sum) >> 23) - 127, 0);
                     most += (float)up;
@@ -756,7 +757,7 @@ ESP_API int esp_attn_decode_kv8(const void* q, const void* k, const void* v, con
     // 48 on 4, 32 that see 512: 1.7, 22.6 and 17.7; 28 on 2 of 96 channels, 20 that see 2,000: 2.1, 17.7 and 18.7).
     long long keys = (long long)table_stride * KV8_PAGE;
     if (window > 0 && window < keys) keys = window;
-    const bool wide = nh / nkv > 8 && n_tokens * nkv * keys / UNIT > 5LL * blocks;
+    const bool wide = nh / nkv > 8 && (long long)n_tokens * nkv * keys / UNIT > 5LL * blocks;
     for (int at = 0; at < n_tokens; at += MAX_ROWS) {                    // more rows than a block's list holds: one call behind the other
         p.n_rows = n_tokens - at < MAX_ROWS ? n_tokens - at : MAX_ROWS;
         p.tok_seq = tok_seq + at, p.tok_pos = tok_pos + at;
