@@ -38,6 +38,11 @@
 namespace {
 constexpr int THREADS = 128, WARPS = 4, CHUNK = 32, UNIT = WARPS * CHUNK, MAX_ROWS = 1024;
 constexpr float WEIGHT_TOP = 6.f, LAG_TOP = 8.f, LAG_SUM = 40.f, RISE = 60.f;
+// A value's exponent is added to its score, and above 2^24 a score has no place for it: scores whose maximum is this far from zero, or from the
+// base they are counted from, are counted from that maximum.  (The place where that is looked for and done is seldom come to, but costs what it
+// takes of registers and instructions: decode up to 1 %, sequences of few new tokens 2 %.  Scores counted from the row's maximum throughout,
+// without a base: decode with sixteen rows a block 4 to 7 %, few new tokens 3 %.)
+constexpr float FROM_ZERO = 1 << 20, FROM_BASE = 32.f;
 constexpr int PARTS = 16;                      // of a pair, that one block joins
 
 struct Params {
@@ -117,6 +122,7 @@ template <int HD, int NT, bool RUN> struct Stream {
     float row_scale[NT][2];
     float o[NT][HD / 16][4], top[NT][2];       // top: M, of the row
     float m[NT][2], l[NT][2];                  // maximum (lagging by LAG_SUM) and sum of the lane's own keys
+    float base[NT][2];                         // of the row: what its scores, m and top are counted from
 
     // asks for the chunk of keys key0 .. key0 + 31 in page ``page``; those outside [k0, k1] are filled with zeros
     static __device__ __forceinline__ void ask(const Params& p, unsigned char* st, int page, int kvh, int key0, int k0, int k1, int lane) {
@@ -184,8 +190,9 @@ template <int HD, int NT, bool RUN> struct Stream {
             }
             // a lane's scores belong to rows 2 tg and 2 tg + 1, whose queries the lanes 8 tg and 8 tg + 4 hold
             const int xa = __shfl_sync(0xffffffffu, x, tg * 8), xb = __shfl_sync(0xffffffffu, x, tg * 8 + 4);
-            row_scale[nt][0] = kv8_pow2(min(xa - 14, 127)) * scale_log2;
-            row_scale[nt][1] = kv8_pow2(min(xb - 14, 127)) * scale_log2;
+            // times 2^16, and a key's factor by 2^-16: neither product passes 32-bit's range unless the score does
+            row_scale[nt][0] = kv8_pow2(min(xa - 14, 127)) * (scale_log2 * 65536.f);
+            row_scale[nt][1] = kv8_pow2(min(xb - 14, 127)) * (scale_log2 * 65536.f);
 #pragma unroll
             for (int i = 0; i < HD / 16; i++)
 #pragma unroll
@@ -193,7 +200,32 @@ template <int HD, int NT, bool RUN> struct Stream {
 #pragma unroll
             for (int j = 0; j < 2; j++) {
                 m[nt][j] = top[nt][j] = -INFINITY;
-                l[nt][j] = 0.f;
+                l[nt][j] = base[nt][j] = 0.f;
+            }
+        }
+    }
+
+    // Scores far from zero: counted from the rows' bases (as they are rounded: equal ones stay equal), which are moved to the rows' maxima where
+    // those have gone away from them.
+    __device__ __forceinline__ void rebase(int nt, float (&s)[NT][2][4], float (&t)[4][2], float (&cm)[2], float (&ct)[2], const float (&ve)[4]) {
+#pragma unroll
+        for (int j = 0; j < 2; j++) {
+            cm[j] = ct[j] = -INFINITY;
+#pragma unroll
+            for (int u = 0; u < 4; u++) cm[j] = fmaxf(cm[j], s[nt][u >> 1][(u & 1) * 2 + j] -= base[nt][j]);
+            float row = fmaxf(m[nt][j], cm[j]), d = 0.f;
+#pragma unroll
+            for (int off = 4; off < 32; off <<= 1) row = fmaxf(row, __shfl_xor_sync(0xffffffffu, row, off));
+            if (fabsf(row) > (base[nt][j] == 0.f ? FROM_ZERO : FROM_BASE) && fabsf(row) < INFINITY) {
+                const float now = base[nt][j] + rintf(row);
+                d = now - base[nt][j];
+                base[nt][j] = now;
+            }
+            m[nt][j] -= d, top[nt][j] -= d, cm[j] -= d;
+#pragma unroll
+            for (int u = 0; u < 4; u++) {
+                t[u][j] = (s[nt][u >> 1][(u & 1) * 2 + j] -= d) + ve[u];
+                ct[j] = fmaxf(ct[j], t[u][j]);
             }
         }
     }
@@ -234,7 +266,7 @@ template <int HD, int NT, bool RUN> struct Stream {
         for (int u = 0; u < 4; u++) {
             const int key = key0 + u * 8 + g8, ke = e_src[u * 8 + g8], vb = e_src[CHUNK + u * 8 + g8];
             seen[u] = key >= k0 && key <= k1 && ke != 0;                  // a stored exponent is never 0: the page was not one
-            kf[u] = ke == KV8_NAN || vb == KV8_NAN ? __int_as_float(0x7fffffff) : __uint_as_float((unsigned)ke << 23);
+            kf[u] = ke == KV8_NAN || vb == KV8_NAN ? __int_as_float(0x7fffffff) : __uint_as_float((unsigned)(ke - 16) << 23);
             ve[u] = (float)(vb - 127);
         }
         unsigned wf[NT][4];                    // the weights as B operands: keys 8 u .. 8 u + 7 by rows
@@ -245,7 +277,7 @@ template <int HD, int NT, bool RUN> struct Stream {
             for (int u = 0; u < 4; u++)
 #pragma unroll
                 for (int j = 0; j < 2; j++) {
-                    float x = s[nt][u >> 1][(u & 1) * 2 + j] * row_scale[nt][j] * kf[u];
+                    float x = s[nt][u >> 1][(u & 1) * 2 + j] * kf[u] * row_scale[nt][j];
                     bool live = seen[u];
                     if constexpr (RUN) {
                         const int key = key0 + u * 8 + g8, pos = pos0 + nt * 8 + 2 * tg + j;
@@ -258,8 +290,12 @@ template <int HD, int NT, bool RUN> struct Stream {
                     ct[j] = fmaxf(ct[j], t[u][j]);
                 }
             // what is in use has been outgrown: the first chunk, and seldom after it
-            const bool far = cm[0] > m[nt][0] + LAG_SUM || cm[1] > m[nt][1] + LAG_SUM || ct[0] > top[nt][0] + LAG_TOP || ct[1] > top[nt][1] + LAG_TOP;
+            bool far = base[nt][0] != 0.f || base[nt][1] != 0.f;
+            far = far || cm[0] > m[nt][0] + LAG_SUM || cm[1] > m[nt][1] + LAG_SUM || ct[0] > top[nt][0] + LAG_TOP || ct[1] > top[nt][1] + LAG_TOP;
             if (__any_sync(0xffffffffu, far)) {
+                const float c0 = fabsf(fmaxf(m[nt][0], cm[0])), c1 = fabsf(fmaxf(m[nt][1], cm[1]));
+                const bool large = base[nt][0] != 0.f || base[nt][1] != 0.f || (c0 > FROM_ZERO && c0 < INFINITY) || (c1 > FROM_ZERO && c1 < INFINITY);
+                if (__any_sync(0xffffffffu, large)) rebase(nt, s, t, cm, ct, ve);
 #pragma unroll
                 for (int j = 0; j < 2; j++) {
                     cm[j] = fmaxf(m[nt][j], cm[j]);
@@ -312,6 +348,8 @@ template <int HD, int NT, bool RUN> struct Stream {
                 float most = m[nt][j];
 #pragma unroll
                 for (int off = 4; off < 32; off <<= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, off));
+                // by the base itself where there is one, as a large base plus a small number is not exact
+                if (base[nt][j] != 0.f) most = 0.f;
                 // a lane without a key counts 0; one whose keys are no numbers is NaN and stays it
                 float sum = l[nt][j] * (m[nt][j] == -INFINITY ? 0.f : exp2_fast(m[nt][j] - most));
 #pragma unroll
@@ -327,7 +365,7 @@ template <int HD, int NT, bool RUN> struct Stream {
                 const int r = nt * 8 + 2 * tg + j;
                 const float f = most == -INFINITY ? 1.f : exp2_fast(top[nt][j] - WEIGHT_TOP - most);
                 if (g8 == 0) {
-                    m_w[r] = most;
+                    m_w[r] = base[nt][j] + most;
                     l_w[r] = sum;
                 }
 #pragma unroll
@@ -380,14 +418,15 @@ __global__ void __launch_bounds__(THREADS) attn_run_kv8_kernel(const Params p) {
         if (threadIdx.x == 0) atomicOr(p.status, ESP_STATUS_BAD_INDEX);
         return;
     }
-    const int start = p.seq_start[seq], end = p.seq_start[seq + 1], past = p.seq_past[seq], head = blockIdx.y, kvh = head / (p.nh / p.nkv);
+    const int start = p.seq_start[seq], end = p.seq_start[seq + 1], head = blockIdx.y, kvh = head / (p.nh / p.nkv);
     // rows that the queries do not have are looked for first: only where there are none is end - start a number of rows
-    const bool there = start >= 0 && end >= start && end <= p.n_rows;
+    const bool there = (unsigned)start <= (unsigned)end && (unsigned)end <= (unsigned)p.n_rows;
     const int rows = there ? min(S::ROWS, end - start - first) : 0;
     if (rows <= 0) {                           // or behind the sequence's last token; a whole tile there is none
         if (threadIdx.x == 0 && first == tile_first) atomicOr(p.status, ESP_STATUS_BAD_INDEX);
         return;
     }
+    const int past = p.seq_past[seq];
     if (past < 0 || ((long long)past + first + rows - 1) / KV8_PAGE >= p.table_stride) {           // positions that the page table does not have
         if (threadIdx.x == 0) atomicOr(p.status, ESP_STATUS_BAD_INDEX);
         return;

@@ -758,6 +758,46 @@ def test_queries_that_are_no_numbers(hd, value):
     assert st.item() == 0 and torch.isnan(one.view(3, nh, hd)[:, 1]).all() and torch.isfinite(one.view(3, nh, hd)[:, 0]).all()
 
 
+def scores_of_one_channel(hd, length, amplitude, best, seed):
+    """Keys whose scores are amplitude / sqrt(hd) times 1 or 2: the largest are those of ``best`` (None: all the same).  (table, k, v, exps, query
+    row of one head, the values in 64 bits)."""
+    table, total = tables([length], 3)
+    k, v, exps = pools(total, 1, hd, seed)
+    k.view(torch.uint8).zero_()
+    k.view(torch.uint8)[..., 0] = 0x40 if best is None or amplitude < 0 else 0x38          # 2 and 1
+    exps[:, :, 0] = 127
+    if best is not None:
+        k.view(torch.uint8)[table[0, best // PAGE].long(), 0, best % PAGE, 0] = 0x38 if amplitude < 0 else 0x40
+    q = torch.zeros(hd, device="cuda", dtype=torch.bfloat16)
+    q[0] = amplitude
+    return table, k, v, exps, q, sequence_rows(v, exps, 1, table[0, :(length + PAGE - 1) // PAGE].long(), length)[0]
+
+
+@pytest.mark.parametrize("nh,hd", [(1, 64), (3, 128), (12, 128), (2, 192), (1, 256)])
+@pytest.mark.parametrize("amplitude", [1e3, 1e7, 3e8, 1e10, 1e15, 1e30, 3e38, -1e7, -1e10, -1e30])
+def test_scores_of_any_size(nh, hd, amplitude):
+    """The value of the one key whose score is far above the others, or the mean where all are the same, be the scores themselves beyond
+    what a value's exponent can be added to."""
+    length, new = 700, 30
+    for best in (5, 300, 660, None):
+        table, k, v, exps, row, values = scores_of_one_channel(hd, length, amplitude, best, 5)
+        q = row.repeat(new, nh)
+        one, st = torch.full_like(q, math.nan), status()
+        pos = torch.arange(length - new, length, dtype=torch.int32, device="cuda")
+        ops.attn_decode_kv8(q, k, v, exps, one, Workspace(q.device), ints([0] * new), pos, table, PAGE, nh, 1, hd, 0, st)
+        outs = [one]
+        if hd > 64:                                       # runs of few tokens and wide heads: the streaming kernel as well
+            outs.append(torch.full_like(q, math.nan))
+            ops.attn_prefill_kv8(q, k, v, exps, outs[-1], ints([0]), ints([0]), ints([0, new]), ints([length - new]), table, PAGE, nh, 1, hd, 0, st)
+        assert st.item() == 0
+        want = torch.stack([values[best] if best is not None else values[:p + 1].mean(0) for p in pos.tolist()])[:, None]
+        spread = torch.stack([values[best].abs() if best is not None else values[:p + 1].abs().mean(0) for p in pos.tolist()])[:, None]
+        for out in outs:
+            off = (out.double().view(new, nh, hd) - want).abs()
+            # the result's rounding; weights are halfs (2^-11), exp2 and sums are 32-bit
+            assert torch.all(off <= 2.0 ** -8 * want.abs() + 2.0 ** -10 * spread + 1e-30), (best, float(off.max()))
+
+
 # ------------------------------------------------------------------------------------------------------- together
 def test_pools_past_32_bits_of_bytes():
     """Pages whose codes lie more than 2^31 bytes into the pool."""
