@@ -7,6 +7,9 @@
 //   O += P V       tcgen05.mma, accumulated in tensor memory
 //
 // m is a whole number near the row's running maximum, which may have outgrown it by 2^LAZY: only then are O and the row's sum scaled anew.
+// Scores are good below 2^30 in units of log2: above it m, rounded to 32 bits, is off from the maximum by as much as a weight's exponent has
+// room for, and a row may be NaN.  (Rounding such scores first, behind a test of m for every 32 of them, cost 7 % of the ragged chunks
+// below; the streaming kernels have no such bound.)
 //
 // The cache's codes cannot be operands beside bfloat16 queries and weights, so eight warps turn them into bfloat16 on their way
 // from global to shared memory: a code's bits moved into a bfloat16's places are the code times 2^-120, subnormal codes
@@ -891,8 +894,8 @@ template <int HD> int launch(const CUtensorMap& map_q, Params p, int device, cud
     p.smem_bytes = (int)smem;
     // An item for each SM at most: singly.  Many: in pairs, and in all launches, as a tile is left to its neighbour, which another launch may
     // list.  Between the two the kernel looks at what the tiles see.  Tiles of sequences of few new tokens count although another kernel has
-    // them: looking there as well costs more than it gains (2,048 tokens beside 100 of one, 28 heads on 4, 252 us and 259 with a
-    // look; 700 behind 4,953 beside 60 of four, 32 on 8, 211 and 216; 100 of 33 beside 60 of one 214 and 233).
+    // them: looking there as well gains nothing (2,048 tokens beside 100 of one, 28 heads on 4, 257 us and 259 with a look; 1,000 beside
+    // 100 of one 233 and 231; 700 behind 4,953 beside 60 of four, 32 on 8, 215 and 216; 100 of 33 beside 60 of one 226 and 233).
     const long long all_items = (long long)p.n_tiles * p.nh;
     p.way = (short)(all_items <= sm_count[device] ? SINGLY : all_items >= 4LL * sm_count[device] || p.n_tiles > FEW ? IN_PAIRS : LOOK);
     for (int at = 0; at < p.n_tiles; at += LIST) {

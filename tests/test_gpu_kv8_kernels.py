@@ -798,6 +798,26 @@ def test_scores_of_any_size(nh, hd, amplitude):
             assert torch.all(off <= 2.0 ** -8 * want.abs() + 2.0 ** -10 * spread + 1e-30), (best, float(off.max()))
 
 
+@pytest.mark.parametrize("nh,hd,new", [(1, 64, 300), (3, 128, 140), (100, 64, 400), (2, 104, 40)])
+@pytest.mark.parametrize("amplitude", [1e3, 1e7, 3e8, 2e9, -1e7, -2e9])
+def test_scores_of_prompts_below_their_bound(nh, hd, new, amplitude):
+    """The same of the tensor-memory kernel, for scores of up to 2^29 in units of log2."""
+    length = 700
+    for best in (5, 150, None):
+        table, k, v, exps, row, values = scores_of_one_channel(hd, length, amplitude, best, 5)
+        q, st = row.repeat(new, nh), status()
+        out = torch.full_like(q, math.nan)
+        firsts = list(range(0, new, 128))
+        ops.attn_prefill_kv8(q, k, v, exps, out, ints([0] * len(firsts)), ints(firsts), ints([0, new]), ints([length - new]), table, PAGE, nh, 1, hd, 0, st)
+        assert st.item() == 0
+        pos = range(length - new, length)
+        want = torch.stack([values[best] if best is not None else values[:p + 1].mean(0) for p in pos])[:, None]
+        spread = torch.stack([values[best].abs() if best is not None else values[:p + 1].abs().mean(0) for p in pos])[:, None]
+        off = (out.double().view(new, nh, hd) - want).abs()
+        # the result's rounding; weights are bfloat16 (2^-8), exp2 and sums are 32-bit
+        assert torch.all(off <= 2.0 ** -8 * want.abs() + (2.0 ** -8 + 2.0 ** -20) * (1 + 2.0 ** -8) * spread + 1e-30), (best, float(off.max()))
+
+
 # ------------------------------------------------------------------------------------------------------- together
 def test_pools_past_32_bits_of_bytes():
     """Pages whose codes lie more than 2^31 bytes into the pool."""
