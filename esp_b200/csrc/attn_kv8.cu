@@ -24,8 +24,8 @@
 // Sums, maxima and accumulators are 32-bit.  Weights and values far apart are held in this form; a warp leaves its result by the maximum of
 // the scores alone, which may lag by 2^LAG_SUM, and moves that where large values' sums would pass 32-bit's range.
 //
-// Measured (B200, one launch behind another): 8 sequences of 4,096 keys, 16 heads of 128, 30.5 us for 135 MB; 64 ragged ones of
-// up to 8,192, 28 heads on 4, 51 us for 231 MB; one of 131,071 34 us; one of 777 7.4 us.  The keys stream at the memory's rate
+// Measured (B200, one launch behind another): 8 sequences of 4,096 keys, 16 heads of 128, 30.7 us for 135 MB; 64 ragged ones of
+// up to 8,192, 28 heads on 4, 52 us for 231 MB; one of 131,071 34 us; one of 777 7.4 us.  The keys stream at the memory's rate
 // (18 of the 30 us); of the rest a block's start takes 2.7 us (from the wait to its first chunk) and the joining of parts about 4 us
 // a level (a fence, a count, two trips to L2); about 5 us are not accounted for, as every block has 13 or 14 units.  A grid of (row, head,
 // split) blocks of one split length took 29.4, 86, 42.5 and 8.9 us, with the best length of each case 29.3, 60, 41 and 8.2.  Three blocks an
@@ -40,7 +40,7 @@ constexpr int THREADS = 128, WARPS = 4, CHUNK = 32, UNIT = WARPS * CHUNK, MAX_RO
 constexpr float WEIGHT_TOP = 6.f, LAG_TOP = 8.f, LAG_SUM = 40.f, RISE = 60.f;
 // A value's exponent is added to its score, and above 2^24 a score has no place for it: scores whose maximum is this far from zero, or from the
 // base they are counted from, are counted from that maximum.  (The place where that is looked for and done is seldom come to, but costs what it
-// takes of registers and instructions: decode up to 1 %, sequences of few new tokens 2 %.  Scores counted from the row's maximum throughout,
+// takes of registers and instructions: decode up to 1 %, sequences of few new tokens 2 %, prompts with wide heads more.  Scores counted from the row's maximum throughout,
 // without a base: decode with sixteen rows a block 4 to 7 %, few new tokens 3 %.)
 constexpr float FROM_ZERO = 1 << 20, FROM_BASE = 32.f;
 constexpr int PARTS = 16;                      // of a pair, that one block joins
@@ -401,8 +401,8 @@ __device__ __forceinline__ float inverse(float sum) { return sum == 0.f ? 0.f : 
 __device__ __forceinline__ void store_pair(bf16* to, float a, float b) { *reinterpret_cast<__nv_bfloat162*>(to) = __floats2bfloat162_rn(a, b); }
 
 // ---------------------------------------------------------------------------------------------------- sixteen tokens of a run
-// Bound by its instructions: every block of sixteen tokens converts the keys that they see.  2,048 tokens: 16 heads of 192 231 us (two
-// blocks an SM; padded to 256 channels, one block, 400), 8 of 256 214 us, 74 and 80 TFLOP/s.
+// Bound by its instructions: every block of sixteen tokens converts the keys that they see.  2,048 tokens: 16 heads of 192 250 us (two
+// blocks an SM; padded to 256 channels, one block, 400), 8 of 256 240 us, 103 and 72 TFLOP/s.
 template <int HD, int NT>
 __global__ void __launch_bounds__(THREADS) attn_run_kv8_kernel(const Params p) {
     pdl_trigger();

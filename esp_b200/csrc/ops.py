@@ -1730,8 +1730,8 @@ def attn_prefill_kv8(q, k, v, exps, out, tile_seq, tile_first, seq_start, seq_pa
     after = (_ptr(status, torch.int32, "status"), _stream())
     # Scores and weighted values in tensor memory, or (wide heads) the streaming kernel, sixteen rows a block.  That one also takes
     # the sequences of few new tokens, where tiles of 128 are mostly empty: 6 sequences behind 3,442 keys, 32 heads of 128 on 16, of 16
-    # new tokens 63 us for 108, of 32 95 for 110 (48 would take 112 for 111); 16 behind 2,000, 28 heads on 4, of 16 75 for 118, of 32 122
-    # for 118; heads of 64 gain nothing (19 and 18 us).  (The engine sends steps of at most 128 rows to the decode kernel as a whole.)  Steps whose tiles are half full on average are left to the first kernel
+    # new tokens 65 us for 114, of 32 99 for 115 (48 would take 119 for 115); 16 behind 2,000, 28 heads on 4, of 16 79 for 122, of 32 131
+    # for 124; heads of 64 gain nothing (19 and 18 us).  (The engine sends steps of at most 128 rows to the decode kernel as a whole.)  Steps whose tiles are half full on average are left to the first kernel
     # as a whole.
     few = KV8_FEW_TOKENS if 64 < hd <= 128 and n * 2 < n_tiles * ATTN_TC05_TILE_ROWS else 0
     if hd <= 128 and (n > few or not few):
