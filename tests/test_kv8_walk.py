@@ -33,7 +33,7 @@ struct Meeting {
             c.notify_all();
             return said;
         }
-        if (!c.wait_for(lock, std::chrono::seconds(5), [&] { return turn != mine; })) {
+        if (!c.wait_for(lock, std::chrono::seconds(30), [&] { return turn != mine; })) {
             std::printf("a meeting of %d waits for %d\n", count, count - here);
             std::fflush(stdout);
             std::_Exit(1);
